@@ -216,6 +216,111 @@ int kq_run_ffn(kq_ctx *ctx, const kq_weight *gate, const kq_weight *up, const kq
 int kq_run_ffn_async(kq_ctx *ctx, const kq_weight *gate, const kq_weight *up, const kq_weight *down,
                      int batch_len, const uint16_t *x_in_dev, const uint16_t *gamma_dev, uint16_t *x_out_dev);
 
+/* ---------------------------------------------------------------- attention over a paged cache
+ *
+ * What stands between the q / k / v products and the o product of a layer: per-head norms and the
+ * position rotation, the append to a paged key-value cache, and attention over that cache -- of one
+ * new token per sequence (decode) or of ragged prompt rows (prefill).  fp16 in and out; sums,
+ * softmax statistics and norms in fp32, rotation angles reduced in fp64, one rounding to fp16 of
+ * each result.  DEVICE pointers, enqueued on the context's stream; all buffers belong to the caller
+ * and to the context's device.  No counterpart on the reference's matmul path: its attention is
+ * ENG:7787-7915 (QK-norm, RoPE, active-window GQA).
+ *
+ * Rows of heads: fp16, one head's head_dim values after another, rows `stride` elements apart
+ * (stride >= heads * head_dim, a multiple of 8; the address a multiple of 16 bytes), so that q, k
+ * and v can be views into one buffer.  head_dim is 64, 128 or 256. */
+#define KQ_MAX_HEAD_DIM 256
+#define KQ_MAX_HEADS 256         /* heads of a row */
+#define KQ_MAX_GROUP 16          /* query heads that share a key head */
+#define KQ_MAX_SEQS 4096
+#define KQ_ROPE_HALF 0           /* pairs (j, j + rot_dim/2) turn together */
+#define KQ_ROPE_ADJACENT 1       /* pairs (2j, 2j + 1) */
+
+/* The position rotation: pair j of a head at position p turns by p * inv_freq[j] radians; values
+ * from rot_dim on pass unchanged.  A plain value: fill it with kq_rope_init and, for a scaled
+ * variant, change inv_freq. */
+typedef struct kq_rope {
+    int rot_dim;                              /* a multiple of 16, <= head_dim; 0: no rotation */
+    int style;                                /* KQ_ROPE_HALF or KQ_ROPE_ADJACENT */
+    double inv_freq[KQ_MAX_HEAD_DIM / 2];
+} kq_rope;
+/* inv_freq[j] = base^(-2j / rot_dim) */
+int kq_rope_init(kq_rope *out, int rot_dim, int style, double base);
+
+/* Keys and values in pages of page_size positions.  Position p of sequence s lies in page
+ * page_table[s * table_stride + p / page_size], slot p % page_size; a page holds, for each key
+ * head, page_size rows of head_dim values.  The table is read on the device when a call runs;
+ * entries that no visible position needs may hold anything.  An entry that is needed and names no
+ * page ([0, n_pages)) is not followed: the position counts as masked (or is not written) and the
+ * next kq_synchronize reports KQ_ERR_SHAPE. */
+typedef struct kq_kv_cache {
+    uint16_t *k, *v;            /* fp16 [n_pages][kv_heads][page_size][head_dim], 16-byte aligned */
+    const int32_t *page_table;  /* [n_seqs][table_stride] */
+    int n_pages;
+    int page_size;              /* a power of two, 16..256 */
+    int kv_heads;
+    int head_dim;
+    int n_seqs;                 /* 1..KQ_MAX_SEQS */
+    int table_stride;           /* table entries per sequence */
+} kq_kv_cache;
+
+/* One set of heads of M rows: in -> out (the same buffer and stride, or one that does not
+ * overlap).  gamma (fp16 [head_dim], or NULL for no norm) scales the RMS-normed head:
+ * x * gamma / sqrt(mean(x^2) + eps). */
+typedef struct kq_heads {
+    const uint16_t *in;
+    size_t in_stride;
+    uint16_t *out;
+    size_t out_stride;
+    int heads;
+    const uint16_t *gamma;
+} kq_heads;
+
+/* Norm of every head (where gamma is given), then the rotation (where rope is given and its
+ * rot_dim is not 0) by the row's position pos_dev[row] (int32, may be NULL without a rotation), in
+ * one pass over M (0..KQ_MAX_M) rows of q and/or k (either may be NULL). */
+int kq_qk_norm_rope_async(kq_ctx *ctx, const kq_rope *rope, int head_dim, int M, const int32_t *pos_dev,
+                          const kq_heads *q, const kq_heads *k, float eps);
+
+/* Row i's keys and values go to position pos_dev[i] of sequence seq_dev[i] (int32 each), the keys
+ * normed and rotated on the way as above, the values as they are; q (may be NULL) is normed and
+ * rotated like kq_qk_norm_rope_async in the same launch.  k->heads = v->heads = cache->kv_heads;
+ * k->out and v->out are NULL, v->gamma too.  A row with seq_dev[i] < 0 is padding: nothing of it is
+ * read or written.  A row whose sequence, position or page lies outside the cache is left out in the
+ * same way (q included) and the next kq_synchronize reports KQ_ERR_SHAPE.  No two rows of a call
+ * may name the same position of the same page. */
+int kq_kv_append_async(kq_ctx *ctx, const kq_kv_cache *cache, const kq_rope *rope, int M, const int32_t *seq_dev,
+                       const int32_t *pos_dev, const kq_heads *q, const kq_heads *k, const kq_heads *v, float eps);
+
+/* Attention of query rows over the cache: out = sum_j softmax_j(scale * q . k_j) v_j over the keys
+ * that the row sees; query head h reads key head h / (heads / kv_heads).  A row at position p sees
+ * key j when 0 <= j <= p and, with a window, j > p - window or j < sinks (the first tokens stay
+ * visible).  A row that sees no key gets zeros.  Keys that a row does not see have no effect on it,
+ * whatever they hold.  Lengths past the table's reach count as its reach, negative ones as 0, and
+ * the next kq_synchronize reports KQ_ERR_SHAPE. */
+typedef struct kq_attn {
+    const uint16_t *q;          /* rows of heads * head_dim, after norm and rotation */
+    size_t q_stride;
+    uint16_t *out;              /* the same shape; may not overlap q or the cache */
+    size_t out_stride;
+    int heads;                  /* a multiple of kv_heads, at most KQ_MAX_GROUP times it */
+    int M;                      /* rows of q and out (0..KQ_MAX_M) */
+    const int32_t *kv_len;      /* [n_seqs] keys of each sequence, the new tokens' among them */
+    const int32_t *q_start;     /* prefill: [n_seqs + 1] first row of each sequence; decode: unused */
+    int window;                 /* keys that a row sees, its own among them; 0: all */
+    int sinks;                  /* first positions visible besides the window; 0 without a window */
+    float scale;                /* 0: 1 / sqrt(head_dim) */
+} kq_attn;
+/* One new token per sequence: row s is sequence s at position kv_len[s] - 1 (M = n_seqs).  The keys
+ * of all sequences are split evenly over the GPU and the parts joined in the same launch, in a
+ * fixed order: the result does not change from run to run. */
+int kq_attn_decode_async(kq_ctx *ctx, const kq_kv_cache *cache, const kq_attn *a);
+/* Rows [q_start[s], q_start[s+1]) are sequence s's last tokens: with n of them the i-th stands at
+ * position kv_len[s] - n + i (a negative one sees nothing).  q_start must not decrease and end at
+ * or below M (else the sequence counts as having no rows, and KQ_ERR_SHAPE); rows outside the
+ * sequences are left as they were. */
+int kq_attn_prefill_async(kq_ctx *ctx, const kq_kv_cache *cache, const kq_attn *a);
+
 /* ---------------------------------------------------------------- LM head */
 
 /* Full-vocabulary LM head over M normalised fp16 rows x [M][K]: logits (fp16 [M][rows], may be

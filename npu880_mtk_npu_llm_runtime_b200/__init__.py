@@ -45,6 +45,7 @@ EXPORTS = (
     "kq_sdot_row_batch", "kq_eval_single_lm_row_dot", "kq_debug_block_sums_async",
     "kq_rmsnorm_fp16_rows", "kq_swiglu_fp16_rows", "kq_rmsnorm_q8k_async", "kq_swiglu_q8k_async",
     "kq_run_ffn", "kq_run_ffn_async",
+    "kq_rope_init", "kq_qk_norm_rope_async", "kq_kv_append_async", "kq_attn_decode_async", "kq_attn_prefill_async",
     "kq_lm_head_argmax", "kq_lm_head_argmax_async", "kq_lm_head_argmax_noalloc", "kq_eval_indexed_rows_argmax",
     "kq_dequant_rows", "kq_dequant_rows_async", "kq_embed_rows", "kq_embed_rows_async",
     "kq_gguf_open", "kq_gguf_open_memory", "kq_gguf_close", "kq_gguf_info", "kq_gguf_tensor_count",
@@ -84,6 +85,31 @@ class Task(C.Structure):
         ("residual", C.c_void_p), ("res_stride", C.c_size_t),
         ("dst_f32", C.c_void_p), ("dst_f32_stride", C.c_size_t),
     ]
+
+
+class RopeStruct(C.Structure):
+    """kq_rope: the position rotation's pairs and their radians per position."""
+    _fields_ = [("rot_dim", C.c_int), ("style", C.c_int), ("inv_freq", C.c_double * 128)]
+
+
+class KvCacheStruct(C.Structure):
+    """kq_kv_cache: pages of keys and values and the table that maps positions to them."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_table", C.c_void_p), ("n_pages", C.c_int),
+                ("page_size", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("n_seqs", C.c_int),
+                ("table_stride", C.c_int)]
+
+
+class HeadsStruct(C.Structure):
+    """kq_heads: one set of heads of the rows of a call."""
+    _fields_ = [("in_", C.c_void_p), ("in_stride", C.c_size_t), ("out", C.c_void_p), ("out_stride", C.c_size_t),
+                ("heads", C.c_int), ("gamma", C.c_void_p)]
+
+
+class AttnStruct(C.Structure):
+    """kq_attn: the query rows of an attention call and what they see."""
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_size_t), ("out", C.c_void_p), ("out_stride", C.c_size_t),
+                ("heads", C.c_int), ("M", C.c_int), ("kv_len", C.c_void_p), ("q_start", C.c_void_p),
+                ("window", C.c_int), ("sinks", C.c_int), ("scale", C.c_float)]
 
 
 _vp, _i, _u32, _sz, _u64 = C.c_void_p, C.c_int, C.c_uint32, C.c_size_t, C.c_uint64
@@ -129,6 +155,11 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "kq_swiglu_q8k_async": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
         "kq_run_ffn": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp]),
         "kq_run_ffn_async": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp]),
+        "kq_rope_init": (_i, [_vp, _i, _i, C.c_double]),
+        "kq_qk_norm_rope_async": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, C.c_float]),
+        "kq_kv_append_async": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, C.c_float]),
+        "kq_attn_decode_async": (_i, [_vp, _vp, _vp]),
+        "kq_attn_prefill_async": (_i, [_vp, _vp, _vp]),
         "kq_lm_head_argmax": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp]),
         "kq_lm_head_argmax_async": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
         "kq_lm_head_argmax_noalloc": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp]),
@@ -181,6 +212,111 @@ def _dp(t):
     if t is None:
         return None
     return t.data_ptr()
+
+
+def _rows(t, what: str, heads: int):
+    """(pointer, row stride, head size, rows) of an fp16 tensor [rows, heads * head_dim] (or [rows,
+    heads, head_dim]) whose rows may lie apart"""
+    import torch
+    if t.dtype != torch.float16 or t.dim() not in (2, 3) or not t.is_cuda:
+        raise ValueError(f"{what}: a 2- or 3-dimensional fp16 CUDA tensor is needed")
+    if t.dim() == 3 and (t.shape[1] != heads or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+        raise ValueError(f"{what}: [rows, heads, head_dim] with the heads of a row side by side is needed")
+    width = t.shape[1] if t.dim() == 2 else t.shape[1] * t.shape[2]
+    if t.stride(-1) != 1 or heads < 1 or width % heads:
+        raise ValueError(f"{what}: rows of {heads} heads with values side by side are needed")
+    stride = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    return t.data_ptr(), stride, width // heads, t.shape[0]
+
+
+def _ints(t, what: str, n: int | None = None):
+    import torch
+    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{what}: a contiguous int32 CUDA tensor" + ("" if n is None else f" of {n}") + " is needed")
+    return t.data_ptr()
+
+
+class Rope:
+    """kq_rope: pair j turns by position * inv_freq[j] radians; `inv_freq` (a list) replaces
+    base ** (-2j / rot_dim)."""
+
+    STYLES = {"half": 0, "adjacent": 1}
+
+    def __init__(self, rot_dim: int, base: float = 1e4, style: str = "half", inv_freq=None):
+        self.struct = RopeStruct()
+        st = load_library().kq_rope_init(C.addressof(self.struct), rot_dim, self.STYLES[style], base)
+        if st != 0:
+            raise KQError(st, f"rope of {rot_dim} values, base {base}")
+        if inv_freq is not None:
+            if len(inv_freq) != rot_dim // 2:
+                raise ValueError(f"inv_freq: {rot_dim // 2} values are needed")
+            for j, f in enumerate(inv_freq):
+                self.struct.inv_freq[j] = float(f)
+        self.ref = C.addressof(self.struct)
+
+
+class KvCache:
+    """kq_kv_cache over the caller's tensors: k, v fp16 [pages, kv_heads, page_size, head_dim], page_table
+    int32 [sequences, pages of a sequence].  Keeps them alive; the table is read when a call runs."""
+
+    def __init__(self, k, v, page_table):
+        import torch
+        for t, what in ((k, "k"), (v, "v")):
+            if t.dtype != torch.float16 or not t.is_cuda or t.dim() != 4 or not t.is_contiguous():
+                raise ValueError(f"{what}: a contiguous fp16 CUDA tensor [pages, kv_heads, page_size, head_dim] is needed")
+        if k.shape != v.shape or k.device != v.device or page_table.dim() != 2 or page_table.device != k.device:
+            raise ValueError("k and v must have one shape, and the table two dimensions, on one device")
+        self.k, self.v, self.page_table, self.device = k, v, page_table, k.device
+        s = self.struct = KvCacheStruct()
+        s.k, s.v, s.page_table = k.data_ptr(), v.data_ptr(), _ints(page_table, "page_table")
+        s.n_pages, s.kv_heads, s.page_size, s.head_dim = k.shape
+        s.n_seqs, s.table_stride = page_table.shape
+        self.ref = C.addressof(s)
+
+
+class Heads:
+    """kq_heads over the caller's tensors: rows of `heads` heads (views with a row stride are fine)."""
+
+    def __init__(self, x, heads: int, gamma=None, out=None):
+        import torch
+        s = self.struct = HeadsStruct()
+        s.in_, s.in_stride, self.head_dim, self.rows = _rows(x, "rows", heads)
+        s.heads = heads
+        if out is not None:
+            s.out, s.out_stride, dim, rows = _rows(out, "out", heads)
+            if (dim, rows) != (self.head_dim, self.rows):
+                raise ValueError("out must have the rows' shape")
+        if gamma is not None:
+            if gamma.dtype != torch.float16 or gamma.numel() != self.head_dim or not gamma.is_contiguous():
+                raise ValueError(f"gamma: {self.head_dim} fp16 values side by side are needed")
+            s.gamma = gamma.data_ptr()
+        for t in (out, gamma):
+            if t is not None and t.device != x.device:
+                raise ValueError("rows, out and gamma must be on one device")
+        self.device, self.keep, self.ref = x.device, (x, out, gamma), C.addressof(s)
+
+
+class Attention:
+    """kq_attn over the caller's tensors: query rows over a KvCache.  One row per sequence (decode), or with
+    q_start [sequences + 1] the sequences' last rows (prefill)."""
+
+    def __init__(self, cache: KvCache, q, out, kv_len, q_start=None, heads: int | None = None, window: int = 0,
+                 sinks: int = 0, scale: float = 0.0):
+        dim = cache.struct.head_dim
+        heads = heads or (q.shape[1] if q.dim() == 3 else q.shape[1] // dim)
+        s = self.struct = AttnStruct()
+        s.q, s.q_stride, qd, s.M = _rows(q, "q", heads)
+        s.out, s.out_stride, od, om = _rows(out, "out", heads)
+        if (qd, od, om) != (dim, dim, s.M):
+            raise ValueError(f"q and out must have the same rows of {heads} heads of {dim}")
+        s.heads, s.window, s.sinks, s.scale = heads, window, sinks, scale
+        s.kv_len = _ints(kv_len, "kv_len", cache.struct.n_seqs)
+        if q_start is not None:
+            s.q_start = _ints(q_start, "q_start", cache.struct.n_seqs + 1)
+        for t in (q, out, kv_len, q_start):
+            if t is not None and t.device != cache.device:
+                raise ValueError("q, out, kv_len and q_start must be on the cache's device")
+        self.cache, self.keep, self.ref = cache, (q, out, kv_len, q_start), C.addressof(s)
 
 
 class Weight:
@@ -404,6 +540,45 @@ class Context:
     def run_ffn_async(self, gate: Weight, up: Weight, down: Weight, M: int, x_dev, gamma_dev, out_dev):
         self.check(self.L.kq_run_ffn_async(self.handle, gate.handle, up.handle, down.handle, M, _dp(x_dev),
                                            _dp(gamma_dev), _dp(out_dev)))
+
+    # ---- attention over a paged cache (kq_rope, kq_kv_cache, kq_heads, kq_attn)
+    def _here(self, *objects):
+        for o in objects:
+            if o is not None and o.device.index != self.device:
+                raise ValueError(f"a tensor lives on {o.device}, the context on device {self.device}")
+
+    def qk_norm_rope_async(self, rope: Rope | None, pos, q: Heads | None, k: Heads | None = None, eps: float = 1e-6):
+        """per-head norm and rotation of q and k rows into their `out` in one launch"""
+        h = q or k
+        if h is None:
+            raise ValueError("q or k rows are needed")
+        if q is not None and k is not None and (q.rows, q.head_dim) != (k.rows, k.head_dim):
+            raise ValueError("q and k must have the same rows and head size")
+        self._here(q, k, pos)
+        p = None if pos is None else _ints(pos, "positions", h.rows)
+        self.check(self.L.kq_qk_norm_rope_async(self.handle, rope and rope.ref, h.head_dim, h.rows, p, q and q.ref,
+                                                k and k.ref, eps))
+
+    def kv_append_async(self, cache: KvCache, rope: Rope | None, seq, pos, k: Heads, v: Heads, q: Heads | None = None,
+                        eps: float = 1e-6):
+        """row i's key (normed, rotated) and value to position pos[i] of sequence seq[i]; q into its `out`"""
+        for h in (k, v, q):
+            if h is not None and (h.rows, h.head_dim) != (k.rows, cache.struct.head_dim):
+                raise ValueError("q, k and v must have the same rows and the cache's head size")
+        self._here(cache, k, v, q, seq, pos)
+        self.check(self.L.kq_kv_append_async(self.handle, cache.ref, rope and rope.ref, k.rows,
+                                             _ints(seq, "sequences", k.rows), _ints(pos, "positions", k.rows),
+                                             q and q.ref, k.ref, v.ref, eps))
+
+    def attn_decode_async(self, a: Attention):
+        """attention of one new token per sequence"""
+        self._here(a.cache)
+        self.check(self.L.kq_attn_decode_async(self.handle, a.cache.ref, a.ref))
+
+    def attn_prefill_async(self, a: Attention):
+        """attention of the sequences' last rows (a.q_start)"""
+        self._here(a.cache)
+        self.check(self.L.kq_attn_prefill_async(self.handle, a.cache.ref, a.ref))
 
     # ---- several GPUs: the gather in the LM head GEMV (kq_peer_*, kq_gemm_peer_gather_async)
     def peer_region_bytes(self, M: int, row_stride: int) -> int:

@@ -4,11 +4,13 @@
 // pool, src/v182_r22_breakthrough_engine.c:3442-4262): argument validation, the
 // pre-quantized-input state, host<->device staging for the host-pointer entry points, and
 // the grouping of tasks into kernel launches.
+#include "kq_attn.h"
 #include "kq_common.cuh"
 #include "kq_internal.h"
 #include "../../include/kq.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -134,6 +136,8 @@ int check_device_status(kq_ctx *c) {
     c->split_dirty = true;  // a kernel that stopped early may have left arrival counts behind
     if (st == kq::DEV_ERR_TIMEOUT) return fail(c, KQ_ERR_TIMEOUT, "a device-side wait timed out");
     if (st == kq::DEV_ERR_INDEX) return fail(c, KQ_ERR_SHAPE, "a row id is past the end of the weight");
+    if (st == kq::DEV_ERR_CACHE)
+        return fail(c, KQ_ERR_SHAPE, "a sequence, position, length, row range or page lies outside the key-value cache");
     return fail(c, KQ_ERR_CUDA, "device error code %d", st);
 }
 
@@ -1101,6 +1105,146 @@ extern "C" int kq_embed_rows(kq_ctx *c, const kq_weight *w, const uint32_t *ids,
     if (int r = kq_embed_rows_async(c, w, dids, n, dout)) return r;
     KQ_CUDA(c, cudaMemcpyAsync(dst, dout, ob, cudaMemcpyDeviceToHost, c->stream));
     return sync_and_check(c);
+}
+
+// =================================================================== attention over a paged cache
+
+extern "C" int kq_rope_init(kq_rope *out, int rot_dim, int style, double base) {
+    if (!out || (style != KQ_ROPE_HALF && style != KQ_ROPE_ADJACENT)) return KQ_ERR_INVALID_ARGUMENT;
+    if (rot_dim < 0 || rot_dim > KQ_MAX_HEAD_DIM || rot_dim % 16 || !(base > 0.0) || std::isinf(base)) return KQ_ERR_SHAPE;
+    *out = kq_rope{};
+    out->rot_dim = rot_dim;
+    out->style = style;
+    for (int j = 0; j < rot_dim / 2; ++j) out->inv_freq[j] = std::pow(base, -2.0 * j / rot_dim);
+    return KQ_OK;
+}
+
+namespace {
+
+kq::KvView kv_view(const kq_kv_cache *c) {
+    kq::KvView v{};
+    v.k = c->k;
+    v.v = c->v;
+    v.table = c->page_table;
+    v.n_pages = c->n_pages;
+    while ((1 << v.page_shift) < c->page_size) ++v.page_shift;
+    v.kv_heads = c->kv_heads;
+    v.head_dim = c->head_dim;
+    v.n_seqs = c->n_seqs;
+    v.table_stride = c->table_stride;
+    return v;
+}
+
+// The context's device while a call launches, the caller's afterwards.
+struct OnDevice {
+    int prev = -1;
+    explicit OnDevice(int device) {
+        if (cudaGetDevice(&prev) != cudaSuccess || prev == device) prev = -1;
+        if (prev >= 0) cudaSetDevice(device);
+    }
+    ~OnDevice() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+// the description that both attention calls launch from
+int attn_launch(kq_ctx *c, const kq_kv_cache *cache, const kq_attn *a, bool prefill, kq::AttnLaunch &L) {
+    if (!c) return KQ_ERR_INVALID_ARGUMENT;
+    const char *why = "";
+    if (int r = kq::check_attn(cache, a, prefill, &why)) return fail(c, r, "%s", why);
+    L.cache = kv_view(cache);
+    L.q = a->q;
+    L.q_stride = (long long)a->q_stride;
+    L.out = a->out;
+    L.out_stride = (long long)a->out_stride;
+    L.heads = a->heads;
+    L.M = a->M;
+    L.kv_len = a->kv_len;
+    L.q_start = prefill ? a->q_start : nullptr;
+    L.window = a->window;
+    L.sinks = a->sinks;
+    L.scale = a->scale > 0.0f ? a->scale : 1.0f / std::sqrt((float)cache->head_dim);
+    L.status = c->d_status;
+    L.num_sms = c->num_sms;
+    L.pdl = c->pdl;
+    return KQ_OK;
+}
+
+}  // namespace
+
+extern "C" int kq_qk_norm_rope_async(kq_ctx *c, const kq_rope *rope, int head_dim, int M, const int32_t *pos,
+                                     const kq_heads *q, const kq_heads *k, float eps) {
+    if (!c) return KQ_ERR_INVALID_ARGUMENT;
+    const char *why = "";
+    int r = kq::check_head_dim(head_dim, &why);
+    if (!r) r = kq::check_rope(rope, head_dim, &why);
+    if (!r) r = kq::check_rows(M, &why);
+    for (const kq_heads *h : {q, k})
+        if (!r && h && M > 0) r = kq::check_heads(h, head_dim, 1, &why);
+    if (r) return fail(c, r, "%s", why);
+    if (rope && rope->rot_dim > 0 && !pos) return fail(c, KQ_ERR_INVALID_ARGUMENT, "positions are NULL");
+    if (!(eps >= 0.0f)) return fail(c, KQ_ERR_INVALID_ARGUMENT, "eps must not be negative");
+    if (M == 0 || (!q && !k)) return KQ_OK;
+    const OnDevice on(c->device);
+    kq::RopeLaunch L{};
+    L.q = q;
+    L.k = k;
+    L.rope = rope;
+    L.head_dim = head_dim;
+    L.M = M;
+    L.pos = pos;
+    L.eps = eps;
+    L.status = c->d_status;
+    L.num_sms = c->num_sms;
+    L.pdl = c->pdl;
+    KQ_CUDA(c, kq::launch_norm_rope(L, c->stream));
+    return KQ_OK;
+}
+
+extern "C" int kq_kv_append_async(kq_ctx *c, const kq_kv_cache *cache, const kq_rope *rope, int M, const int32_t *seq,
+                                  const int32_t *pos, const kq_heads *q, const kq_heads *k, const kq_heads *v,
+                                  float eps) {
+    if (!c) return KQ_ERR_INVALID_ARGUMENT;
+    const char *why = "";
+    if (int r = kq::check_append(cache, rope, M, seq, pos, q, k, v, &why)) return fail(c, r, "%s", why);
+    if (!(eps >= 0.0f)) return fail(c, KQ_ERR_INVALID_ARGUMENT, "eps must not be negative");
+    if (M == 0) return KQ_OK;
+    const OnDevice on(c->device);
+    const kq::KvView view = kv_view(cache);
+    kq::RopeLaunch L{};
+    L.q = q;
+    L.k = k;
+    L.v = v;
+    L.cache = &view;
+    L.rope = rope;
+    L.head_dim = cache->head_dim;
+    L.M = M;
+    L.seq = seq;
+    L.pos = pos;
+    L.eps = eps;
+    L.status = c->d_status;
+    L.num_sms = c->num_sms;
+    L.pdl = c->pdl;
+    KQ_CUDA(c, kq::launch_norm_rope(L, c->stream));
+    return KQ_OK;
+}
+
+extern "C" int kq_attn_decode_async(kq_ctx *c, const kq_kv_cache *cache, const kq_attn *a) {
+    kq::AttnLaunch L{};
+    if (int r = attn_launch(c, cache, a, false, L)) return r;
+    if (L.M == 0) return KQ_OK;
+    const OnDevice on(c->device);
+    KQ_CUDA(c, kq::launch_attn_rows(L, c->stream));
+    return KQ_OK;
+}
+
+extern "C" int kq_attn_prefill_async(kq_ctx *c, const kq_kv_cache *cache, const kq_attn *a) {
+    kq::AttnLaunch L{};
+    if (int r = attn_launch(c, cache, a, true, L)) return r;
+    if (L.M == 0) return KQ_OK;
+    const OnDevice on(c->device);
+    KQ_CUDA(c, kq::launch_attn_rows(L, c->stream));
+    return KQ_OK;
 }
 
 // =================================================================== LM head

@@ -28,6 +28,7 @@ constexpr int TYPE_Q6_K = 14;
 constexpr int DEV_OK = 0;
 constexpr int DEV_ERR_TIMEOUT = 1;
 constexpr int DEV_ERR_INDEX = 2;  // a row id past the end of a weight (the access was skipped)
+constexpr int DEV_ERR_CACHE = 3;  // a sequence, position, length, row range or page outside the key-value cache
 
 // BlockQ8K of the reference (ENG:868-872): 292 bytes
 struct BlockQ8K {
