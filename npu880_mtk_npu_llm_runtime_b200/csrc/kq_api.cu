@@ -43,6 +43,7 @@ struct kq_ctx {
 
     // scratch (grown on demand, freed at destroy)
     DevBuf x, res, out16, out32, q8k_pending, q8k_cur, q80_cur, tmp, misc, keys, tcpack, tcterms;
+    DevBuf attn_parts, attn_count;  // attention: parts of shared rows, arrival counts (zero between launches)
     DevBuf lmlogits;  // fp16 logits of a many-token LM head when the caller keeps none
     // balanced GEMV launches: shared-row-group term slots and arrival counts (zero between
     // launches; re-cleared after a launch that stopped early)
@@ -499,7 +500,7 @@ extern "C" int kq_destroy(kq_ctx *c) {
     cudaSetDevice(c->device);
     cudaStreamSynchronize(c->stream);
     for (DevBuf *b : {&c->x, &c->res, &c->out16, &c->out32, &c->q8k_pending, &c->q8k_cur, &c->q80_cur, &c->tmp,
-                      &c->misc, &c->keys, &c->tcpack, &c->tcterms, &c->gsplit, &c->gcount, &c->lmlogits})
+                      &c->misc, &c->keys, &c->tcpack, &c->tcterms, &c->gsplit, &c->gcount, &c->lmlogits, &c->attn_parts, &c->attn_count})
         if (b->p) cudaFree(b->p);
     cudaFree(c->exp_tab);
     cudaFreeHost(c->h_status);
@@ -1147,6 +1148,17 @@ struct OnDevice {
     }
 };
 
+// Scratch of the attention kernels: one size for all shapes, so that it never grows after the first call.
+int attn_scratch(kq_ctx *c, kq::AttnLaunch &L) {
+    if (int r = ensure(c, c->attn_parts, kq::attn_decode_part_bytes(c->num_sms))) return r;
+    const bool fresh = !c->attn_count.p;
+    if (int r = ensure(c, c->attn_count, sizeof(unsigned) * (size_t)c->num_sms)) return r;
+    if (fresh) KQ_CUDA(c, cudaMemsetAsync(c->attn_count.p, 0, c->attn_count.cap, c->stream));
+    L.parts = static_cast<float *>(c->attn_parts.p);
+    L.count = static_cast<unsigned *>(c->attn_count.p);
+    return KQ_OK;
+}
+
 // the description that both attention calls launch from
 int attn_launch(kq_ctx *c, const kq_kv_cache *cache, const kq_attn *a, bool prefill, kq::AttnLaunch &L) {
     if (!c) return KQ_ERR_INVALID_ARGUMENT;
@@ -1232,9 +1244,9 @@ extern "C" int kq_kv_append_async(kq_ctx *c, const kq_kv_cache *cache, const kq_
 extern "C" int kq_attn_decode_async(kq_ctx *c, const kq_kv_cache *cache, const kq_attn *a) {
     kq::AttnLaunch L{};
     if (int r = attn_launch(c, cache, a, false, L)) return r;
-    if (L.M == 0) return KQ_OK;
     const OnDevice on(c->device);
-    KQ_CUDA(c, kq::launch_attn_rows(L, c->stream));
+    if (int r = attn_scratch(c, L)) return r;
+    KQ_CUDA(c, kq::launch_attn_decode(L, c->stream));
     return KQ_OK;
 }
 

@@ -36,7 +36,14 @@ struct AttnLaunch {
     int *status;
     int num_sms;
     bool pdl;
+    // scratch: parts of rows that several CTAs share; arrival counts, all zero between launches
+    float *parts;
+    unsigned *count;
 };
+// kq_attn_decode.cu
+size_t attn_decode_part_bytes(int num_sms);
+cudaError_t launch_attn_decode(const AttnLaunch &L, cudaStream_t stream);
+// kq_attn.cu
 cudaError_t launch_attn_rows(const AttnLaunch &L, cudaStream_t stream);
 
 }  // namespace kq

@@ -1,0 +1,476 @@
+// kq_attn_decode.cu -- attention of one new token per sequence over the paged cache.
+//
+// out = sum_j w_j v_j / sum_j w_j,  w_j = 2^(x_j - m),  x_j = scale log2(e) q.k_j,  m a running
+// maximum: one pass over K and V.  Two parts (m, l = sum w, o = sum w v) of one row join as
+// M = max(m, m'), l 2^(m - M) + l' 2^(m' - M), and o likewise.
+//
+// Bound by the cache's bytes: every visible key and value once, 4 D bytes for 4 D G operations
+// (G query heads share a key head).  So the work is cut by bytes: a unit is 16 keys of one
+// (sequence, key head) item, the units of all items stand in one row, and every CTA (one per SM)
+// and in it every warp takes an equal, contiguous range of them -- few or many sequences, equal
+// or ragged, load the SMs alike.  A warp works alone, without shared memory or barriers, and keeps
+// a whole unit (16 keys, 4 KB of K and 4 KB of V at D = 128) in flight in registers; the parts
+// of an item that several warps share meet in shared memory, those that several CTAs share in
+// global memory, joined in unit order by the last CTA that arrives.
+//
+// The products run on mma.m16n8k16 with the keys (then the values' dimensions) as the 16 rows and
+// the query heads as the 8 columns, so a group of up to 8 heads wastes nothing of the registers:
+//   S^T = K Q^T: a lane's 16-byte load of a key row is its A fragment of two steps, because which
+//   k slot stands for which dimension is free as long as Q's B fragment uses the same order;
+//   O^T = V^T P^T: lane (g, t) loads dimensions 8g.. of keys 2t, 2t+1, 2t+8, 2t+9 and pairs the
+//   keys of a dimension with byte permutes; P^T's fragment is S^T's transposed by movmatrix.
+// tcgen05 has nothing to add here: the tensor pipe idles either way while the bytes come in.
+#include "kq_attn_dev.cuh"
+
+#include <mutex>
+
+namespace kq {
+
+namespace {
+
+// Weights reach 2^kBias: their fp16 rounding (11 bits, for the second product) then stays relative
+// down to 2^-22 of the largest instead of 2^-14; sums stay fp32.
+constexpr float kBias = 8.0f;
+constexpr int kUnit = 16;  // keys of a unit; a page holds a multiple of it
+
+template <int D, int NB>
+struct Cfg {
+    // registers of a lane: Q D/8 NB, O D/4 NB, K and V D/4 each, so D = 256 takes 8 heads at a time
+    static constexpr int WARPS = (D * NB <= 128) ? 12 : 8;
+    static constexpr int THREADS = 32 * WARPS;
+};
+
+struct DecodeParams {
+    AttnLaunch a;
+    float scale_log2;
+    int group, rows, splits;  // query heads of a key head; of an item; items of a key head
+    float *parts;             // [CTA][2] parts of rows x D values, then [rows][2] (m, l)
+    unsigned *count;          // [CTA] arrivals at the item that begins in a CTA and ends in a later one
+};
+
+__device__ __forceinline__ uint4 load_stream(const uint16_t *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ float max_over_keys(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+__device__ __forceinline__ float sum_over_keys(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 4);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+// The units of one item that a warp takes, and its place in them.
+struct Item {
+    int seq, vhead, tiles;       // sequence, item of the sequence (key head x splits), units of it
+    long long begin;             // its first unit
+};
+
+// prefix[s]: units of one item of sequences 0..s-1; `per` items a sequence
+__device__ __forceinline__ Item item_of(const long long *prefix, int n_seqs, int per, long long unit) {
+    int lo = 0, hi = n_seqs;  // prefix[lo] * per <= unit < prefix[hi] * per
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] * per <= unit) lo = mid;
+        else hi = mid;
+    }
+    Item it;
+    it.seq = lo;
+    it.tiles = (int)(prefix[lo + 1] - prefix[lo]);
+    const long long r = unit - prefix[lo] * per;
+    it.vhead = (int)(r / it.tiles);
+    it.begin = prefix[lo] * per + (long long)it.vhead * it.tiles;
+    return it;
+}
+
+// How a part with nothing above -inf is marked: m = -inf, and l = 0 when it saw no key, +inf when
+// every score was -inf, NaN when one was NaN.
+struct Join {
+    float M, L;
+    bool seen;
+};
+__device__ __forceinline__ void join_max(Join &j, float m) { j.M = fmaxf(j.M, m); }
+// weight of a part, its l added
+__device__ __forceinline__ float join_add(Join &j, float m, float l) {
+    if (m == -INFINITY) {
+        if (l != l) j.L = l;
+        else if (l > 0.0f) j.seen = true;
+        return 0.0f;
+    }
+    j.seen = true;
+    const float w = exp2f(m - j.M);
+    j.L += w * l;
+    return w;
+}
+
+template <int D, int NB>
+__global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const __grid_constant__ DecodeParams p) {
+    using C = Cfg<D, NB>;
+    constexpr int KC = D / 32;  // 16-byte pieces of a key row per lane
+    constexpr int VC = D / 64;  // of a value row
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ long long s_warp[C::WARPS];
+    __shared__ int s_item[2 * C::WARPS];  // item of each warp's first and last part (-1: none)
+    __shared__ int s_last;
+    const AttnLaunch &a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int S = a.cache.n_seqs, per = a.cache.kv_heads * p.splits;
+    const int part_floats = p.rows * (D + 2);
+    float *s_parts = reinterpret_cast<float *>(smem);
+    long long *prefix = reinterpret_cast<long long *>(smem + (size_t)2 * C::WARPS * part_floats * 4);
+
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // units of every sequence, and where they begin
+    {
+        const int chunk = (S + C::THREADS - 1) / C::THREADS, s0 = tid * chunk;
+        long long sum = 0;
+        for (int s = s0; s < s0 + chunk && s < S; ++s) {
+            bool bad = false;
+            const int len = kv_length(a.cache, __ldg(a.kv_len + s), bad);
+            if (bad && blockIdx.x == 0) report_error(a.status, DEV_ERR_CACHE);
+            const KvSpan sp = kv_span(len - 1, len, a.window, a.sinks);
+            const int n = kv_blocks(sp.kept, sp.lo, sp.hi, kUnit).count;
+            prefix[s] = sum;
+            sum += n;
+            if (n == 0 && s % gridDim.x == blockIdx.x)  // sees nothing: zeros
+                for (int i = 0; i < a.heads * D / 8; ++i)
+                    *reinterpret_cast<uint4 *>(a.out + s * a.out_stride + 8 * i) = make_uint4(0, 0, 0, 0);
+        }
+        long long run = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long o = __shfl_up_sync(0xffffffffu, run, d);
+            if (lane >= d) run += o;
+        }
+        if (lane == 31) s_warp[warp] = run;
+        if (tid < 2 * C::WARPS) s_item[tid] = -1;
+        __syncthreads();
+        long long base = run - sum;
+        for (int w = 0; w < warp; ++w) base += s_warp[w];
+        for (int s = s0; s < s0 + chunk && s < S; ++s) prefix[s] += base;
+        if (tid == C::THREADS - 1) prefix[S] = base + sum;
+        __syncthreads();
+    }
+    const long long total = prefix[S] * per;
+    // no more CTAs than give every warp a unit
+    const int parts = (int)min((long long)gridDim.x, (total + C::WARPS - 1) / C::WARPS);
+    if ((int)blockIdx.x >= parts) return;
+    const long long c0 = part_begin(total, parts, blockIdx.x), c1 = part_begin(total, parts, blockIdx.x + 1);
+    const long long w0 = c0 + part_begin(c1 - c0, C::WARPS, warp), w1 = c0 + part_begin(c1 - c0, C::WARPS, warp + 1);
+
+    int slot = 0;  // this warp's next part in shared memory
+    for (long long unit = w0; unit < w1;) {
+        const Item it = item_of(prefix, S, per, unit);
+        const int kv_head = it.vhead / p.splits, row0 = (it.vhead % p.splits) * p.rows;
+        const int n_rows = min(p.rows, p.group - row0);
+        const int t0 = (int)(unit - it.begin), t1 = (int)min((long long)it.tiles, w1 - it.begin);
+        unit = it.begin + t1;
+        bool bad = false;
+        const int len = kv_length(a.cache, __ldg(a.kv_len + it.seq), bad);
+        const KvSpan span = kv_span(len - 1, len, a.window, a.sinks);
+        const KvBlocks blocks = kv_blocks(span.kept, span.lo, span.hi, kUnit);
+        const int head0 = kv_head * p.group + row0;
+        const int32_t *table = a.cache.table + (long long)it.seq * a.cache.table_stride;
+
+        uint4 q[NB][KC];
+        float o[NB][VC * 4][4], m[NB][2], l[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int r = 8 * b + g;
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+                q[b][c] = r < n_rows ? *reinterpret_cast<const uint4 *>(a.q + it.seq * a.q_stride + (head0 + r) * D + 32 * c + 8 * t)
+                                     : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < VC * 4; ++i) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.0f;
+            m[b][0] = m[b][1] = -INFINITY;
+            l[b][0] = l[b][1] = 0.0f;
+        }
+        bool seen = false;
+        int next_page = __ldg(table + ((kv_block(blocks, t0) * kUnit) >> a.cache.page_shift));
+        for (int i = t0; i < t1; ++i) {
+            const int j0 = kv_block(blocks, i) * kUnit;
+            const int page = next_page;
+            if (i + 1 < t1) next_page = __ldg(table + ((kv_block(blocks, i + 1) * kUnit) >> a.cache.page_shift));
+            if (!kv_page_ok(a.cache, page)) {  // uniform: the unit counts as masked
+                if (lane == 0) report_error(a.status, DEV_ERR_CACHE);
+                continue;
+            }
+            const long long row = kv_row(a.cache, page, kv_head, j0 & ((1 << a.cache.page_shift) - 1));
+            const uint16_t *kp = a.cache.k + row + 8 * t, *vp = a.cache.v + row + 8 * g;
+            // Keys that the row does not see are not loaded: zeros stand for them, whatever they hold.
+            const bool full = j0 >= span.lo && j0 + kUnit <= span.hi;
+            const bool k0 = full || kv_sees(span, j0 + g), k1 = full || kv_sees(span, j0 + g + 8);
+            uint4 kr[2][KC], vr[4][VC];
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                kr[0][c] = k0 ? load_stream(kp + g * D + 32 * c) : zero;
+                kr[1][c] = k1 ? load_stream(kp + (g + 8) * D + 32 * c) : zero;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int key = 2 * t + (u & 1) + 4 * (u & 2);
+                const bool vis = full || kv_sees(span, j0 + key);
+#pragma unroll
+                for (int c = 0; c < VC; ++c) vr[u][c] = vis ? load_stream(vp + key * D + 64 * c) : zero;
+            }
+            seen = true;
+            uint32_t pb[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    mma_f16(s, kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, q[b][c].x, q[b][c].y);
+                    mma_f16(s, kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, q[b][c].z, q[b][c].w);
+                }
+                // s[0], s[1]: key g, rows 2t, 2t+1; s[2], s[3]: key g+8
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] = (e < 2 ? k0 : k1) ? s[e] * p.scale_log2 : -INFINITY;
+                float al[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mn = fmaxf(m[b][e], max_over_keys(fmaxf(s[e], s[e + 2])));
+                    const float ref = (mn == -INFINITY) ? 0.0f : mn;
+                    al[e] = exp2f(m[b][e] - ref);
+                    m[b][e] = mn;
+                    s[e] = exp2f(s[e] - ref + kBias);
+                    s[e + 2] = exp2f(s[e + 2] - ref + kBias);
+                    l[b][e] = l[b][e] * al[e] + (s[e] + s[e + 2]);
+                }
+                if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
+#pragma unroll
+                    for (int i2 = 0; i2 < VC * 4; ++i2) {
+                        o[b][i2][0] *= al[0];
+                        o[b][i2][1] *= al[1];
+                        o[b][i2][2] *= al[0];
+                        o[b][i2][3] *= al[1];
+                    }
+                }
+                pb[b][0] = transpose8x8(f2_to_h2(s[0], s[1]));
+                pb[b][1] = transpose8x8(f2_to_h2(s[2], s[3]));
+            }
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    const uint32_t x0 = word(vr[0][c], jj), x1 = word(vr[1][c], jj);
+                    const uint32_t x2 = word(vr[2][c], jj), x3 = word(vr[3][c], jj);
+                    const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
+                    const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) mma_f16(o[b][4 * c + jj], a0, a1, a2, a3, pb[b][0], pb[b][1]);
+                }
+        }
+
+        // o[b][4c + jj]: dimensions 64c + 8g + 2jj (elements 0, 1) and the next (2, 3), rows 2t (0, 2), 2t+1 (1, 3)
+        const bool whole = t0 == 0 && t1 == it.tiles;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float sum = sum_over_keys(l[b][e]);
+                const int r = 8 * b + 2 * t + e;
+                if (r >= n_rows) continue;
+                if (whole) {
+                    // scores all -inf: 0 / 0 as in the formula; no key there: zeros
+                    const float inv = seen ? 1.0f / sum : 0.0f;
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int jj = 0; jj < 4; ++jj) v[jj] = f2_to_h2(o[b][4 * c + jj][e] * inv, o[b][4 * c + jj][e + 2] * inv);
+                        *reinterpret_cast<uint4 *>(a.out + it.seq * a.out_stride + (head0 + r) * D + 64 * c + 8 * g) =
+                            make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                } else {
+                    float *part = s_parts + (size_t)(2 * warp + slot) * part_floats;
+#pragma unroll
+                    for (int c = 0; c < VC; ++c)
+#pragma unroll
+                        for (int jj = 0; jj < 4; ++jj)
+                            *reinterpret_cast<float2 *>(part + r * D + 64 * c + 8 * g + 2 * jj) =
+                                make_float2(o[b][4 * c + jj][e], o[b][4 * c + jj][e + 2]);
+                    if (g == 0) {
+                        part[p.rows * D + 2 * r] = m[b][e];
+                        part[p.rows * D + 2 * r + 1] = (m[b][e] == -INFINITY && seen && sum == 0.0f) ? INFINITY : sum;
+                    }
+                }
+            }
+        if (!whole) {
+            if (lane == 0) s_item[2 * warp + slot] = it.seq * per + it.vhead;
+            ++slot;
+        }
+    }
+    __syncthreads();
+
+    // Join the warps' parts of each item (they stand in unit order): into the output, or into this
+    // CTA's part of an item that other CTAs share too.
+    int shared_item[2] = {-1, -1};  // the item that began before this CTA, the one that goes on after it
+    for (int i0 = 0; i0 < 2 * C::WARPS;) {
+        const int id = s_item[i0];
+        if (id < 0) {
+            ++i0;
+            continue;
+        }
+        int i1 = i0 + 1;  // parts [i0, i1) that are there and of this item
+        while (i1 < 2 * C::WARPS && (s_item[i1] == id || s_item[i1] < 0)) ++i1;
+        const int seq = id / per, vh = id % per;
+        const int tiles = (int)(prefix[seq + 1] - prefix[seq]);
+        const long long b0 = prefix[seq] * per + (long long)vh * tiles, b1 = b0 + tiles;
+        const bool mine = b0 >= c0 && b1 <= c1;
+        const int which = b0 < c0 ? 0 : 1;
+        if (!mine) shared_item[which] = id;
+        const int row0 = (vh % p.splits) * p.rows, n_rows = min(p.rows, p.group - row0);
+        const int head0 = (vh / p.splits) * p.group + row0;
+        float *out_part = p.parts + (size_t)(2 * blockIdx.x + which) * part_floats;
+        for (int e = tid; e < n_rows * (D / 2); e += C::THREADS) {
+            const int r = e / (D / 2), d = 2 * (e % (D / 2));
+            Join jn = {-INFINITY, 0.0f, false};
+            for (int i = i0; i < i1; ++i)
+                if (s_item[i] == id) join_max(jn, s_parts[(size_t)i * part_floats + p.rows * D + 2 * r]);
+            float2 acc = make_float2(0.0f, 0.0f);
+            for (int i = i0; i < i1; ++i) {
+                if (s_item[i] != id) continue;
+                const float *part = s_parts + (size_t)i * part_floats;
+                const float w = join_add(jn, part[p.rows * D + 2 * r], part[p.rows * D + 2 * r + 1]);
+                if (w == 0.0f) continue;
+                const float2 v = *reinterpret_cast<const float2 *>(part + r * D + d);
+                acc.x += w * v.x;
+                acc.y += w * v.y;
+            }
+            if (mine) {
+                const float inv = 1.0f / jn.L;
+                *reinterpret_cast<uint32_t *>(a.out + seq * a.out_stride + (head0 + r) * D + d) =
+                    (jn.seen || jn.L != jn.L) ? f2_to_h2(acc.x * inv, acc.y * inv) : 0u;
+            } else {
+                *reinterpret_cast<float2 *>(out_part + r * D + d) = acc;
+                if (d == 0) {
+                    out_part[p.rows * D + 2 * r] = jn.M;
+                    out_part[p.rows * D + 2 * r + 1] = (jn.M == -INFINITY && jn.seen && jn.L == 0.0f) ? INFINITY : jn.L;
+                }
+            }
+        }
+        i0 = i1;
+    }
+
+    // Items shared with other CTAs: the last to arrive joins their parts in unit order.
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        const int id = shared_item[which];
+        if (id < 0) continue;  // uniform over the CTA
+        const int seq = id / per, vh = id % per;
+        const int tiles = (int)(prefix[seq + 1] - prefix[seq]);
+        const long long b0 = prefix[seq] * per + (long long)vh * tiles;
+        const int first = part_of(total, parts, b0), last = part_of(total, parts, b0 + tiles - 1);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            const unsigned n = atomicAdd(p.count + first, 1u);
+            s_last = n == (unsigned)(last - first);
+            if (s_last) p.count[first] = 0;  // for the next launch
+            __threadfence();
+        }
+        __syncthreads();
+        if (!s_last) continue;
+        const int row0 = (vh % p.splits) * p.rows, n_rows = min(p.rows, p.group - row0);
+        const int head0 = (vh / p.splits) * p.group + row0;
+        for (int e = tid; e < n_rows * (D / 2); e += C::THREADS) {
+            const int r = e / (D / 2), d = 2 * (e % (D / 2));
+            Join jn = {-INFINITY, 0.0f, false};
+#pragma unroll 4
+            for (int c = first; c <= last; ++c)
+                join_max(jn, __ldcg(p.parts + (size_t)(2 * c + (c == first)) * part_floats + p.rows * D + 2 * r));
+            float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+            for (int c = first; c <= last; ++c) {
+                const float *part = p.parts + (size_t)(2 * c + (c == first)) * part_floats;
+                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part + p.rows * D + 2 * r));
+                const float2 v = __ldcg(reinterpret_cast<const float2 *>(part + r * D + d));
+                const float w = join_add(jn, ml.x, ml.y);
+                if (w != 0.0f) {
+                    acc.x += w * v.x;
+                    acc.y += w * v.y;
+                }
+            }
+            const float inv = 1.0f / jn.L;
+            *reinterpret_cast<uint32_t *>(a.out + seq * a.out_stride + (head0 + r) * D + d) =
+                (jn.seen || jn.L != jn.L) ? f2_to_h2(acc.x * inv, acc.y * inv) : 0u;
+        }
+    }
+}
+
+template <int D, int NB>
+cudaError_t launch(DecodeParams &p, cudaStream_t stream) {
+    using C = Cfg<D, NB>;
+    p.rows = p.group < 8 * NB ? p.group : 8 * NB;
+    p.splits = (p.group + p.rows - 1) / p.rows;
+    const size_t smem = (size_t)2 * C::WARPS * p.rows * (D + 2) * 4 + (size_t)(p.a.cache.n_seqs + 1) * 8;
+    {
+        static std::mutex mu;
+        static bool configured[64] = {};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev < 0 || dev >= 64 || !configured[dev]) {
+            cudaError_t e = cudaFuncSetAttribute(kq_attn_decode<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+            if (e != cudaSuccess) return e;
+            if (dev >= 0 && dev < 64) configured[dev] = true;
+        }
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.a.num_sms);
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = p.a.pdl ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kq_attn_decode<D, NB>, p);
+}
+
+}  // namespace
+
+size_t attn_decode_part_bytes(int num_sms) { return (size_t)2 * num_sms * KQ_MAX_GROUP * (KQ_MAX_HEAD_DIM + 2) * 4; }
+
+cudaError_t launch_attn_decode(const AttnLaunch &L, cudaStream_t stream) {
+    DecodeParams p{};
+    p.a = L;
+    p.scale_log2 = L.scale * 1.4426950408889634f;
+    p.group = L.heads / L.cache.kv_heads;
+    p.parts = L.parts;
+    p.count = L.count;
+    const bool wide = p.group > 8;
+    switch (L.cache.head_dim) {
+        case 64: return wide ? launch<64, 2>(p, stream) : launch<64, 1>(p, stream);
+        case 128: return wide ? launch<128, 2>(p, stream) : launch<128, 1>(p, stream);
+        case 256: return launch<256, 1>(p, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace kq
