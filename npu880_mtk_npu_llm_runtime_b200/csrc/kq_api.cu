@@ -52,6 +52,7 @@ struct kq_ctx {
     bool gemv_half = true;  // Q4_K / Q5_K GEMV launches of 1-2 rows: 8-row halves per CTA where better
     bool ffn_fused = true;  // FFN blocks of 1-2 tokens as one persistent kernel where a plan exists
     bool split_dirty = false;
+    bool attn_dirty = false;  // an attention kernel that stopped early may have left arrival counts
     bool graph_holds_scratch = false;  // a call of this context was captured into a CUDA graph
 
     // the engine's g_sdot_input state: pending pre-quantized Q8_K input (ENG:4184) and the
@@ -134,6 +135,7 @@ int check_device_status(kq_ctx *c) {
     const int st = *hs;
     if (st == kq::DEV_OK) return KQ_OK;
     *hs = kq::DEV_OK;
+    c->attn_dirty = true;
     c->split_dirty = true;  // a kernel that stopped early may have left arrival counts behind
     if (st == kq::DEV_ERR_TIMEOUT) return fail(c, KQ_ERR_TIMEOUT, "a device-side wait timed out");
     if (st == kq::DEV_ERR_INDEX) return fail(c, KQ_ERR_SHAPE, "a row id is past the end of the weight");
@@ -1150,10 +1152,12 @@ struct OnDevice {
 
 // Scratch of the attention kernels: one size for all shapes, so that it never grows after the first call.
 int attn_scratch(kq_ctx *c, kq::AttnLaunch &L) {
-    if (int r = ensure(c, c->attn_parts, kq::attn_decode_part_bytes(c->num_sms))) return r;
-    const bool fresh = !c->attn_count.p;
+    if (int r = ensure(c, c->attn_parts, std::max(kq::attn_decode_part_bytes(c->num_sms),
+                                                            kq::attn_prefill_part_bytes(c->num_sms)))) return r;
+    const bool clear = !c->attn_count.p || c->attn_dirty;
     if (int r = ensure(c, c->attn_count, sizeof(unsigned) * (size_t)c->num_sms)) return r;
-    if (fresh) KQ_CUDA(c, cudaMemsetAsync(c->attn_count.p, 0, c->attn_count.cap, c->stream));
+    if (clear) KQ_CUDA(c, cudaMemsetAsync(c->attn_count.p, 0, c->attn_count.cap, c->stream));
+    c->attn_dirty = false;
     L.parts = static_cast<float *>(c->attn_parts.p);
     L.count = static_cast<unsigned *>(c->attn_count.p);
     return KQ_OK;
@@ -1179,6 +1183,8 @@ int attn_launch(kq_ctx *c, const kq_kv_cache *cache, const kq_attn *a, bool pref
     L.status = c->d_status;
     L.num_sms = c->num_sms;
     L.pdl = c->pdl;
+    L.timeout_ns = c->timeout_ns;
+    L.inject = c->inject_timeout ? 1 : 0;
     return KQ_OK;
 }
 
@@ -1255,7 +1261,8 @@ extern "C" int kq_attn_prefill_async(kq_ctx *c, const kq_kv_cache *cache, const 
     if (int r = attn_launch(c, cache, a, true, L)) return r;
     if (L.M == 0) return KQ_OK;
     const OnDevice on(c->device);
-    KQ_CUDA(c, kq::launch_attn_rows(L, c->stream));
+    if (int r = attn_scratch(c, L)) return r;
+    KQ_CUDA(c, kq::launch_attn_prefill(L, c->stream));
     return KQ_OK;
 }
 

@@ -21,7 +21,7 @@ struct RopeLaunch {
 };
 cudaError_t launch_norm_rope(const RopeLaunch &L, cudaStream_t stream);
 
-// Attention over the cache (kq_attn.cu): M rows, of one token per sequence (q_start == nullptr)
+// Attention over the cache: M rows, of one token per sequence (q_start == nullptr)
 // or of the sequences' last rows.
 struct AttnLaunch {
     KvView cache;
@@ -39,11 +39,13 @@ struct AttnLaunch {
     // scratch: parts of rows that several CTAs share; arrival counts, all zero between launches
     float *parts;
     unsigned *count;
+    unsigned long long timeout_ns;
+    int inject;  // failure-path test hook (see kq_set_option "inject_timeout")
 };
+// kq_attn_prefill.cu
+size_t attn_prefill_part_bytes(int num_sms);
+cudaError_t launch_attn_prefill(const AttnLaunch &L, cudaStream_t stream);
 // kq_attn_decode.cu
 size_t attn_decode_part_bytes(int num_sms);
 cudaError_t launch_attn_decode(const AttnLaunch &L, cudaStream_t stream);
-// kq_attn.cu
-cudaError_t launch_attn_rows(const AttnLaunch &L, cudaStream_t stream);
-
 }  // namespace kq

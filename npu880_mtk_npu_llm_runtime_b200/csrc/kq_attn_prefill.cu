@@ -1,0 +1,994 @@
+// kq_attn_prefill.cu -- attention of ragged prompt rows over the paged cache on the 5th-generation
+// tensor cores (tcgen05.mma kind::f16, accumulators in TMEM).
+//
+// out = sum_j w_j v_j / sum_j w_j,  w_j = 2^(x_j - m),  x_j = scale log2(e) q.k_j: one pass over
+// the keys with a running maximum.  m may lag behind the true maximum by up to 2^kLag (any m gives
+// the same quotient), so the accumulated rows are rescaled only when it falls further behind.
+//
+// Rows: the query heads that share a key head are packed side by side, row = token * G + head, so a
+// 128-row MMA tile holds 128 / G tokens and short prompts fill it too.  A CTA takes NT = 2 such
+// tiles (heads of 64 and 128; 1 for 256) over the same key blocks: while the softmax of one tile
+// runs, the tensor core works for the other.  Bound by the tensor pipe and the exponentials alike
+// (128 x 128 x 2 x 128 operations and 128 x 128 exponentials take about the same time).
+//
+// Warps 0-3 and 4-7: softmax of tile 0 and 1, one row a thread: S from TMEM to registers, maximum,
+// exponentials, P as fp16 back into S's columns (the second product's A operand), and the epilogue.
+// Warp 8 issues the MMAs: P(j-1) V(j-1) then Q K(j) per tile, so S's columns are free when they are
+// written.  Warp 9 loads: Q as one box of [tokens][G heads][64 values] per 64 values, K and V page
+// by page (TMA, 128-byte swizzle) into a ring of blocks of BN keys; V stays as it lies in the cache
+// and is the MMA's MN-major B operand.
+//
+// Work: an item is a row tile of one key head, a unit one of its key blocks.  Items go whole to
+// the CTAs, longest first in snake order, when that balances; else (few items, long caches) every
+// CTA takes an equal range of units, and the parts of an item that several CTAs share are joined
+// in order by the last of them.
+#include "kq_attn_dev.cuh"
+
+#include <cuda.h>
+#include <mutex>
+
+namespace kq {
+
+namespace {
+
+constexpr float kBias = 4.0f;  // weights reach 2^(kBias + kLag) < 65504: fp16's relative precision reaches further down
+constexpr float kLag = 8.0f;
+constexpr int kThreads = 384;
+constexpr int kSortTiles = 512;
+// A join costs about as much as this many blocks: whole items unless the longest is that much
+// longer than an even share.
+constexpr int kJoinBlocks = 8;
+
+template <int D>
+struct Cfg {
+    static constexpr int NT = D == 256 ? 1 : 2;    // MMA tiles of 128 rows
+    static constexpr int BN = D == 256 ? 64 : 128; // keys of a block
+    static constexpr int CH = D / 64;              // 128-byte wide pieces of a row
+    static constexpr uint32_t Q_TILE = 128 * D * 2;
+    static constexpr uint32_t STAGE = BN * D * 2;
+    static constexpr int MAX_STAGES = 8;
+    static constexpr uint32_t S_COL = BN;          // TMEM columns: S slots, then O
+    static constexpr uint32_t O_COL = 256;
+    static constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((128u >> 4) << 24);
+    static constexpr uint32_t IDESC_O = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+};
+
+struct PrefillParams {
+    AttnLaunch a;
+    float scale_log2;
+    int group, tpt;   // query heads of a key head; tokens of an MMA tile
+    int box_rows;     // keys of one K/V box: the smaller of a page and a block
+    int stages;
+    unsigned long long timeout_ns;
+    int inject;
+};
+
+// ------------------------------------------------------------------ PTX
+
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
+    // 128-byte swizzle, 8-row groups 1,024 bytes apart (descriptor version 1)
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0));
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap *m, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *m, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(m), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *r) {
+    uint32_t *u = reinterpret_cast<uint32_t *>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{ .reg .pred P; elect.sync _|P, 0xffffffff; selp.u32 %0, 1, 0, P; }" : "=r"(pred));
+    return pred != 0;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ------------------------------------------------------------------ work
+
+// What the CTA's roles walk: the same segments (an item, or a range of its blocks) in the same order.
+struct Plan {
+    const int *seq_tiles;            // [n_seqs + 1] first row tile of each sequence
+    const unsigned short *order;     // whole items: row tiles, longest first (nullptr: last first)
+    int tiles;                       // row tiles of all sequences
+    int whole;                       // items go whole
+    int parts;                       // else: CTAs that share the units
+    int start_tile;                  // else: the tile of this CTA's first unit, and that tile's first unit
+    long long start_begin, total, c0, c1;
+};
+
+struct Segment {
+    int seq, head, tile;
+    int tok, n_tok;         // tokens of the sequence: first, number of them in the tile
+    int row0;               // row of the first
+    int pos0, len;          // its position; keys of the sequence
+    KvBlocks blocks;
+    KvSpan first, last;     // keys that the first and the last token see
+    int b0, b1, nb;         // blocks of this segment, blocks of the item
+    int live, bad;          // 0: no more segments; 1: a page that a token sees is missing
+    long long begin;        // first unit of the item
+};
+
+// The row tile `tile` of sequence `seq` as a segment of all its blocks.  At least one block, so that
+// a tile that sees nothing still writes its zeros.
+template <int D>
+__device__ __forceinline__ void tile_of(const PrefillParams &p, int seq, int tile_in_seq, Segment &s) {
+    using C = Cfg<D>;
+    bool bad = false;
+    const KvRows rows = kv_rows(__ldg(p.a.q_start + seq), __ldg(p.a.q_start + seq + 1), p.a.M, bad);
+    s.seq = seq;
+    s.len = kv_length(p.a.cache, __ldg(p.a.kv_len + seq), bad);
+    s.tok = tile_in_seq * C::NT * p.tpt;
+    s.n_tok = min(C::NT * p.tpt, rows.n - s.tok);
+    s.row0 = rows.begin + s.tok;
+    s.pos0 = s.len - rows.n + s.tok;
+    s.first = kv_span(s.pos0, s.len, p.a.window, p.a.sinks);
+    s.last = kv_span(s.pos0 + s.n_tok - 1, s.len, p.a.window, p.a.sinks);
+    s.blocks = kv_blocks(s.last.kept, s.first.lo, s.last.hi, C::BN);
+    if (s.blocks.count == 0) s.blocks.count = 1;
+    s.nb = s.blocks.count;
+    s.b0 = 0;
+    s.b1 = s.nb;
+}
+
+__device__ __forceinline__ int seq_of_tile(const int *seq_tiles, int n_seqs, int tile) {
+    int lo = 0, hi = n_seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (seq_tiles[mid] <= tile) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Does any token of the tile see a key of [j, j + n)?
+__device__ __forceinline__ bool tile_sees(const Segment &s, int j, int n) {
+    return (j < s.last.hi && j + n > s.first.lo) || j < s.last.kept;
+}
+
+template <int D>
+struct Walk {
+    const PrefillParams &p;
+    const Plan &plan;
+    int k = 0;            // whole items: the CTA's next
+    long long unit;       // else: the next unit
+    int tile;
+    long long begin;
+    __device__ Walk(const PrefillParams &pp, const Plan &pl)
+        : p(pp), plan(pl), unit(pl.c0), tile(pl.start_tile), begin(pl.start_begin) {}
+    __device__ bool next(Segment &s) {
+        const int heads = p.a.cache.kv_heads;
+        if (plan.whole) {
+            const long long G = gridDim.x, c = blockIdx.x;
+            const long long idx = k * G + ((k & 1) ? G - 1 - c : c);
+            if (k * G >= (long long)plan.tiles * heads) return false;
+            ++k;
+            if (idx >= (long long)plan.tiles * heads) return next(s);
+            const int rank = (int)(idx / heads);
+            s.head = (int)(idx % heads);
+            s.tile = plan.order ? plan.order[rank] : plan.tiles - 1 - rank;
+            const int seq = seq_of_tile(plan.seq_tiles, p.a.cache.n_seqs, s.tile);
+            tile_of<D>(p, seq, s.tile - plan.seq_tiles[seq], s);
+            s.begin = 0;
+            return true;
+        }
+        if (unit >= plan.c1) return false;
+        const int seq = seq_of_tile(plan.seq_tiles, p.a.cache.n_seqs, tile);
+        tile_of<D>(p, seq, tile - plan.seq_tiles[seq], s);
+        s.tile = tile;
+        const long long r = unit - begin;
+        s.head = (int)(r / s.nb);
+        s.b0 = (int)(r % s.nb);
+        s.begin = begin + (long long)s.head * s.nb;
+        const long long left = plan.c1 - unit;
+        s.b1 = s.nb - s.b0 < left ? s.nb : s.b0 + (int)left;
+        unit += s.b1 - s.b0;
+        if (unit >= begin + (long long)s.nb * heads) {
+            begin += (long long)s.nb * heads;
+            ++tile;
+        }
+        return true;
+    }
+};
+
+// ------------------------------------------------------------------ kernel
+
+constexpr int kSegs = 4;  // segments on their way from the loader to the other roles
+
+struct Shared {
+    unsigned long long full[8], empty[8], q_full, q_empty, s_full[2], p_ready[2], o_full[2], pv_done, tail, join, never;
+    unsigned long long seg_full[kSegs], seg_empty[kSegs];
+    Segment seg[kSegs];
+    uint32_t tmem;
+    int abort, last;
+    long long red[kThreads / 32];
+    int red_max[kThreads / 32];
+    Plan plan;
+};
+
+static_assert(sizeof(Shared) <= 1024, "a CTA has 227 KB of shared memory");
+constexpr size_t kSmem = 226 * 1024;  // dynamic
+
+// Bounded wait on a phase: false when it did not complete in time or another role gave up.
+struct Waiter {
+    Shared &sh;
+    unsigned long long timeout_ns;
+    int *status;
+    __device__ __forceinline__ bool operator()(unsigned long long &bar, uint32_t parity) const {
+        const uint32_t b = smem_u32(&bar);
+        if (mbar_try_wait(b, parity)) return true;
+        uint64_t t0 = 0;
+        for (uint32_t polls = 1;; ++polls) {
+            if (mbar_try_wait(b, parity)) return true;
+            if (polls & 63) continue;
+            if (*reinterpret_cast<volatile int *>(&sh.abort)) return false;
+            const uint64_t now = global_timer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > timeout_ns) {
+                *reinterpret_cast<volatile int *>(&sh.abort) = 1;
+                report_error(status, DEV_ERR_TIMEOUT);
+                return false;
+            }
+        }
+    }
+};
+
+// The CTA's plan, by all its threads.  scratch: at least 4 bytes per row tile.
+template <int D>
+__device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, int *seq_tiles, unsigned short *order, int *nbs) {
+    using C = Cfg<D>;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = p.a.cache.n_seqs;
+    const int per = C::NT * p.tpt;
+    {
+        const int chunk = (S + kThreads - 1) / kThreads, s0 = tid * chunk;
+        int sum = 0;
+        for (int s = s0; s < s0 + chunk && s < S; ++s) {
+            bool bad = false;
+            const KvRows r = kv_rows(__ldg(p.a.q_start + s), __ldg(p.a.q_start + s + 1), p.a.M, bad);
+            kv_length(p.a.cache, __ldg(p.a.kv_len + s), bad);
+            if (bad && blockIdx.x == 0) report_error(p.a.status, DEV_ERR_CACHE);
+            seq_tiles[s] = sum;
+            sum += (r.n + per - 1) / per;
+        }
+        int run = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, run, d);
+            if (lane >= d) run += o;
+        }
+        if (lane == 31) sh.red[warp] = run;
+        __syncthreads();
+        int base = run - sum;
+        for (int w = 0; w < warp; ++w) base += (int)sh.red[w];
+        for (int s = s0; s < s0 + chunk && s < S; ++s) seq_tiles[s] += base;
+        if (tid == kThreads - 1) seq_tiles[S] = base + sum;
+        __syncthreads();
+    }
+    const int tiles = seq_tiles[S], heads = p.a.cache.kv_heads;
+    const int chunk = (tiles + kThreads - 1) / kThreads, i0 = tid * chunk;
+    long long sum = 0;
+    int most = 0;
+    for (int i = i0; i < i0 + chunk && i < tiles; ++i) {
+        Segment s;
+        const int seq = seq_of_tile(seq_tiles, S, i);
+        tile_of<D>(p, seq, i - seq_tiles[seq], s);
+        nbs[i] = s.nb;
+        sum += s.nb;
+        most = max(most, s.nb);
+    }
+    long long run = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, run, d);
+        if (lane >= d) run += o;
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+    }
+    if (lane == 31) sh.red[warp] = run;
+    if (lane == 0) sh.red_max[warp] = most;
+    __syncthreads();
+    long long before = run - sum, total = 0;
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) before += sh.red[w];
+        total += sh.red[w];
+        most = max(most, sh.red_max[w]);
+    }
+    total *= heads;
+    const int whole = most <= total / (int)gridDim.x + kJoinBlocks;
+    const int parts = (int)min((long long)gridDim.x, total);
+    const bool sorted = whole && tiles <= kSortTiles;
+    if (sorted) {
+        for (int i = tid; i < tiles; i += kThreads) {
+            int rank = 0;
+            for (int j = 0; j < tiles; ++j) rank += nbs[j] > nbs[i] || (nbs[j] == nbs[i] && j < i);
+            order[rank] = (unsigned short)i;
+        }
+    }
+    if (tid == 0) {
+        Plan &pl = sh.plan;
+        pl.seq_tiles = seq_tiles;
+        pl.order = sorted ? order : nullptr;
+        pl.tiles = tiles;
+        pl.whole = whole;
+        pl.parts = parts;
+        pl.total = total;
+        pl.c0 = pl.c1 = 0;
+        pl.start_tile = 0;
+        pl.start_begin = 0;
+        if (!whole && (int)blockIdx.x < parts) {
+            pl.c0 = part_begin(total, parts, blockIdx.x);
+            pl.c1 = part_begin(total, parts, blockIdx.x + 1);
+        }
+    }
+    __syncthreads();
+    if (!whole && sh.plan.c1 > sh.plan.c0) {
+        const long long c0 = sh.plan.c0;
+        for (int i = i0; i < i0 + chunk && i < tiles; ++i) {
+            if (before * heads <= c0 && c0 < (before + nbs[i]) * heads) {
+                sh.plan.start_tile = i;
+                sh.plan.start_begin = before * heads;
+            }
+            before += nbs[i];
+        }
+    }
+    __syncthreads();
+}
+
+// Loads of one CTA, by a warp: segments to the other roles, Q, K and V to shared memory.  n counts
+// the ring blocks issued.
+template <int D>
+__device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, const Waiter &wait, const CUtensorMap &mq,
+                                          const CUtensorMap &mk, const CUtensorMap &mv, unsigned char *s_q,
+                                          unsigned char *s_ring, int lane, uint32_t &n) {
+    using C = Cfg<D>;
+    constexpr int NT = C::NT, BN = C::BN, CH = C::CH;
+    const AttnLaunch &a = p.a;
+    const int boxes = (BN / p.box_rows) * CH;
+    const int sub = lane / CH, piece = lane % CH;  // this lane's box of a block
+    uint32_t tails = 0;
+    Walk<D> walk(p, sh.plan);
+    for (uint32_t k = 0;; ++k) {
+        Segment s;
+        const bool have = walk.next(s);
+        Segment &rec = sh.seg[k % kSegs];
+        if (!wait(sh.seg_empty[k % kSegs], ((k / kSegs) & 1) ^ 1)) return;
+        if (lane == 0) {
+            s.bad = 0;
+            s.live = have;
+            rec = s;
+            mbar_arrive(smem_u32(&sh.seg_full[k % kSegs]));
+        }
+        __syncwarp();
+        if (!have) return;
+        const int subs = s.n_tok > p.tpt ? NT : 1;
+        const int32_t *table = a.cache.table + (long long)s.seq * a.cache.table_stride;
+        // block i of the segment's K (kv = 0) or V (1) into the ring
+        auto load = [&](int i, int kv) {
+            const int st = n % p.stages;
+            if (!wait(sh.empty[st], ((n / p.stages) & 1) ^ 1)) return false;
+            ++n;
+            const int j0 = kv_block(s.blocks, i) * BN;
+            unsigned char *to = s_ring + (size_t)st * C::STAGE;
+            // V rows past the sequence's end may hold anything, and 0 * NaN is NaN: zeroed once they landed
+            const bool tail = kv == 1 && j0 + BN > s.len;
+            const uint32_t bar = smem_u32(tail ? &sh.tail : &sh.full[st]);
+            if (lane == 0) mbar_arrive_expect_tx(bar, C::STAGE);
+            __syncwarp();
+            if (lane < boxes) {
+                const int j = j0 + sub * p.box_rows;
+                int page = a.cache.n_pages;  // out of range: the box is filled with zeros
+                if (tile_sees(s, j, p.box_rows)) {
+                    const int q = __ldg(table + (j >> a.cache.page_shift));
+                    if (kv_page_ok(a.cache, q)) page = q;
+                    else rec.bad = 1;
+                }
+                tma4(smem_u32(to) + piece * (BN * 128) + sub * p.box_rows * 128, kv ? &mv : &mk, 64 * piece,
+                     j & ((1 << a.cache.page_shift) - 1), s.head, page, bar);
+            }
+            if (tail) {
+                if (!wait(sh.tail, tails & 1)) return false;
+                ++tails;
+                for (int e = lane + max(0, s.len - j0) * 8; e < BN * 8; e += 32)
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+                        *reinterpret_cast<uint4 *>(to + c * (BN * 128) + e * 16) = make_uint4(0, 0, 0, 0);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.full[st]));
+            }
+            __syncwarp();
+            return true;
+        };
+        if (!load(s.b0, 0)) return;
+        if (!wait(sh.q_empty, (k & 1) ^ 1)) return;
+        if (lane == 0) mbar_arrive_expect_tx(smem_u32(&sh.q_full), (uint32_t)(subs * p.tpt * p.group * D * 2));
+        __syncwarp();
+        if (lane < subs * CH)
+            tma3(smem_u32(s_q) + sub * C::Q_TILE + piece * (128 * 128), &mq, 64 * piece, s.head * p.group,
+                 s.row0 + sub * p.tpt, smem_u32(&sh.q_full));
+        __syncwarp();
+        // the rest in the order in which the MMAs read it
+        if (NT == 2) {
+            for (int i = s.b0; i < s.b1; ++i) {
+                if (i > s.b0 && !load(i, 0)) return;
+                if (!load(i, 1)) return;
+            }
+        } else {
+            if (s.b0 + 1 < s.b1 && !load(s.b0 + 1, 0)) return;
+            for (int i = s.b0; i < s.b1; ++i) {
+                if (!load(i, 1)) return;
+                if (i + 2 < s.b1 && !load(i + 2, 0)) return;
+            }
+        }
+    }
+}
+
+// The MMAs of one CTA, by a converged warp.
+template <int D>
+__device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, const Waiter &wait, uint32_t q0, uint32_t ring,
+                                         uint32_t tmem) {
+    using C = Cfg<D>;
+    constexpr int NT = C::NT, BN = C::BN;
+    uint32_t n = 0, np[2] = {0, 0};  // ring blocks read, P's read of each slot
+    if (p.inject && !wait(sh.never, 0)) return;
+    // S slot = Q tile t times the K block in ring stage st
+    auto mma_s = [&](int t, int slot, uint32_t st) {
+        if (elect_one()) {
+            const uint32_t kb = ring + st * C::STAGE, qb = q0 + t * C::Q_TILE;
+#pragma unroll
+            for (int e = 0; e < D / 16; ++e)
+                mma_ss(tmem + slot * C::S_COL, desc_sw128(qb + (e / 4) * (128 * 128) + (e % 4) * 32, 16),
+                       desc_sw128(kb + (e / 4) * (BN * 128) + (e % 4) * 32, 16), C::IDESC_S, e > 0);
+            commit(smem_u32(&sh.s_full[slot]));
+        }
+        __syncwarp();
+    };
+    // O tile t (+)= P of the slot times the V block in ring stage st
+    auto mma_o = [&](int t, int slot, uint32_t st, bool first) {
+        if (!wait(sh.p_ready[slot], np[slot] & 1)) return false;
+        ++np[slot];
+        fence_after();
+        if (elect_one()) {
+            const uint32_t vb = ring + st * C::STAGE;
+#pragma unroll
+            for (int e = 0; e < BN / 16; ++e)
+                mma_ts(tmem + C::O_COL + t * D, tmem + slot * C::S_COL + e * 8, desc_sw128(vb + e * 2048, BN * 128), C::IDESC_O,
+                       !(first && e == 0));
+        }
+        __syncwarp();
+        return true;
+    };
+    auto arrive = [&](unsigned long long &bar) {
+        if (elect_one()) commit(smem_u32(&bar));
+        __syncwarp();
+    };
+    auto stage = [&](uint32_t i) { return i % p.stages; };
+    auto wait_full = [&](uint32_t i) {
+        if (!wait(sh.full[i % p.stages], (i / p.stages) & 1)) return false;
+        fence_after();
+        return true;
+    };
+    for (uint32_t k = 0;; ++k) {
+        if (!wait(sh.seg_full[k % kSegs], (k / kSegs) & 1)) return;
+        const Segment &s = sh.seg[k % kSegs];
+        if (!s.live) return;
+        const int subs = s.n_tok > p.tpt ? NT : 1, nb = s.b1 - s.b0;
+        __syncwarp();
+        if (elect_one()) mbar_arrive(smem_u32(&sh.seg_empty[k % kSegs]));
+        if (!wait(sh.q_full, k & 1)) return;
+        fence_after();
+        if (NT == 2) {
+            // ring: K0 V0 K1 V1 ...
+            for (int j = 0; j < nb; ++j) {
+                const uint32_t kk = n + 2 * j;
+                if (!wait_full(kk)) return;
+                if (j > 0 && !wait_full(kk - 1)) return;
+                for (int t = 0; t < subs; ++t) {
+                    if (j > 0 && !mma_o(t, t, stage(kk - 1), j == 1)) return;
+                    mma_s(t, t, stage(kk));
+                }
+                if (j > 0) arrive(sh.empty[stage(kk - 1)]);
+                arrive(sh.empty[stage(kk)]);
+                if (j == nb - 1) arrive(sh.q_empty);
+            }
+            const uint32_t v = n + 2 * nb - 1;
+            if (!wait_full(v)) return;
+            for (int t = 0; t < subs; ++t) {
+                if (!mma_o(t, t, stage(v), nb == 1)) return;
+                arrive(sh.o_full[t]);
+            }
+            arrive(sh.empty[stage(v)]);
+        } else {
+            // ring: K0 K1 V0 K2 V1 ... K(i) V(i-2) ... V(nb-1)
+            auto k_at = [&](int i) { return n + (i < 2 ? i : 2 * i - 1); };
+            auto v_at = [&](int i) { return n + (i + 2 < nb ? 2 * i + 2 : nb + i); };
+            for (int i = 0; i < 2 && i < nb; ++i) {
+                if (!wait_full(k_at(i))) return;
+                mma_s(0, i, stage(k_at(i)));
+                arrive(sh.empty[stage(k_at(i))]);
+                if (i == nb - 1) arrive(sh.q_empty);
+            }
+            for (int i = 0; i < nb; ++i) {
+                if (!wait_full(v_at(i))) return;
+                if (!mma_o(0, i & 1, stage(v_at(i)), i == 0)) return;
+                arrive(i == nb - 1 ? sh.o_full[0] : sh.pv_done);
+                arrive(sh.empty[stage(v_at(i))]);
+                if (i + 2 < nb) {
+                    if (!wait_full(k_at(i + 2))) return;
+                    mma_s(0, i & 1, stage(k_at(i + 2)));
+                    arrive(sh.empty[stage(k_at(i + 2))]);
+                    if (i + 2 == nb - 1) arrive(sh.q_empty);
+                }
+            }
+        }
+        n += 2 * nb;
+    }
+}
+
+// Rows of a warp whose plain result does not stand: computed key by key, over exactly their own
+// keys.  These see nothing (zeros), or have a value that is not finite: a weight of 0 times an
+// infinity that only other rows see is NaN in the matrix product; or a page is missing.
+template <int D>
+__device__ __forceinline__ void mend_rows(const PrefillParams &p, const Segment &s, bool odd, int tok, int head, int lane) {
+    uint32_t todo = __ballot_sync(0xffffffffu, odd);
+    while (todo) {
+        const int src = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const int tk = __shfl_sync(0xffffffffu, tok, src), hd = __shfl_sync(0xffffffffu, head, src);
+        const long long row = s.row0 + tk;
+        attn_row<D>(p.a.cache, s.seq, s.head, kv_span(s.pos0 + tk, s.len, p.a.window, p.a.sinks),
+                    p.a.q + row * p.a.q_stride + hd * D, p.a.out + row * p.a.out_stride + hd * D, p.a.scale, lane, p.a.status);
+    }
+}
+
+// 32 values of a row, rounded, to out (where `write`); true when one is not finite
+__device__ __forceinline__ bool put32(const float *o, uint16_t *out, bool write) {
+    bool odd = false;
+    uint32_t h[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        odd |= !(fabsf(o[2 * e]) <= 65504.0f) || !(fabsf(o[2 * e + 1]) <= 65504.0f);
+        h[e] = f2_to_h2(o[2 * e], o[2 * e + 1]);
+    }
+    if (write)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4 *>(out + 8 * e) = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+    return odd;
+}
+
+// Softmax and epilogue of row tile t, by 128 threads with a row each.
+template <int D>
+__device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh, const Waiter &wait, uint32_t tmem) {
+    using C = Cfg<D>;
+    constexpr int NT = C::NT, BN = C::BN;
+    constexpr int part_rows = NT * 128;
+    const AttnLaunch &a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = warp >> 2, r = tid & 127;
+    const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
+    const uint32_t o_base = lane_base + C::O_COL + t * D;
+    uint32_t ns[2] = {0, 0}, no = 0, npv = 0, nj = 0;
+    // all softmax warps of the CTA (bounded, unlike a hardware barrier)
+    auto together = [&] {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.join));
+        return wait(sh.join, nj++ & 1);
+    };
+    for (uint32_t k = 0;; ++k) {
+        if (!wait(sh.seg_full[k % kSegs], (k / kSegs) & 1)) return;
+        const Segment &s = sh.seg[k % kSegs];
+        if (!s.live) return;
+        const bool active = t == 0 || s.n_tok > p.tpt;
+        const bool whole = s.b0 == 0 && s.b1 == s.nb;
+        const int tok = t * p.tpt + r / p.group, head = s.head * p.group + r % p.group;
+        const bool mine = active && r < p.tpt * p.group && tok < s.n_tok;
+        uint16_t *out = a.out + (long long)(s.row0 + tok) * a.out_stride + head * D;
+        if (active) {
+            const KvSpan span = kv_span(s.pos0 + tok, s.len, a.window, a.sinks);
+            // blocks in [all_lo, all_hi) or below all_kept: every row of the tile sees them whole
+            const int all_hi = kv_span(s.pos0 + t * p.tpt, s.len, a.window, a.sinks).hi;
+            const int all_kept = kv_span(s.pos0 + t * p.tpt, s.len, a.window, a.sinks).kept;
+            const int all_lo = kv_span(s.pos0 + min(s.n_tok, (t + 1) * p.tpt) - 1, s.len, a.window, a.sinks).lo;
+            const int b0 = s.b0, b1 = s.b1;
+            const KvBlocks blocks = s.blocks;
+            float m = -INFINITY, l = 0.0f;
+            for (int i = b0; i < b1; ++i) {
+                const int slot = NT == 2 ? t : (i - b0) & 1;
+                const uint32_t s_base = lane_base + slot * C::S_COL;
+                const int j0 = kv_block(blocks, i) * BN;
+                const bool full = j0 + BN <= all_hi && (j0 >= all_lo || j0 + BN <= all_kept);
+                if (!wait(sh.s_full[slot], ns[slot] & 1)) return;
+                ++ns[slot];
+                fence_after();
+                float x[BN];
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_base + 32 * c, x + 32 * c);
+                wait_ld();
+                if (!full) {
+#pragma unroll
+                    for (int c = 0; c < BN / 32; ++c) {
+                        // bit e: the row sees key j0 + 32 c + e
+                        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+                        const int at = j0 + 32 * c;
+                        const uint32_t bits = below(span.hi - at) & (~below(span.lo - at) | below(span.kept - at));
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[32 * c + e] = (bits >> e & 1) ? x[32 * c + e] : -INFINITY;
+                    }
+                }
+                float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int e = 4; e < BN; e += 4)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], x[e + u]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                const bool raise = top > m + kLag;  // the first score above -inf raises from -inf
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float to = raise ? top : m;
+                    const float alpha = m == to ? 1.0f : exp2_fast(m - to);
+                    l *= alpha;
+                    m = to;
+                    if (i > b0) {
+                        if (NT == 1) {
+                            // S of this block only tells that P V of the block before the last is done
+                            if (!wait(sh.pv_done, (npv + (i - b0) - 1) & 1)) return;
+                            fence_after();
+                        }
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(o_base + 16 * c, o);
+                            wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                            tmem_st16(o_base + 16 * c, o);
+                        }
+                    }
+                }
+                const float off = (m == -INFINITY ? 0.0f : -m) + kBias;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) {
+                    uint32_t h[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float w0 = exp2_fast(fmaf(x[32 * c + 2 * e], p.scale_log2, off));
+                        const float w1 = exp2_fast(fmaf(x[32 * c + 2 * e + 1], p.scale_log2, off));
+                        sum[2 * (e & 1)] += w0;
+                        sum[2 * (e & 1) + 1] += w1;
+                        h[e] = f2_to_h2(w0, w1);
+                    }
+                    tmem_st16(s_base + 16 * c, h);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready[slot]));
+            }
+            if (!wait(sh.o_full[t], no & 1)) return;
+            ++no;
+            npv += b1 - b0 - 1;
+            fence_after();
+            if (*reinterpret_cast<const volatile int *>(&s.bad)) l = NAN;  // mended below
+            if (whole) {
+                const float inv = 1.0f / l;
+                bool odd = false;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    float o[32];
+                    tmem_ld32(o_base + 32 * c, o);
+                    wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] *= inv;
+                    odd |= put32(o, out + 32 * c, mine);
+                }
+                mend_rows<D>(p, s, mine && odd, tok, head, lane);
+            } else {
+                // this CTA's part: [value][row], then m and l
+                float *part = a.parts + (size_t)(2 * blockIdx.x + (b0 == 0)) * part_rows * (D + 2) + t * 128 + r;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    float o[32];
+                    tmem_ld32(o_base + 32 * c, o);
+                    wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) part[(size_t)(32 * c + e) * part_rows] = o[e];
+                }
+                part[(size_t)D * part_rows] = m;
+                part[(size_t)(D + 1) * part_rows] = l;
+            }
+        }
+        if (!whole) {
+            // the last CTA that brings a part of the item joins them in order
+            const int first = part_of(sh.plan.total, sh.plan.parts, s.begin);
+            const int last = part_of(sh.plan.total, sh.plan.parts, s.begin + s.nb - 1);
+            __threadfence();
+            if (!together()) return;
+            if (tid == 0) {
+                const unsigned arrived = atomicAdd(a.count + first, 1u);
+                sh.last = arrived == (unsigned)(last - first);
+                if (sh.last) a.count[first] = 0;  // for the next launch
+                __threadfence();
+            }
+            if (!together()) return;
+            const bool join = sh.last != 0;
+            if (!together()) return;
+            if (join && active) {
+                auto part_at = [&](int c) {
+                    return a.parts + (size_t)(2 * c + (c == first)) * part_rows * (D + 2) + t * 128 + r;
+                };
+                float M = -INFINITY, L = 0.0f;
+                for (int c = first; c <= last; ++c) M = fmaxf(M, __ldcg(part_at(c) + (size_t)D * part_rows));
+                for (int c = first; c <= last; ++c) {
+                    const float mc = __ldcg(part_at(c) + (size_t)D * part_rows);
+                    const float lc = __ldcg(part_at(c) + (size_t)(D + 1) * part_rows);
+                    // a part without a score above -inf adds nothing; NaN (a NaN score, a missing page) stays
+                    L += mc == -INFINITY ? (lc != lc ? lc : 0.0f) : exp2_fast(mc - M) * lc;
+                }
+                const float inv = 1.0f / L;
+                bool odd = !(fabsf(inv) <= 3e38f);
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    float o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+#pragma unroll 1
+                    for (int c = first; c <= last; ++c) {
+                        const float *part = part_at(c);
+                        const float mc = __ldcg(part + (size_t)D * part_rows);
+                        const float w = mc == -INFINITY ? 0.0f : exp2_fast(mc - M) * inv;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] += w * __ldcg(part + (size_t)(c0 + e) * part_rows);
+                    }
+                    odd |= put32(o, out + c0, mine);
+                }
+                mend_rows<D>(p, s, mine && odd, tok, head, lane);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.seg_empty[k % kSegs]));
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_constant__ PrefillParams p,
+                                                               const __grid_constant__ CUtensorMap mq,
+                                                               const __grid_constant__ CUtensorMap mk,
+                                                               const __grid_constant__ CUtensorMap mv) {
+    using C = Cfg<D>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ Shared sh;
+    const AttnLaunch &a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    unsigned char *s_q = smem, *s_ring = smem + C::NT * C::Q_TILE;
+    int *seq_tiles = reinterpret_cast<int *>(s_ring + (size_t)p.stages * C::STAGE);
+    unsigned short *order = reinterpret_cast<unsigned short *>(seq_tiles + a.cache.n_seqs + 1);
+
+    pdl_launch_dependents();
+    if (tid == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            mbar_init(smem_u32(&sh.full[i]), 1);
+            mbar_init(smem_u32(&sh.empty[i]), 1);
+        }
+        mbar_init(smem_u32(&sh.q_full), 1);
+        mbar_init(smem_u32(&sh.q_empty), 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(smem_u32(&sh.s_full[t]), 1);
+            mbar_init(smem_u32(&sh.p_ready[t]), 4);
+            mbar_init(smem_u32(&sh.o_full[t]), 1);
+        }
+        mbar_init(smem_u32(&sh.pv_done), 1);
+        mbar_init(smem_u32(&sh.tail), 1);
+        mbar_init(smem_u32(&sh.join), 4 * C::NT);
+        mbar_init(smem_u32(&sh.never), 1);
+        for (int i = 0; i < kSegs; ++i) {
+            mbar_init(smem_u32(&sh.seg_full[i]), 1);
+            mbar_init(smem_u32(&sh.seg_empty[i]), 4 * C::NT + 1);
+        }
+        mbar_init_fence();
+        sh.abort = 0;
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    pdl_wait();
+    make_plan<D>(p, sh, seq_tiles, order, reinterpret_cast<int *>(s_ring));
+    fence_async();  // the ring's memory goes from the plan to the TMA
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sh.tmem;
+    const Waiter wait{sh, p.timeout_ns, a.status};
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 9) {
+            uint32_t n = 0;
+            load_role<D>(p, sh, wait, mq, mk, mv, s_q, s_ring, lane, n);
+            __syncwarp();
+            if (*reinterpret_cast<volatile int *>(&sh.abort)) {
+                // let the copies in flight land before the CTA's memory goes (bounded)
+                const uint64_t t0 = global_timer_ns();
+                for (uint32_t i = n > (uint32_t)p.stages ? n - p.stages : 0; i < n; ++i)
+                    while (!mbar_test_wait(smem_u32(&sh.full[i % p.stages]), (i / p.stages) & 1) &&
+                           global_timer_ns() - t0 < 2000000ull) {
+                    }
+                while (global_timer_ns() - t0 < 50000ull) {
+                }
+            }
+        } else if (warp == 8) {
+            mma_role<D>(p, sh, wait, smem_u32(s_q), smem_u32(s_ring), tmem);
+            __syncwarp();
+            if (*reinterpret_cast<volatile int *>(&sh.abort)) {
+                // let the MMAs in flight end before the accumulators go (bounded)
+                if (elect_one()) commit(smem_u32(&sh.never));
+                __syncwarp();
+                const uint64_t t0 = global_timer_ns();
+                while (!mbar_test_wait(smem_u32(&sh.never), 0) && global_timer_ns() - t0 < 2000000ull) {
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        if (warp < 4 * C::NT) softmax_role<D>(p, sh, wait, tmem);
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// ------------------------------------------------------------------ host
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult r{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeFn>(f);
+    }();
+    return fn;
+}
+
+bool encode(CUtensorMap *m, const void *base, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    return encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, ones,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+cudaError_t launch(PrefillParams &p, cudaStream_t stream) {
+    using C = Cfg<D>;
+    const AttnLaunch &a = p.a;
+    const int page = 1 << a.cache.page_shift;
+    p.box_rows = page < C::BN ? page : C::BN;
+    // most row tiles: one per sequence more than the rows fill
+    const size_t tables = (size_t)(a.cache.n_seqs + 1) * 4 + (size_t)kSortTiles * 2;
+    const size_t room = kSmem - tables - C::NT * C::Q_TILE;
+    p.stages = (int)(room / C::STAGE);
+    if (p.stages > C::MAX_STAGES) p.stages = C::MAX_STAGES;
+    const size_t smem = C::NT * C::Q_TILE + (size_t)p.stages * C::STAGE + tables;
+
+    CUtensorMap mq, mk, mv;
+    const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)a.M};
+    const cuuint64_t qs[2] = {(cuuint64_t)D * 2, (cuuint64_t)a.q_stride * 2};
+    const cuuint32_t qb[3] = {64, (cuuint32_t)p.group, (cuuint32_t)p.tpt};
+    const cuuint64_t kd[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)a.cache.kv_heads, (cuuint64_t)a.cache.n_pages};
+    const cuuint64_t ks[3] = {(cuuint64_t)D * 2, (cuuint64_t)page * D * 2, (cuuint64_t)page * D * 2 * a.cache.kv_heads};
+    const cuuint32_t kb[4] = {64, (cuuint32_t)p.box_rows, 1, 1};
+    if (!encode_fn()) return cudaErrorNotSupported;
+    if (!encode(&mq, a.q, 3, qd, qs, qb) || !encode(&mk, a.cache.k, 4, kd, ks, kb) || !encode(&mv, a.cache.v, 4, kd, ks, kb))
+        return cudaErrorInvalidValue;
+    {
+        static std::mutex mu;
+        static bool configured[64] = {};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev < 0 || dev >= 64 || !configured[dev]) {
+            cudaError_t e = cudaFuncSetAttribute(kq_attn_prefill<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)kSmem);
+            if (e != cudaSuccess) return e;
+            if (dev >= 0 && dev < 64) configured[dev] = true;
+        }
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.num_sms);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = a.pdl ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kq_attn_prefill<D>, p, mq, mk, mv);
+}
+
+}  // namespace
+
+size_t attn_prefill_part_bytes(int num_sms) {
+    size_t most = 0;
+    for (size_t rows_d : {(size_t)256 * (64 + 2), (size_t)256 * (128 + 2), (size_t)128 * (256 + 2)})
+        if (rows_d > most) most = rows_d;
+    return (size_t)2 * num_sms * most * 4;
+}
+
+cudaError_t launch_attn_prefill(const AttnLaunch &L, cudaStream_t stream) {
+    PrefillParams p{};
+    p.a = L;
+    p.scale_log2 = L.scale * 1.4426950408889634f;
+    p.group = L.heads / L.cache.kv_heads;
+    p.tpt = 128 / p.group;
+    p.timeout_ns = L.timeout_ns;
+    p.inject = L.inject;
+    switch (L.cache.head_dim) {
+        case 64: return launch<64>(p, stream);
+        case 128: return launch<128>(p, stream);
+        case 256: return launch<256>(p, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace kq

@@ -595,3 +595,55 @@ def test_empty_prefill(kqctx):
     z = dev(np.zeros(2, np.int32))
     kqctx.attn_prefill_async(kq.Attention(cache, q, torch.empty_like(q), z[:1], q_start=z))
     kqctx.synchronize()
+
+
+def test_prefill_wait_that_runs_out(kqctx):
+    """a wait inside the kernel that nothing completes ends with KQ_ERR_TIMEOUT, and the context stays usable"""
+    rng = np.random.default_rng(0)
+    D, n = 128, 300
+    p = R.Paged(rng, [n], 2, 16, D)
+    q = rng.standard_normal((n, 4, D)).astype(np.float16)
+    out = dev(np.zeros_like(q))
+    ctx = kq.Context(0)
+    try:
+        a = kq.Attention(cache_of(p), dev(q), out, dev(np.array([n], np.int32)), q_start=dev(np.array([0, n], np.int32)))
+        ctx.set_option("timeout_ms", 20)
+        ctx.set_option("inject_timeout", 1)
+        ctx.attn_prefill_async(a)
+        with pytest.raises(kq.KQError) as e:
+            ctx.synchronize()
+        assert e.value.status == -7
+        ctx.set_option("inject_timeout", 0)
+        ctx.set_option("timeout_ms", 1000)
+        ctx.attn_prefill_async(a)
+        ctx.synchronize()
+        want, tol = R.expect(p, q, [(i, 0, i, n) for i in range(n)], 0, 0)
+        close(out.cpu().numpy(), want, tol)
+    finally:
+        ctx.close()
+
+
+@pytest.mark.parametrize("D, H, K, seqs, window", [
+    (128, 8, 2, [(20, 6000)], 0), (64, 4, 4, [(70, 5000), (3, 40)], 0), (256, 8, 2, [(9, 3000), (40, 40)], 0),
+    (128, 4, 1, [(150, 9000)], 0), (128, 4, 1, [(150, 9000), (1, 8000)], 5000), (256, 2, 1, [(200, 4000)], 0), (64, 16, 1, [(30, 7001)], 6000),
+])
+def test_prefill_long_cache(kqctx, D, H, K, seqs, window):
+    """few rows over long caches: the keys of an item are split over CTAs and joined"""
+    rng = np.random.default_rng(D + H)
+    p = R.Paged(rng, [b for _, b in seqs], K, 32, D)
+    start = np.cumsum([0] + [a for a, _ in seqs]).astype(np.int32)
+    q = (1.5 * rng.standard_normal((int(start[-1]), H, D))).astype(np.float16)
+    out = dev(np.full_like(q, SENTINEL))
+    a = kq.Attention(cache_of(p), dev(q), out, dev(np.array([b for _, b in seqs], np.int32)), q_start=dev(start), window=window,
+                     sinks=7 if window else 0)
+    kqctx.attn_prefill_async(a)
+    kqctx.synchronize()
+    rows = [(start[s] + i, s, b - n + i, b) for s, (n, b) in enumerate(seqs) for i in range(n)]
+    rows = [rows[i] for i in sorted({0, 1, len(rows) - 1, len(rows) - 2, *rng.integers(0, len(rows), 25).tolist()})]
+    want, tol = R.expect(p, q, rows, window, 7 if window else 0)
+    close(out.cpu().numpy()[[r[0] for r in rows]], want, tol)
+    first = out.clone()
+    for _ in range(3):
+        kqctx.attn_prefill_async(a)
+    kqctx.synchronize()
+    assert (out == first).all()
