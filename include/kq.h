@@ -261,7 +261,7 @@ typedef struct kq_kv_cache {
     int kv_heads;
     int head_dim;
     int n_seqs;                 /* 1..KQ_MAX_SEQS */
-    int table_stride;           /* table entries per sequence */
+    int table_stride;           /* table entries per sequence; table_stride * page_size <= 2^30, times n_seqs <= 2^34 */
 } kq_kv_cache;
 
 /* One set of heads of M rows: in -> out (the same buffer and stride, or one that does not

@@ -32,6 +32,10 @@ namespace {
 // down to 2^-22 of the largest instead of 2^-14; sums stay fp32.
 constexpr float kBias = 8.0f;
 constexpr int kUnit = 16;  // keys of a unit; a page holds a multiple of it
+// Beginning an item (its queries, its first page) costs a warp about as much as this many units:
+// every item counts that many more when the work is cut, or the warps with the short sequences
+// would end last.
+constexpr int kBegin = 2;
 
 template <int D, int NB>
 struct Cfg {
@@ -44,15 +48,19 @@ struct DecodeParams {
     AttnLaunch a;
     float scale_log2;
     int group, rows, splits;  // query heads of a key head; of an item; items of a key head
+    int part_floats;          // floats of a part: rows x (D + 2), to a multiple of 16 bytes
+    int floats;               // shared memory before the tables
     float *parts;             // [CTA][2] parts of rows x D values, then [rows][2] (m, l)
     unsigned *count;          // [CTA] arrivals at the item that begins in a CTA and ends in a later one
 };
 
-__device__ __forceinline__ uint4 load_stream(const uint16_t *p) {
+// The cache streams through: first to leave L2, so that what is used again (the kernel's code, the
+// tables, the parts) stays there.
+__device__ __forceinline__ uint4 load_stream(const uint16_t *p, uint64_t policy) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
+                 : "l"(p), "l"(policy));
     return v;
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -79,48 +87,88 @@ __device__ __forceinline__ float sum_over_keys(float v) {
     return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
 
-// The units of one item that a warp takes, and its place in them.
-struct Item {
-    int seq, vhead, tiles;       // sequence, item of the sequence (key head x splits), units of it
-    long long begin;             // its first unit
+// Total units cut into `parts` contiguous shares that differ by one at most.
+struct Shares {
+    long long q;          // total / parts
+    unsigned r, parts;    // total % parts
+    float inv;            // about parts / total
+    __device__ __forceinline__ Shares(long long total, int n) : parts((unsigned)n) {
+        if (total < 0xffffffffll) {  // 32-bit division where it will do
+            q = (unsigned)total / parts;
+        } else {
+            q = total / n;
+        }
+        r = (unsigned)(total - q * n);
+        inv = (float)n / (float)total;
+    }
+    __device__ __forceinline__ long long begin(int c) const { return q * c + (r * (unsigned)c) / parts; }
+    __device__ __forceinline__ int of(long long u) const {
+        int c = min((int)((float)u * inv), (int)parts - 1);
+        while (c + 1 < (int)parts && begin(c + 1) <= u) ++c;
+        while (c > 0 && begin(c) > u) --c;
+        return c;
+    }
 };
 
-// prefix[s]: units of one item of sequences 0..s-1; `per` items a sequence
-__device__ __forceinline__ Item item_of(const long long *prefix, int n_seqs, int per, long long unit) {
+struct Item {
+    int seq, vhead, cost;  // sequence, item of the sequence (key head x splits), kBegin + its units
+    long long begin;       // where its cost begins; its first unit stands kBegin later
+};
+
+// prefix[s]: cost of one item of each of the sequences 0..s-1; `per` items a sequence
+__device__ __forceinline__ Item item_of(const int *prefix, int n_seqs, int per, long long unit) {
     int lo = 0, hi = n_seqs;  // prefix[lo] * per <= unit < prefix[hi] * per
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (prefix[mid] * per <= unit) lo = mid;
+        if ((long long)prefix[mid] * per <= unit) lo = mid;
         else hi = mid;
     }
     Item it;
     it.seq = lo;
-    it.tiles = (int)(prefix[lo + 1] - prefix[lo]);
-    const long long r = unit - prefix[lo] * per;
-    it.vhead = (int)(r / it.tiles);
-    it.begin = prefix[lo] * per + (long long)it.vhead * it.tiles;
+    it.cost = prefix[lo + 1] - prefix[lo];
+    const long long first = (long long)prefix[lo] * per, r = unit - first;
+    it.vhead = (int)((float)r / (float)it.cost);  // at most 2^9: one off at most
+    if ((long long)it.vhead * it.cost > r) --it.vhead;
+    if ((long long)(it.vhead + 1) * it.cost <= r) ++it.vhead;
+    it.begin = first + (long long)it.vhead * it.cost;
     return it;
 }
 
-// How a part with nothing above -inf is marked: m = -inf, and l = 0 when it saw no key, +inf when
-// every score was -inf, NaN when one was NaN.
-struct Join {
-    float M, L;
-    bool seen;
-};
-__device__ __forceinline__ void join_max(Join &j, float m) { j.M = fmaxf(j.M, m); }
-// weight of a part, its l added
-__device__ __forceinline__ float join_add(Join &j, float m, float l) {
-    if (m == -INFINITY) {
-        if (l != l) j.L = l;
-        else if (l > 0.0f) j.seen = true;
-        return 0.0f;
+// Parts of a row joined one after another: four of its values.  A part with nothing above -inf is
+// marked: m = -inf, and l = 0 when it saw no key, +inf when every score was -inf, NaN when one was NaN.
+struct Joint {
+    float M = -INFINITY, L = 0.0f;
+    bool seen = false;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __device__ __forceinline__ void add(float2 ml, float4 x) {
+        const float top = fmaxf(M, ml.x);
+        const float old = M == -INFINITY ? 1.0f : exp2f(M - top);  // before the first score: L is 0 or NaN, v is 0
+        const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
+        L = L * old + (ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.0f) : w * ml.y);
+        v.x = v.x * old + w * x.x;
+        v.y = v.y * old + w * x.y;
+        v.z = v.z * old + w * x.z;
+        v.w = v.w * old + w * x.w;
+        M = top;
+        seen |= ml.x > -INFINITY || ml.y > 0.0f;
     }
-    j.seen = true;
-    const float w = exp2f(m - j.M);
-    j.L += w * l;
-    return w;
-}
+    __device__ __forceinline__ float2 mark() const {
+        return make_float2(M, M == -INFINITY && seen && L == 0.0f ? INFINITY : L);
+    }
+    // scores all -inf: 0 / 0, NaN as in the formula; no key there: zeros
+    __device__ __forceinline__ uint2 result() const {
+        if (!seen && L == L) return make_uint2(0u, 0u);
+        const float inv = 1.0f / L;
+        return make_uint2(f2_to_h2(v.x * inv, v.y * inv), f2_to_h2(v.z * inv, v.w * inv));
+    }
+};
+
+// A warp's part of an item: which one, where its rows go, and the item's units.
+struct PartInfo {
+    int id;  // -1: none
+    int seq, head0, n_rows;
+    long long begin, end;  // of its units
+};
 
 template <int D, int NB>
 __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const __grid_constant__ DecodeParams p) {
@@ -128,15 +176,18 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
     constexpr int KC = D / 32;  // 16-byte pieces of a key row per lane
     constexpr int VC = D / 64;  // of a value row
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ long long s_warp[C::WARPS];
-    __shared__ int s_item[2 * C::WARPS];  // item of each warp's first and last part (-1: none)
-    __shared__ int s_last;
+    __shared__ int s_warp[C::WARPS];
+    __shared__ PartInfo s_part[2 * C::WARPS];  // each warp's first and last part
+    __shared__ uint32_t s_run[2 * C::WARPS];  // the parts of each item, as bits
+    __shared__ int s_runs;                    // items that have parts
+    __shared__ int s_last[2];
     const AttnLaunch &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int S = a.cache.n_seqs, per = a.cache.kv_heads * p.splits;
-    const int part_floats = p.rows * (D + 2);
+    const int part_floats = p.part_floats;
     float *s_parts = reinterpret_cast<float *>(smem);
-    long long *prefix = reinterpret_cast<long long *>(smem + (size_t)2 * C::WARPS * part_floats * 4);
+    int *prefix = reinterpret_cast<int *>(s_parts + p.floats);
+    int *lens = prefix + S + 1;
 
     pdl_launch_dependents();
     pdl_wait();
@@ -144,50 +195,55 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
     // units of every sequence, and where they begin
     {
         const int chunk = (S + C::THREADS - 1) / C::THREADS, s0 = tid * chunk;
-        long long sum = 0;
+        int sum = 0;
         for (int s = s0; s < s0 + chunk && s < S; ++s) {
             bool bad = false;
             const int len = kv_length(a.cache, __ldg(a.kv_len + s), bad);
+            lens[s] = len;
             if (bad && blockIdx.x == 0) report_error(a.status, DEV_ERR_CACHE);
             const KvSpan sp = kv_span(len - 1, len, a.window, a.sinks);
             const int n = kv_blocks(sp.kept, sp.lo, sp.hi, kUnit).count;
             prefix[s] = sum;
-            sum += n;
+            sum += n ? n + kBegin : 0;
             if (n == 0 && s % gridDim.x == blockIdx.x)  // sees nothing: zeros
                 for (int i = 0; i < a.heads * D / 8; ++i)
                     *reinterpret_cast<uint4 *>(a.out + s * a.out_stride + 8 * i) = make_uint4(0, 0, 0, 0);
         }
-        long long run = sum;
+        int run = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const long long o = __shfl_up_sync(0xffffffffu, run, d);
+            const int o = __shfl_up_sync(0xffffffffu, run, d);
             if (lane >= d) run += o;
         }
         if (lane == 31) s_warp[warp] = run;
-        if (tid < 2 * C::WARPS) s_item[tid] = -1;
+        if (tid < 2 * C::WARPS) s_part[tid].id = -1;
         __syncthreads();
-        long long base = run - sum;
+        int base = run - sum;
         for (int w = 0; w < warp; ++w) base += s_warp[w];
         for (int s = s0; s < s0 + chunk && s < S; ++s) prefix[s] += base;
         if (tid == C::THREADS - 1) prefix[S] = base + sum;
         __syncthreads();
     }
-    const long long total = prefix[S] * per;
+    const long long total = (long long)prefix[S] * per;
     // no more CTAs than give every warp a unit
     const int parts = (int)min((long long)gridDim.x, (total + C::WARPS - 1) / C::WARPS);
     if ((int)blockIdx.x >= parts) return;
-    const long long c0 = part_begin(total, parts, blockIdx.x), c1 = part_begin(total, parts, blockIdx.x + 1);
-    const long long w0 = c0 + part_begin(c1 - c0, C::WARPS, warp), w1 = c0 + part_begin(c1 - c0, C::WARPS, warp + 1);
+    const Shares shares(total, parts);
+    const long long c0 = shares.begin(blockIdx.x), c1 = shares.begin(blockIdx.x + 1);
+    const Shares mine_shares(c1 - c0, C::WARPS);
+    const long long w0 = c0 + mine_shares.begin(warp), w1 = c0 + mine_shares.begin(warp + 1);
 
+    const uint64_t policy = l2_evict_first_policy();
     int slot = 0;  // this warp's next part in shared memory
     for (long long unit = w0; unit < w1;) {
         const Item it = item_of(prefix, S, per, unit);
         const int kv_head = it.vhead / p.splits, row0 = (it.vhead % p.splits) * p.rows;
         const int n_rows = min(p.rows, p.group - row0);
-        const int t0 = (int)(unit - it.begin), t1 = (int)min((long long)it.tiles, w1 - it.begin);
-        unit = it.begin + t1;
-        bool bad = false;
-        const int len = kv_length(a.cache, __ldg(a.kv_len + it.seq), bad);
+        const int to = (int)min((long long)it.cost, w1 - it.begin);
+        const int t0 = max((int)(unit - it.begin) - kBegin, 0), t1 = max(to - kBegin, 0);
+        unit = it.begin + to;
+        if (t0 == t1) continue;  // nothing but the item's beginning
+        const int len = lens[it.seq];
         const KvSpan span = kv_span(len - 1, len, a.window, a.sinks);
         const KvBlocks blocks = kv_blocks(span.kept, span.lo, span.hi, kUnit);
         const int head0 = kv_head * p.group + row0;
@@ -226,15 +282,15 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
             const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                kr[0][c] = k0 ? load_stream(kp + g * D + 32 * c) : zero;
-                kr[1][c] = k1 ? load_stream(kp + (g + 8) * D + 32 * c) : zero;
+                kr[0][c] = k0 ? load_stream(kp + g * D + 32 * c, policy) : zero;
+                kr[1][c] = k1 ? load_stream(kp + (g + 8) * D + 32 * c, policy) : zero;
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int key = 2 * t + (u & 1) + 4 * (u & 2);
                 const bool vis = full || kv_sees(span, j0 + key);
 #pragma unroll
-                for (int c = 0; c < VC; ++c) vr[u][c] = vis ? load_stream(vp + key * D + 64 * c) : zero;
+                for (int c = 0; c < VC; ++c) vr[u][c] = vis ? load_stream(vp + key * D + 64 * c, policy) : zero;
             }
             seen = true;
             uint32_t pb[NB][2];
@@ -286,7 +342,7 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
         }
 
         // o[b][4c + jj]: dimensions 64c + 8g + 2jj (elements 0, 1) and the next (2, 3), rows 2t (0, 2), 2t+1 (1, 3)
-        const bool whole = t0 == 0 && t1 == it.tiles;
+        const bool whole = t0 == 0 && t1 == it.cost - kBegin;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -320,7 +376,7 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
                 }
             }
         if (!whole) {
-            if (lane == 0) s_item[2 * warp + slot] = it.seq * per + it.vhead;
+            if (lane == 0) s_part[2 * warp + slot] = PartInfo{it.seq * per + it.vhead, it.seq, head0, n_rows, it.begin + kBegin, it.begin + it.cost};
             ++slot;
         }
     }
@@ -328,97 +384,100 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
 
     // Join the warps' parts of each item (they stand in unit order): into the output, or into this
     // CTA's part of an item that other CTAs share too.
-    int shared_item[2] = {-1, -1};  // the item that began before this CTA, the one that goes on after it
-    for (int i0 = 0; i0 < 2 * C::WARPS;) {
-        const int id = s_item[i0];
-        if (id < 0) {
-            ++i0;
-            continue;
-        }
-        int i1 = i0 + 1;  // parts [i0, i1) that are there and of this item
-        while (i1 < 2 * C::WARPS && (s_item[i1] == id || s_item[i1] < 0)) ++i1;
-        const int seq = id / per, vh = id % per;
-        const int tiles = (int)(prefix[seq + 1] - prefix[seq]);
-        const long long b0 = prefix[seq] * per + (long long)vh * tiles, b1 = b0 + tiles;
-        const bool mine = b0 >= c0 && b1 <= c1;
-        const int which = b0 < c0 ? 0 : 1;
-        if (!mine) shared_item[which] = id;
-        const int row0 = (vh % p.splits) * p.rows, n_rows = min(p.rows, p.group - row0);
-        const int head0 = (vh / p.splits) * p.group + row0;
-        float *out_part = p.parts + (size_t)(2 * blockIdx.x + which) * part_floats;
-        for (int e = tid; e < n_rows * (D / 2); e += C::THREADS) {
-            const int r = e / (D / 2), d = 2 * (e % (D / 2));
-            Join jn = {-INFINITY, 0.0f, false};
-            for (int i = i0; i < i1; ++i)
-                if (s_item[i] == id) join_max(jn, s_parts[(size_t)i * part_floats + p.rows * D + 2 * r]);
-            float2 acc = make_float2(0.0f, 0.0f);
-            for (int i = i0; i < i1; ++i) {
-                if (s_item[i] != id) continue;
-                const float *part = s_parts + (size_t)i * part_floats;
-                const float w = join_add(jn, part[p.rows * D + 2 * r], part[p.rows * D + 2 * r + 1]);
-                if (w == 0.0f) continue;
-                const float2 v = *reinterpret_cast<const float2 *>(part + r * D + d);
-                acc.x += w * v.x;
-                acc.y += w * v.y;
-            }
-            if (mine) {
-                const float inv = 1.0f / jn.L;
-                *reinterpret_cast<uint32_t *>(a.out + seq * a.out_stride + (head0 + r) * D + d) =
-                    (jn.seen || jn.L != jn.L) ? f2_to_h2(acc.x * inv, acc.y * inv) : 0u;
-            } else {
-                *reinterpret_cast<float2 *>(out_part + r * D + d) = acc;
-                if (d == 0) {
-                    out_part[p.rows * D + 2 * r] = jn.M;
-                    out_part[p.rows * D + 2 * r + 1] = (jn.M == -INFINITY && jn.seen && jn.L == 0.0f) ? INFINITY : jn.L;
-                }
-            }
-        }
-        i0 = i1;
+    if (warp == 0) {
+        const int id = lane < 2 * C::WARPS ? s_part[lane].id : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, id);
+        const bool lead = id >= 0 && lane == __ffs(same) - 1;
+        const uint32_t leads = __ballot_sync(0xffffffffu, lead);
+        if (lead) s_run[__popc(leads & ((1u << lane) - 1u))] = same;
+        if (lane == 0) s_runs = __popc(leads);
     }
+    __syncthreads();
+    const int elems = p.rows * (D / 4);  // a thread takes four values of a row
+    const int runs = s_runs;
+    // the item that began before this CTA, and the one that goes on after it: their parts (-1: none)
+    int before = -1, after = -1;
+    if (runs > 0) {
+        const int i0 = __ffs(s_run[0]) - 1, i1 = __ffs(s_run[runs - 1]) - 1;
+        if (s_part[i0].begin < c0) before = i0;
+        if (s_part[i1].end > c1 && s_part[i1].begin >= c0) after = i1;
+    }
+    for (int e = tid; e < runs * elems; e += C::THREADS) {
+        uint32_t bits = s_run[e / elems];
+        const int lead = __ffs(bits) - 1;
+        const int r = (e % elems) / (D / 4), d = 4 * (e % (D / 4));
+        const PartInfo &info = s_part[lead];
+        if (r >= info.n_rows) continue;
+        Joint jn;
+#pragma unroll 1
+        for (; bits; bits &= bits - 1) {
+            const float *part = s_parts + (size_t)(__ffs(bits) - 1) * part_floats;
+            jn.add(*reinterpret_cast<const float2 *>(part + p.rows * D + 2 * r), *reinterpret_cast<const float4 *>(part + r * D + d));
+        }
+        if (lead == before || lead == after) {
+            float *part = p.parts + (size_t)(2 * blockIdx.x + (lead == before ? 0 : 1)) * part_floats;
+            *reinterpret_cast<float4 *>(part + r * D + d) = jn.v;
+            if (d == 0) *reinterpret_cast<float2 *>(part + p.rows * D + 2 * r) = jn.mark();
+        } else {
+            *reinterpret_cast<uint2 *>(a.out + info.seq * a.out_stride + (info.head0 + r) * D + d) = jn.result();
+        }
+    }
+    if (before < 0 && after < 0) return;  // uniform over the CTA
 
     // Items shared with other CTAs: the last to arrive joins their parts in unit order.
+    int first[2] = {0, 0}, last[2] = {0, 0};
+    if (before >= 0) {
+        first[0] = shares.of(s_part[before].begin);
+        last[0] = s_part[before].end > c1 ? shares.of(s_part[before].end - 1) : (int)blockIdx.x;
+    }
+    if (after >= 0) {
+        first[1] = blockIdx.x;
+        last[1] = shares.of(s_part[after].end - 1);
+    }
+    __syncthreads();
+    if (tid < 2) {
+        int is_last = 0;
+        if ((tid ? after : before) >= 0) {
+            const int f = tid ? first[1] : first[0], l = tid ? last[1] : last[0];
+            // after the barrier: the release covers the whole CTA's part
+            is_last = count_arrival(p.count + f) == (unsigned)(l - f);
+            if (is_last) p.count[f] = 0;  // for the next launch
+        }
+        s_last[tid] = is_last;
+    }
+    __syncthreads();
+    const int groups = elems < C::THREADS ? C::THREADS / elems : 1;  // threads left over share the parts
+    float2 *s_ml = reinterpret_cast<float2 *>(s_parts + 4 * C::THREADS);
+    float4 *s_v = reinterpret_cast<float4 *>(s_parts);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-        const int id = shared_item[which];
-        if (id < 0) continue;  // uniform over the CTA
-        const int seq = id / per, vh = id % per;
-        const int tiles = (int)(prefix[seq + 1] - prefix[seq]);
-        const long long b0 = prefix[seq] * per + (long long)vh * tiles;
-        const int first = part_of(total, parts, b0), last = part_of(total, parts, b0 + tiles - 1);
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-            const unsigned n = atomicAdd(p.count + first, 1u);
-            s_last = n == (unsigned)(last - first);
-            if (s_last) p.count[first] = 0;  // for the next launch
-            __threadfence();
-        }
-        __syncthreads();
-        if (!s_last) continue;
-        const int row0 = (vh % p.splits) * p.rows, n_rows = min(p.rows, p.group - row0);
-        const int head0 = (vh / p.splits) * p.group + row0;
-        for (int e = tid; e < n_rows * (D / 2); e += C::THREADS) {
-            const int r = e / (D / 2), d = 2 * (e % (D / 2));
-            Join jn = {-INFINITY, 0.0f, false};
+        if (!s_last[which]) continue;  // uniform over the CTA
+        const PartInfo info = s_part[which ? after : before];
+        const int f = first[which], n = last[which] - f + 1;
+        for (int e0 = 0; e0 < elems; e0 += C::THREADS) {
+            const int e = groups > 1 ? tid % elems : e0 + tid, grp = groups > 1 ? tid / elems : 0;
+            const int r = e / (D / 4), d = 4 * (e % (D / 4));
+            const bool on = e < elems && grp < groups && r < info.n_rows;
+            Joint jn;
+            if (on) {
 #pragma unroll 4
-            for (int c = first; c <= last; ++c)
-                join_max(jn, __ldcg(p.parts + (size_t)(2 * c + (c == first)) * part_floats + p.rows * D + 2 * r));
-            float2 acc = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-            for (int c = first; c <= last; ++c) {
-                const float *part = p.parts + (size_t)(2 * c + (c == first)) * part_floats;
-                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part + p.rows * D + 2 * r));
-                const float2 v = __ldcg(reinterpret_cast<const float2 *>(part + r * D + d));
-                const float w = join_add(jn, ml.x, ml.y);
-                if (w != 0.0f) {
-                    acc.x += w * v.x;
-                    acc.y += w * v.y;
+                for (int i = grp; i < n; i += groups) {
+                    const float *part = p.parts + (size_t)(2 * (f + i) + (i == 0)) * part_floats;
+                    jn.add(__ldcg(reinterpret_cast<const float2 *>(part + p.rows * D + 2 * r)),
+                           __ldcg(reinterpret_cast<const float4 *>(part + r * D + d)));
+                }
+                if (grp > 0) {
+                    s_v[tid] = jn.v;
+                    s_ml[tid] = jn.mark();
                 }
             }
-            const float inv = 1.0f / jn.L;
-            *reinterpret_cast<uint32_t *>(a.out + seq * a.out_stride + (head0 + r) * D + d) =
-                (jn.seen || jn.L != jn.L) ? f2_to_h2(acc.x * inv, acc.y * inv) : 0u;
+            if (groups > 1) __syncthreads();
+            if (on && grp == 0) {
+                for (int k = 1; k < groups; ++k) jn.add(s_ml[k * elems + e], s_v[k * elems + e]);
+                *reinterpret_cast<uint2 *>(a.out + info.seq * a.out_stride + (info.head0 + r) * D + d) = jn.result();
+            }
         }
+        __syncthreads();
     }
 }
 
@@ -427,7 +486,11 @@ cudaError_t launch(DecodeParams &p, cudaStream_t stream) {
     using C = Cfg<D, NB>;
     p.rows = p.group < 8 * NB ? p.group : 8 * NB;
     p.splits = (p.group + p.rows - 1) / p.rows;
-    const size_t smem = (size_t)2 * C::WARPS * p.rows * (D + 2) * 4 + (size_t)(p.a.cache.n_seqs + 1) * 8;
+    // the warps' parts; later, in the same place, the threads' sums of a join
+    p.part_floats = (p.rows * (D + 2) + 3) & ~3;
+    const size_t room = (size_t)2 * C::WARPS * p.part_floats * 4, join = (size_t)C::THREADS * 24;
+    p.floats = (int)((room > join ? room : join) / 4);
+    const size_t smem = (size_t)p.floats * 4 + (size_t)(2 * p.a.cache.n_seqs + 1) * 4;
     {
         static std::mutex mu;
         static bool configured[64] = {};

@@ -12,6 +12,14 @@ __device__ __forceinline__ uint32_t f2_to_h2(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// One more arrival at a counter other CTAs count on too: releases this thread's (and, after a barrier,
+// its CTA's) writes, acquires those of the arrivals before it, whose number it returns.
+__device__ __forceinline__ unsigned count_arrival(unsigned *count) {
+    unsigned n;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(count) : "memory");
+    return n;
+}
+
 // The page that holds position j of sequence seq, or -1 (and an error) where the table names none.
 __device__ __forceinline__ int kv_page(const KvView &c, int seq, int j, int *status) {
     const int page = __ldg(c.table + (long long)seq * c.table_stride + (j >> c.page_shift));

@@ -755,13 +755,11 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
             // the last CTA that brings a part of the item joins them in order
             const int first = part_of(sh.plan.total, sh.plan.parts, s.begin);
             const int last = part_of(sh.plan.total, sh.plan.parts, s.begin + s.nb - 1);
-            __threadfence();
             if (!together()) return;
             if (tid == 0) {
-                const unsigned arrived = atomicAdd(a.count + first, 1u);
-                sh.last = arrived == (unsigned)(last - first);
+                // after the barrier: the release covers all of the CTA's rows
+                sh.last = count_arrival(a.count + first) == (unsigned)(last - first);
                 if (sh.last) a.count[first] = 0;  // for the next launch
-                __threadfence();
             }
             if (!together()) return;
             const bool join = sh.last != 0;

@@ -146,6 +146,10 @@ inline int check_cache(const kq_kv_cache *c, const char **why) {
         *why = "a sequence may reach 2^30 positions at most";
         return KQ_ERR_SHAPE;
     }
+    if ((long long)c->n_seqs * c->table_stride * c->page_size > (1ll << 34)) {
+        *why = "the table may reach 2^34 positions at most";
+        return KQ_ERR_SHAPE;
+    }
     return KQ_OK;
 }
 

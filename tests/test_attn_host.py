@@ -152,6 +152,7 @@ INVALID, SHAPE = -1, -3
     (dict(page_size=8), SHAPE), (dict(page_size=512), SHAPE), (dict(page_size=48), SHAPE), (dict(page_size=-16), SHAPE),
     (dict(kv_heads=0), SHAPE), (dict(kv_heads=257), SHAPE), (dict(n_pages=0), SHAPE), (dict(n_seqs=0), SHAPE),
     (dict(n_seqs=4097), SHAPE), (dict(table_stride=0), SHAPE), (dict(table_stride=2 ** 27), SHAPE), (dict(table_stride=2 ** 26), 0),
+    (dict(table_stride=2 ** 26, n_seqs=16), 0), (dict(table_stride=2 ** 26, n_seqs=17), SHAPE),
 ])
 def test_cache_refusals(host, change, status):
     assert host.c_cache(C.byref(cache_struct(**change))) == status
