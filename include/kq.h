@@ -285,8 +285,8 @@ int kq_qk_norm_rope_async(kq_ctx *ctx, const kq_rope *rope, int head_dim, int M,
 /* Row i's keys and values go to position pos_dev[i] of sequence seq_dev[i] (int32 each), the keys
  * normed and rotated on the way as above, the values as they are; q (may be NULL) is normed and
  * rotated like kq_qk_norm_rope_async in the same launch.  k->heads = v->heads = cache->kv_heads;
- * k->out and v->out are NULL, v->gamma too.  A row with seq_dev[i] < 0 is padding: nothing of it is
- * read or written.  A row whose sequence, position or page lies outside the cache is left out in the
+ * k->out and v->out are NULL, v->gamma too.  A row with seq_dev[i] < 0 is padding: nothing of it
+ * goes anywhere.  A row whose sequence, position or page lies outside the cache is left out in the
  * same way (q included) and the next kq_synchronize reports KQ_ERR_SHAPE.  No two rows of a call
  * may name the same position of the same page. */
 int kq_kv_append_async(kq_ctx *ctx, const kq_kv_cache *cache, const kq_rope *rope, int M, const int32_t *seq_dev,

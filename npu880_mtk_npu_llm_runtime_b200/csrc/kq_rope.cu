@@ -3,15 +3,15 @@
 // One kernel for both calls (kq_qk_norm_rope_async, kq_kv_append_async): a head x of D values
 // becomes  y = x * gamma / sqrt(mean(x^2) + eps)  and pair (a, b) of y at position p turns by
 // t = p * f:  (a cos t - b sin t, a sin t + b cos t).  Values are copied.
-#include "kq_common.cuh"
-#include "kq_attn.h"
+#include "kq_attn_dev.cuh"
 
 namespace kq {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxPasses = 4;  // heads of a row that one CTA takes: up to this many per thread group
+constexpr int kThreads = 128;
+constexpr int kCtasPerSm = 7;  // all rows of a call (4,096 at most) resident at once, one warp each: no second wave
+constexpr int kInFlight = 4;  // passes whose loads a lane issues at once, one batch ahead of the arithmetic
 
 struct RowSet {
     const __half *in;
@@ -23,150 +23,184 @@ struct RowSet {
 };
 
 struct RopeParams {
-    RowSet q, k, v;  // heads in this order; heads = 0: none
+    RowSet q, k, v;  // heads = 0: none
     KvView cache;    // table == nullptr: no append
     const int32_t *seq, *pos;
     int *status;
     float eps;
-    int rot, adjacent, passes;
+    int M, rot, adjacent, chunks;
     double turns[KQ_MAX_HEAD_DIM / 2];  // full turns per position: inv_freq / (2 pi)
 };
 
-__device__ __forceinline__ float2 h2f(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
-__device__ __forceinline__ uint32_t f2h(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
+__device__ __forceinline__ uint4 load_row(const __half *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
 }
 
-// Grid: (rows, chunks of heads).  LPH lanes hold a head, 8 values (16 bytes) each, so a warp takes
-// 32 / LPH heads and all its loads and stores are whole 16-byte vectors.  cos and sin of a
-// position are the same for every head of the row: computed once per CTA into shared memory.
-// The angle is p * f / (2 pi) turns in fp64 less its nearest integer (positions of a million keep
-// 1e-10 of a turn; fp32 would be off by whole radians), then sin / cos of the fraction in fp32.
-template <int D>
-__global__ __launch_bounds__(kThreads) void kq_norm_rope(const __grid_constant__ RopeParams p) {
-    constexpr int LPH = D / 8;
-    constexpr int HPP = kThreads / LPH;  // heads per pass
-    __shared__ __align__(16) float s_cos[D / 2], s_sin[D / 2];
-    const int tid = threadIdx.x, lane = tid & 31, l = tid % LPH;
-    const int row = blockIdx.x;
-    pdl_launch_dependents();
-    pdl_wait();
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 
-    int seq = 0, pos = 0, page = 0;
-    if (p.pos) pos = p.pos[row];
+// A warp takes one row, or (few rows) a chunk of one row's heads; LPH lanes hold a head, 8 values
+// (16 bytes) each, so every access is a whole vector and a warp has 32 / LPH heads per pass.
+//
+// cos and sin of the row's position are the same for all heads: the warp's lanes compute them once
+// (the angle is p * f / (2 pi) turns in fp64 less its nearest integer -- positions of a million
+// keep 1e-10 of a turn, where fp32 would be off by whole radians -- then the fraction's sine and
+// cosine in fp32).  With gamma they make two factors for each of a lane's values x and the other
+// value z of its pair: y = (x A + z B) / sqrt(mean(x^2) + eps), so a head costs little more than
+// its loads, conversions and the sum of squares.
+//
+// Bound by the bytes, 2 in and 2 out per value, and close behind by the instructions.  4,096 rows of
+// 40 heads of 128 (84 MB): 19 us, 4.4 TB/s; a CTA per row that applied gamma, cos and sin to every
+// head took 29; 6 CTAs an SM (more registers, but a second wave of 0.15) 24; batches of 2 passes 20.
+template <int D>
+__global__ __launch_bounds__(kThreads, kCtasPerSm) void kq_norm_rope(const __grid_constant__ RopeParams p) {
+    constexpr int LPH = D / 8, HPP = 32 / LPH;
+    __shared__ __align__(16) float s_cos[kThreads / 32][D / 2], s_sin[kThreads / 32][D / 2];
+    __shared__ double s_turns[D / 2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LPH, sub = lane / LPH;
+    const int task = blockIdx.x * (kThreads / 32) + warp, row = task / p.chunks, chunk = task % p.chunks;
+    pdl_launch_dependents();
+    // (read from the parameters lane by lane, each lane another address, these would be serial for every warp)
+    if (threadIdx.x < p.rot / 2) s_turns[threadIdx.x] = p.turns[threadIdx.x];
+    __syncthreads();
+    pdl_wait();
+    if (row >= p.M) return;
+    // passes of q, k and v one after another; this warp's share of them
+    const int nq = (p.q.heads + HPP - 1) / HPP, nk = (p.k.heads + HPP - 1) / HPP, nv = (p.v.heads + HPP - 1) / HPP;
+    const int n0 = (nq + nk + nv) * chunk / p.chunks, n1 = (nq + nk + nv) * (chunk + 1) / p.chunks;
+    // loads of the passes from n on, of n's set
+    auto load = [&](int n, uint4 (&x)[kInFlight]) {
+        const bool is_q = n < nq, is_k = !is_q && n < nq + nk;
+        const RowSet &s = is_q ? p.q : is_k ? p.k : p.v;
+        const int i0 = is_q ? n : is_k ? n - nq : n - nq - nk;
+        const __half *in = s.in + (long long)row * s.in_stride + 8 * l;
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) {
+            const int h = (i0 + i) * HPP + sub;
+            x[i] = n + i < n1 && h < s.heads ? load_row(in + h * D) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    uint4 ahead[kInFlight];  // the first heads are on their way while the angles are computed
+    load(n0, ahead);
+
+    int pos = 0, page = 0;
+    if (p.pos) pos = __ldg(p.pos + row);
     if (p.cache.table) {
-        seq = p.seq[row];
-        if (seq < 0) return;  // padding (uniform over the CTA)
+        const int seq = __ldg(p.seq + row);
+        if (seq < 0) return;  // padding
         bool ok = seq < p.cache.n_seqs && pos >= 0 && pos < kv_reach(p.cache);
         if (ok) {
-            page = p.cache.table[(long long)seq * p.cache.table_stride + (pos >> p.cache.page_shift)];
+            page = __ldg(p.cache.table + (long long)seq * p.cache.table_stride + (pos >> p.cache.page_shift));
             ok = kv_page_ok(p.cache, page);
         }
         if (!ok) {
-            if (tid == 0) report_error(p.status, DEV_ERR_CACHE);
+            if (lane == 0) report_error(p.status, DEV_ERR_CACHE);
             return;
         }
     }
-    const int total = p.q.heads + p.k.heads + p.v.heads;
-    const int h0 = blockIdx.y * p.passes * HPP + tid / LPH;
-
-    uint4 x[kMaxPasses];
-#pragma unroll
-    for (int i = 0; i < kMaxPasses; ++i) {
-        const int h = h0 + i * HPP;
-        if (i < p.passes && h < total) {
-            const RowSet &s = h < p.q.heads ? p.q : h < p.q.heads + p.k.heads ? p.k : p.v;
-            const int hh = h < p.q.heads ? h : h < p.q.heads + p.k.heads ? h - p.q.heads : h - p.q.heads - p.k.heads;
-            x[i] = *reinterpret_cast<const uint4 *>(s.in + (long long)row * s.in_stride + hh * D + 8 * l);
-        } else {
-            x[i] = make_uint4(0, 0, 0, 0);
-        }
-    }
     if (p.rot > 0) {
-        if (tid < p.rot / 2) {
-            const double u = (double)pos * p.turns[tid];
+        for (int j = lane; j < p.rot / 2; j += 32) {
+            const double u = (double)pos * s_turns[j];
             float sn, cs;
             sincospif(2.0f * (float)(u - rint(u)), &sn, &cs);
-            s_cos[tid] = cs;
-            s_sin[tid] = sn;
+            s_cos[warp][j] = cs;
+            s_sin[warp][j] = sn;
         }
-        __syncthreads();
+        __syncwarp();
     }
-#pragma unroll
-    for (int i = 0; i < kMaxPasses; ++i) {
-        if (i >= p.passes) break;
-        const int h = h0 + i * HPP;
-        const bool have = h < total;
-        const bool is_q = h < p.q.heads, is_k = !is_q && h < p.q.heads + p.k.heads;
-        const RowSet &s = is_q ? p.q : is_k ? p.k : p.v;
-        const int hh = is_q ? h : is_k ? h - p.q.heads : h - p.q.heads - p.k.heads;
-        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        uint32_t o[4] = {w[0], w[1], w[2], w[3]};
-        // every lane of the warp takes part in the shuffles; a head without work holds zeros
-        float ss = 0.0f;
-        float2 y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            y[j] = h2f(w[j]);
-            ss += y[j].x * y[j].x + y[j].y * y[j].y;
-        }
-#pragma unroll
-        for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-        const int half = p.rot / 2, hc = half / 8;
-        int src = l;  // the lane that holds the other values of this lane's pairs
-        if (!p.adjacent && 8 * l < p.rot) src = (8 * l < half) ? l + hc : l - hc;
-        float2 z[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) z[j] = h2f(__shfl_sync(0xffffffffu, w[j], (lane & ~(LPH - 1)) + src));
-        if (!have) continue;
-        if (is_q || is_k) {
+    const int half = p.rot / 2;
+    const bool turned = 8 * l < p.rot, first = 8 * l < half;
+    const int src = p.adjacent || !turned ? lane : first ? lane + half / 8 : lane - half / 8;  // who holds the pairs' other values
+
+    auto address = [&](const RowSet &s, int h, uint16_t *pages) {
+        return pages ? pages + kv_row(p.cache, page, h, pos & ((1 << p.cache.page_shift) - 1)) + 8 * l
+                     : reinterpret_cast<uint16_t *>(s.out) + (long long)row * s.out_stride + h * D + 8 * l;
+    };
+    // passes [from, to) of a set whose first pass is pass `base` of the row
+    auto turn = [&](const RowSet &s, int base, int from, int to, uint16_t *pages) {
+        if (from >= to) return;
+        float2 A[4], B[4];
+        {
+            uint4 ga = make_uint4(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u), gb = ga;  // ones
             if (s.gamma) {
-                const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
-                const uint4 g = __ldg(reinterpret_cast<const uint4 *>(s.gamma + 8 * l));
-                const uint4 gz = __ldg(reinterpret_cast<const uint4 *>(s.gamma + 8 * src));
-                const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, gzw[4] = {gz.x, gz.y, gz.z, gz.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 a = h2f(gw[j]), b = h2f(gzw[j]);
-                    y[j].x *= inv * a.x;
-                    y[j].y *= inv * a.y;
-                    z[j].x *= inv * b.x;
-                    z[j].y *= inv * b.y;
-                }
+                ga = __ldg(reinterpret_cast<const uint4 *>(s.gamma + 8 * l));
+                gb = __ldg(reinterpret_cast<const uint4 *>(s.gamma + 8 * (src % LPH)));
             }
-            if (8 * l < p.rot) {
+            const uint32_t aw[4] = {ga.x, ga.y, ga.z, ga.w}, bw[4] = {gb.x, gb.y, gb.z, gb.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                A[e] = h2_to_f2(aw[e]);
+                B[e] = h2_to_f2(p.adjacent ? __byte_perm(bw[e], 0, 0x1032) : bw[e]);
+                if (!turned) continue;
                 if (p.adjacent) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float c = s_cos[4 * l + j], sn = s_sin[4 * l + j];
-                        const float2 a = y[j];
-                        y[j].x = a.x * c - a.y * sn;
-                        y[j].y = a.x * sn + a.y * c;
-                    }
+                    const float c = s_cos[warp][4 * l + e], sn = s_sin[warp][4 * l + e];
+                    A[e] = mul2(A[e], make_float2(c, c));
+                    B[e] = mul2(B[e], make_float2(-sn, sn));
                 } else {
-                    const bool first = 8 * l < half;
-                    const int at = first ? 8 * l : 8 * l - half;
-                    const float sg = first ? -1.0f : 1.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 c = *reinterpret_cast<const float2 *>(s_cos + at + 2 * j);
-                        const float2 sn = *reinterpret_cast<const float2 *>(s_sin + at + 2 * j);
-                        y[j].x = y[j].x * c.x + sg * z[j].x * sn.x;
-                        y[j].y = y[j].y * c.y + sg * z[j].y * sn.y;
-                    }
+                    const int j = (first ? 8 * l : 8 * l - half) + 2 * e;
+                    const float2 sn = *reinterpret_cast<const float2 *>(&s_sin[warp][j]);
+                    A[e] = mul2(A[e], *reinterpret_cast<const float2 *>(&s_cos[warp][j]));
+                    B[e] = mul2(B[e], first ? make_float2(-sn.x, -sn.y) : sn);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = f2h(y[j].x, y[j].y);
         }
-        uint16_t *to;
-        if (p.cache.table && !is_q)
-            to = (is_k ? p.cache.k : p.cache.v) +
-                 kv_row(p.cache, page, hh, pos & ((1 << p.cache.page_shift) - 1)) + 8 * l;
-        else
-            to = reinterpret_cast<uint16_t *>(s.out) + (long long)row * s.out_stride + hh * D + 8 * l;
-        *reinterpret_cast<uint4 *>(to) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int i0 = from; i0 < to; i0 += kInFlight) {
+            uint4 x[kInFlight];
+#pragma unroll
+            for (int i = 0; i < kInFlight; ++i) x[i] = ahead[i];
+            const int next = base + min(i0 + kInFlight, to);
+            if (next < n1) load(next, ahead);
+#pragma unroll
+            for (int i = 0; i < kInFlight; ++i) {
+                if (i0 + i >= to) break;
+                const int h = (i0 + i) * HPP + sub;
+                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                float2 y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = h2_to_f2(w[e]);
+                float inv = 1.0f;
+                if (s.gamma) {
+                    float2 s2 = mul2(y[0], y[0]);
+#pragma unroll
+                    for (int e = 1; e < 4; ++e) s2 = fma2(y[e], y[e], s2);
+                    float ss = s2.x + s2.y;
+#pragma unroll
+                    for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+                    inv = rsqrtf(ss * (1.0f / D) + p.eps);
+                }
+                const float2 inv2 = make_float2(inv, inv);
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float2 r = mul2(y[e], A[e]);
+                    if (p.rot > 0) {
+                        const float2 z = h2_to_f2(p.adjacent ? __byte_perm(w[e], 0, 0x1032) : __shfl_sync(0xffffffffu, w[e], src));
+                        // values past the rotation have no partner: an infinity must not meet a factor of 0
+                        const float2 both = fma2(z, B[e], r);
+                        r.x = turned ? both.x : r.x;
+                        r.y = turned ? both.y : r.y;
+                    }
+                    r = mul2(r, inv2);
+                    o[e] = f2_to_h2(r.x, r.y);
+                }
+                if (h < s.heads) *reinterpret_cast<uint4 *>(address(s, h, pages)) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+    };
+    turn(p.q, 0, n0, min(n1, nq), nullptr);
+    turn(p.k, nq, max(n0 - nq, 0), min(n1 - nq, nk), p.cache.table ? p.cache.k : nullptr);
+    for (int n = max(n0, nq + nk); n < n1; n += kInFlight) {  // values as they are
+        uint4 x[kInFlight];
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) x[i] = ahead[i];
+        if (n + kInFlight < n1) load(n + kInFlight, ahead);
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) {
+            const int h = (n - nq - nk + i) * HPP + sub;
+            if (n + i < n1 && h < p.v.heads) *reinterpret_cast<uint4 *>(address(p.v, h, p.cache.v)) = x[i];
+        }
     }
 }
 
@@ -184,14 +218,15 @@ RowSet row_set(const kq_heads *h) {
 
 template <int D>
 cudaError_t launch(RopeParams &p, int M, int num_sms, cudaStream_t stream, bool pdl) {
-    constexpr int HPP = kThreads / (D / 8);
-    const int total = p.q.heads + p.k.heads + p.v.heads;
-    const int need = (total + HPP - 1) / HPP;
-    p.passes = 1;
-    while (p.passes < kMaxPasses && p.passes < need && (long long)M * ((need + p.passes - 1) / p.passes) > 4ll * num_sms)
-        ++p.passes;
+    constexpr int HPP = 32 / (D / 8);
+    const int passes = (p.q.heads + HPP - 1) / HPP + (p.k.heads + HPP - 1) / HPP + (p.v.heads + HPP - 1) / HPP;
+    // a warp per row when the rows alone fill the GPU, else chunks of a row's passes
+    p.M = M;
+    p.chunks = kCtasPerSm * (kThreads / 32) * num_sms / M;
+    if (p.chunks > passes) p.chunks = passes;
+    if (p.chunks < 1) p.chunks = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(M, (need + p.passes - 1) / p.passes);
+    cfg.gridDim = dim3((unsigned)(((long long)M * p.chunks + kThreads / 32 - 1) / (kThreads / 32)));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
