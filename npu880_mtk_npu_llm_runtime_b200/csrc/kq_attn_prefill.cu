@@ -33,6 +33,7 @@ namespace {
 
 constexpr float kBias = 4.0f;  // weights reach 2^(kBias + kLag) < 65504: fp16's relative precision reaches further down
 constexpr float kLag = 8.0f;
+constexpr int kPolyEvery = 4;  // every so many pairs of exponentials one by polynomial
 constexpr int kThreads = 384;
 constexpr int kSortTiles = 512;
 // A join costs about as much as this many blocks: whole items unless the longest is that much
@@ -65,22 +66,22 @@ struct PrefillParams {
 
 // ------------------------------------------------------------------ PTX
 
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
-    // 128-byte swizzle, 8-row groups 1,024 bytes apart (descriptor version 1)
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Shared-memory operand, 128-byte swizzle, 8-row groups 1,024 bytes apart (descriptor version 1): the
+// low word (address and leading stride in 16-byte units), to which offsets in 16-byte units add, and
+// the constant high word.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return ((saddr >> 4) & 0x3FFFu) | (lbo >> 4) << 16; }
+constexpr uint32_t kDescHi = (1024 >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0));
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(0), "r"(kDescHi));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0));
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %6};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(0), "r"(kDescHi));
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -136,6 +137,31 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// 2^x without the special-function unit, which alone takes as long over a block's exponentials as the
+// tensor core over its products: x = n + r with n the nearest integer (Cody and Waite's reduction, n
+// from the low bits of x + 1.5 2^23), 2^r on [-1/2, 1/2] by the polynomial of degree 4 of least
+// relative error (2.6e-6, fitted; the result is rounded to 11 bits), n added to the exponent.  x is at
+// most a few; below -126 it gives 2^-126 (0 in fp16), and a NaN leaves a value past fp16's range.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.0f));
+    const float2 magic = make_float2(12582912.0f, 12582912.0f), minus = make_float2(-1.0f, -1.0f);
+    const float2 t = __fadd2_rn(x, magic);
+    const float2 r = __ffma2_rn(__fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f)), minus, x);
+    float2 y = make_float2(0.00957010128f, 0.00957010128f);
+    y = __ffma2_rn(y, r, make_float2(0.0559178603f, 0.0559178603f));
+    y = __ffma2_rn(y, r, make_float2(0.240247448f, 0.240247448f));
+    y = __ffma2_rn(y, r, make_float2(0.693121815f, 0.693121815f));
+    y = __ffma2_rn(y, r, make_float2(0.999999261f, 0.999999261f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
 }
 
 // ------------------------------------------------------------------ work
@@ -250,7 +276,7 @@ struct Walk {
 constexpr int kSegs = 4;  // segments on their way from the loader to the other roles
 
 struct Shared {
-    unsigned long long full[8], empty[8], q_full, q_empty, s_full[2], p_ready[2], o_full[2], pv_done, tail, join, never;
+    unsigned long long full[8], empty[8], q_full, q_empty, s_full[2], p_ready[2][2], o_full[2], pv_done, tail, join, never;
     unsigned long long seg_full[kSegs], seg_empty[kSegs];
     Segment seg[kSegs];
     uint32_t tmem;
@@ -262,6 +288,18 @@ struct Shared {
 
 static_assert(sizeof(Shared) <= 1024, "a CTA has 227 KB of shared memory");
 constexpr size_t kSmem = 226 * 1024;  // dynamic
+
+// Place in the ring: advanced block by block (a division by the number of stages would cost more than
+// the rest of an MMA's issue).
+struct Cursor {
+    uint32_t stage = 0, phase = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++stage == (uint32_t)stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+};
 
 // Bounded wait on a phase: false when it did not complete in time or another role gave up.
 struct Waiter {
@@ -387,12 +425,12 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
     __syncthreads();
 }
 
-// Loads of one CTA, by a warp: segments to the other roles, Q, K and V to shared memory.  n counts
-// the ring blocks issued.
+// Loads of one CTA, by a warp: segments to the other roles, Q, K and V to shared memory.  `at`: the
+// ring's next block.
 template <int D>
 __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, const Waiter &wait, const CUtensorMap &mq,
                                           const CUtensorMap &mk, const CUtensorMap &mv, unsigned char *s_q,
-                                          unsigned char *s_ring, int lane, uint32_t &n) {
+                                          unsigned char *s_ring, int lane, Cursor &at) {
     using C = Cfg<D>;
     constexpr int NT = C::NT, BN = C::BN, CH = C::CH;
     const AttnLaunch &a = p.a;
@@ -415,11 +453,21 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
         if (!have) return;
         const int subs = s.n_tok > p.tpt ? NT : 1;
         const int32_t *table = a.cache.table + (long long)s.seq * a.cache.table_stride;
+        // The page of this lane's box of block i; n_pages, out of range, where no token sees the box
+        // (the copy fills it with zeros) or the table names no page.
+        auto page_of = [&](int i) {
+            const int j = kv_block(s.blocks, i) * BN + sub * p.box_rows;
+            if (lane >= boxes || !tile_sees(s, j, p.box_rows)) return a.cache.n_pages;
+            const int q = __ldg(table + (j >> a.cache.page_shift));
+            if (kv_page_ok(a.cache, q)) return q;
+            rec.bad = 1;
+            return a.cache.n_pages;
+        };
         // block i of the segment's K (kv = 0) or V (1) into the ring
-        auto load = [&](int i, int kv) {
-            const int st = n % p.stages;
-            if (!wait(sh.empty[st], ((n / p.stages) & 1) ^ 1)) return false;
-            ++n;
+        auto load = [&](int i, int kv, int page) {
+            const uint32_t st = at.stage;
+            if (!wait(sh.empty[st], at.phase ^ 1)) return false;
+            at.next(p.stages);
             const int j0 = kv_block(s.blocks, i) * BN;
             unsigned char *to = s_ring + (size_t)st * C::STAGE;
             // V rows past the sequence's end may hold anything, and 0 * NaN is NaN: zeroed once they landed
@@ -429,12 +477,6 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
             __syncwarp();
             if (lane < boxes) {
                 const int j = j0 + sub * p.box_rows;
-                int page = a.cache.n_pages;  // out of range: the box is filled with zeros
-                if (tile_sees(s, j, p.box_rows)) {
-                    const int q = __ldg(table + (j >> a.cache.page_shift));
-                    if (kv_page_ok(a.cache, q)) page = q;
-                    else rec.bad = 1;
-                }
                 tma4(smem_u32(to) + piece * (BN * 128) + sub * p.box_rows * 128, kv ? &mv : &mk, 64 * piece,
                      j & ((1 << a.cache.page_shift) - 1), s.head, page, bar);
             }
@@ -452,7 +494,8 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
             __syncwarp();
             return true;
         };
-        if (!load(s.b0, 0)) return;
+        int page = page_of(s.b0);  // of the block whose K is loaded next
+        if (!load(s.b0, 0, page)) return;
         if (!wait(sh.q_empty, (k & 1) ^ 1)) return;
         if (lane == 0) mbar_arrive_expect_tx(smem_u32(&sh.q_full), (uint32_t)(subs * p.tpt * p.group * D * 2));
         __syncwarp();
@@ -460,67 +503,57 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
             tma3(smem_u32(s_q) + sub * C::Q_TILE + piece * (128 * 128), &mq, 64 * piece, s.head * p.group,
                  s.row0 + sub * p.tpt, smem_u32(&sh.q_full));
         __syncwarp();
-        // the rest in the order in which the MMAs read it
+        // the rest in the order in which the MMAs read it, pages looked up a block ahead
         if (NT == 2) {
             for (int i = s.b0; i < s.b1; ++i) {
-                if (i > s.b0 && !load(i, 0)) return;
-                if (!load(i, 1)) return;
+                const int next = i + 1 < s.b1 ? page_of(i + 1) : 0;
+                if (!load(i, 1, page)) return;
+                page = next;
+                if (i + 1 < s.b1 && !load(i + 1, 0, page)) return;
             }
         } else {
-            if (s.b0 + 1 < s.b1 && !load(s.b0 + 1, 0)) return;
+            int page1 = s.b0 + 1 < s.b1 ? page_of(s.b0 + 1) : 0;
+            if (s.b0 + 1 < s.b1 && !load(s.b0 + 1, 0, page1)) return;
             for (int i = s.b0; i < s.b1; ++i) {
-                if (!load(i, 1)) return;
-                if (i + 2 < s.b1 && !load(i + 2, 0)) return;
+                const int next = i + 2 < s.b1 ? page_of(i + 2) : 0;
+                if (!load(i, 1, page)) return;
+                page = page1;
+                page1 = next;
+                if (i + 2 < s.b1 && !load(i + 2, 0, page1)) return;
             }
         }
     }
 }
 
-// The MMAs of one CTA, by a converged warp.
+// The MMAs of one CTA, by a converged warp, one elected lane issuing.
 template <int D>
 __device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, const Waiter &wait, uint32_t q0, uint32_t ring,
                                          uint32_t tmem) {
     using C = Cfg<D>;
     constexpr int NT = C::NT, BN = C::BN;
-    uint32_t n = 0, np[2] = {0, 0};  // ring blocks read, P's read of each slot
+    constexpr uint32_t kStep = C::STAGE >> 4;
+    Cursor at;                // the ring's next block to read
+    uint32_t np[2] = {0, 0};  // P's begun of each slot
     if (p.inject && !wait(sh.never, 0)) return;
+    const uint32_t q_lo = desc_lo(q0, 16), k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, BN * 128);
     // S slot = Q tile t times the K block in ring stage st
     auto mma_s = [&](int t, int slot, uint32_t st) {
-        if (elect_one()) {
-            const uint32_t kb = ring + st * C::STAGE, qb = q0 + t * C::Q_TILE;
+        const uint32_t kb = k_lo + st * kStep, qb = q_lo + t * (C::Q_TILE >> 4);
 #pragma unroll
-            for (int e = 0; e < D / 16; ++e)
-                mma_ss(tmem + slot * C::S_COL, desc_sw128(qb + (e / 4) * (128 * 128) + (e % 4) * 32, 16),
-                       desc_sw128(kb + (e / 4) * (BN * 128) + (e % 4) * 32, 16), C::IDESC_S, e > 0);
-            commit(smem_u32(&sh.s_full[slot]));
-        }
-        __syncwarp();
+        for (int e = 0; e < D / 16; ++e)
+            mma_ss(tmem + slot * C::S_COL, qb + (e / 4) * (128 * 128 / 16) + (e % 4) * 2, kb + (e / 4) * (BN * 128 / 16) + (e % 4) * 2,
+                   C::IDESC_S, e > 0);
+        commit(smem_u32(&sh.s_full[slot]));
     };
-    // O tile t (+)= P of the slot times the V block in ring stage st
-    auto mma_o = [&](int t, int slot, uint32_t st, bool first) {
-        if (!wait(sh.p_ready[slot], np[slot] & 1)) return false;
-        ++np[slot];
-        fence_after();
-        if (elect_one()) {
-            const uint32_t vb = ring + st * C::STAGE;
+    // O tile t (+)= half h of the slot's P times its keys' rows of the V block in ring stage st
+    auto mma_o = [&](int t, int slot, uint32_t st, bool first, int h) {
+        const uint32_t vb = v_lo + st * kStep + h * (BN / 32) * 128, pb = tmem + slot * C::S_COL + h * (BN / 32) * 8;
 #pragma unroll
-            for (int e = 0; e < BN / 16; ++e)
-                mma_ts(tmem + C::O_COL + t * D, tmem + slot * C::S_COL + e * 8, desc_sw128(vb + e * 2048, BN * 128), C::IDESC_O,
-                       !(first && e == 0));
-        }
-        __syncwarp();
-        return true;
+        for (int e = 0; e < BN / 32; ++e)
+            mma_ts(tmem + C::O_COL + t * D, pb + e * 8, vb + e * 128, C::IDESC_O, !(first && h == 0 && e == 0));
     };
-    auto arrive = [&](unsigned long long &bar) {
-        if (elect_one()) commit(smem_u32(&bar));
-        __syncwarp();
-    };
-    auto stage = [&](uint32_t i) { return i % p.stages; };
-    auto wait_full = [&](uint32_t i) {
-        if (!wait(sh.full[i % p.stages], (i / p.stages) & 1)) return false;
-        fence_after();
-        return true;
-    };
+    // a half of the slot's next P (each half has a barrier of its own: both may come before either is waited for)
+    auto wait_p = [&](int slot, int h) { return wait(sh.p_ready[slot][h], (h == 0 ? np[slot]++ : np[slot] - 1) & 1); };
     for (uint32_t k = 0;; ++k) {
         if (!wait(sh.seg_full[k % kSegs], (k / kSegs) & 1)) return;
         const Segment &s = sh.seg[k % kSegs];
@@ -529,52 +562,76 @@ __device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, con
         __syncwarp();
         if (elect_one()) mbar_arrive(smem_u32(&sh.seg_empty[k % kSegs]));
         if (!wait(sh.q_full, k & 1)) return;
-        fence_after();
         if (NT == 2) {
-            // ring: K0 V0 K1 V1 ...
-            for (int j = 0; j < nb; ++j) {
-                const uint32_t kk = n + 2 * j;
-                if (!wait_full(kk)) return;
-                if (j > 0 && !wait_full(kk - 1)) return;
-                for (int t = 0; t < subs; ++t) {
-                    if (j > 0 && !mma_o(t, t, stage(kk - 1), j == 1)) return;
-                    mma_s(t, t, stage(kk));
+            // ring: K0 V0 K1 V1 ...; V(j-1) and K(j) are read together
+            uint32_t v = 0;
+            for (int j = 0; j <= nb; ++j) {
+                if (j > 0) {
+                    v = at.stage;
+                    if (!wait(sh.full[v], at.phase)) return;
+                    at.next(p.stages);
                 }
-                if (j > 0) arrive(sh.empty[stage(kk - 1)]);
-                arrive(sh.empty[stage(kk)]);
-                if (j == nb - 1) arrive(sh.q_empty);
+                const uint32_t kk = at.stage;
+                if (j < nb) {
+                    if (!wait(sh.full[kk], at.phase)) return;
+                    at.next(p.stages);
+                }
+                for (int t = 0; t < subs; ++t) {
+                    if (j > 0) {
+                        if (!wait_p(t, 0)) return;
+                        fence_after();
+                        if (elect_one()) mma_o(t, t, v, j == 1, 0);
+                        __syncwarp();
+                        if (!wait_p(t, 1)) return;
+                    }
+                    fence_after();
+                    if (elect_one()) {
+                        if (j > 0) mma_o(t, t, v, false, 1);
+                        if (j < nb) mma_s(t, t, kk);
+                        else commit(smem_u32(&sh.o_full[t]));
+                        if (t == subs - 1) {
+                            if (j > 0) commit(smem_u32(&sh.empty[v]));
+                            if (j < nb) commit(smem_u32(&sh.empty[kk]));
+                            if (j == nb - 1) commit(smem_u32(&sh.q_empty));
+                        }
+                    }
+                    __syncwarp();
+                }
             }
-            const uint32_t v = n + 2 * nb - 1;
-            if (!wait_full(v)) return;
-            for (int t = 0; t < subs; ++t) {
-                if (!mma_o(t, t, stage(v), nb == 1)) return;
-                arrive(sh.o_full[t]);
-            }
-            arrive(sh.empty[stage(v)]);
         } else {
             // ring: K0 K1 V0 K2 V1 ... K(i) V(i-2) ... V(nb-1)
-            auto k_at = [&](int i) { return n + (i < 2 ? i : 2 * i - 1); };
-            auto v_at = [&](int i) { return n + (i + 2 < nb ? 2 * i + 2 : nb + i); };
-            for (int i = 0; i < 2 && i < nb; ++i) {
-                if (!wait_full(k_at(i))) return;
-                mma_s(0, i, stage(k_at(i)));
-                arrive(sh.empty[stage(k_at(i))]);
-                if (i == nb - 1) arrive(sh.q_empty);
-            }
-            for (int i = 0; i < nb; ++i) {
-                if (!wait_full(v_at(i))) return;
-                if (!mma_o(0, i & 1, stage(v_at(i)), i == 0)) return;
-                arrive(i == nb - 1 ? sh.o_full[0] : sh.pv_done);
-                arrive(sh.empty[stage(v_at(i))]);
+            for (int i = -2; i < nb; ++i) {
+                if (i >= 0) {
+                    const uint32_t v = at.stage;
+                    if (!wait(sh.full[v], at.phase)) return;
+                    at.next(p.stages);
+                    if (!wait_p(i & 1, 0)) return;
+                    fence_after();
+                    if (elect_one()) mma_o(0, i & 1, v, i == 0, 0);
+                    __syncwarp();
+                    if (!wait_p(i & 1, 1)) return;
+                    fence_after();
+                    if (elect_one()) {
+                        mma_o(0, i & 1, v, false, 1);
+                        commit(smem_u32(i == nb - 1 ? &sh.o_full[0] : &sh.pv_done));
+                        commit(smem_u32(&sh.empty[v]));
+                    }
+                    __syncwarp();
+                }
                 if (i + 2 < nb) {
-                    if (!wait_full(k_at(i + 2))) return;
-                    mma_s(0, i & 1, stage(k_at(i + 2)));
-                    arrive(sh.empty[stage(k_at(i + 2))]);
-                    if (i + 2 == nb - 1) arrive(sh.q_empty);
+                    const uint32_t kk = at.stage;
+                    if (!wait(sh.full[kk], at.phase)) return;
+                    at.next(p.stages);
+                    fence_after();
+                    if (elect_one()) {
+                        mma_s(0, i & 1, kk);
+                        commit(smem_u32(&sh.empty[kk]));
+                        if (i + 2 == nb - 1) commit(smem_u32(&sh.q_empty));
+                    }
+                    __syncwarp();
                 }
             }
         }
-        n += 2 * nb;
     }
 }
 
@@ -668,12 +725,13 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                         for (int e = 0; e < 32; ++e) x[32 * c + e] = (bits >> e & 1) ? x[32 * c + e] : -INFINITY;
                     }
                 }
-                float mx[4] = {x[0], x[1], x[2], x[3]};
+                float mx[2] = {x[0], x[1]};
 #pragma unroll
-                for (int e = 4; e < BN; e += 4)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], x[e + u]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                for (int e = 2; e < BN; e += 4) {
+                    mx[0] = max3(mx[0], x[e], x[e + 1]);
+                    if (e + 3 < BN) mx[1] = max3(mx[1], x[e + 2], x[e + 3]);
+                }
+                const float top = fmaxf(mx[0], mx[1]) * p.scale_log2;
                 const bool raise = top > m + kLag;  // the first score above -inf raises from -inf
                 if (__any_sync(0xffffffffu, raise)) {
                     const float to = raise ? top : m;
@@ -698,25 +756,33 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                     }
                 }
                 const float off = (m == -INFINITY ? 0.0f : -m) + kBias;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), off2 = make_float2(off, off);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c) {
-                    uint32_t h[16];
+                for (int half = 0; half < 2; ++half) {  // P goes to the MMA in halves: the first runs while the second is made
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float w0 = exp2_fast(fmaf(x[32 * c + 2 * e], p.scale_log2, off));
-                        const float w1 = exp2_fast(fmaf(x[32 * c + 2 * e + 1], p.scale_log2, off));
-                        sum[2 * (e & 1)] += w0;
-                        sum[2 * (e & 1) + 1] += w1;
-                        h[e] = f2_to_h2(w0, w1);
+                    for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
+                        uint32_t h[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float2 w = __ffma2_rn(make_float2(x[32 * c + 2 * e], x[32 * c + 2 * e + 1]), scale2, off2);
+                            if (e % kPolyEvery == kPolyEvery - 1) {
+                                w = exp2_poly(w);
+                            } else {
+                                w.x = exp2_fast(w.x);
+                                w.y = exp2_fast(w.y);
+                            }
+                            sum[e & 1] = __fadd2_rn(sum[e & 1], w);
+                            h[e] = f2_to_h2(w.x, w.y);
+                        }
+                        tmem_st16(s_base + 16 * c, h);
                     }
-                    tmem_st16(s_base + 16 * c, h);
+                    wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready[slot][half]));
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready[slot]));
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             if (!wait(sh.o_full[t], no & 1)) return;
             ++no;
@@ -725,7 +791,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
             if (*reinterpret_cast<const volatile int *>(&s.bad)) l = NAN;  // mended below
             if (whole) {
                 const float inv = 1.0f / l;
-                bool odd = false;
+                bool odd = m == -INFINITY;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     float o[32];
@@ -777,7 +843,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                     L += mc == -INFINITY ? (lc != lc ? lc : 0.0f) : exp2_fast(mc - M) * lc;
                 }
                 const float inv = 1.0f / L;
-                bool odd = !(fabsf(inv) <= 3e38f);
+                bool odd = M == -INFINITY || !(fabsf(inv) <= 3e38f);
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
                     float o[32];
@@ -825,7 +891,8 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
         mbar_init(smem_u32(&sh.q_empty), 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(smem_u32(&sh.s_full[t]), 1);
-            mbar_init(smem_u32(&sh.p_ready[t]), 4);
+            mbar_init(smem_u32(&sh.p_ready[t][0]), 4);
+            mbar_init(smem_u32(&sh.p_ready[t][1]), 4);
             mbar_init(smem_u32(&sh.o_full[t]), 1);
         }
         mbar_init(smem_u32(&sh.pv_done), 1);
@@ -855,14 +922,14 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 9) {
-            uint32_t n = 0;
-            load_role<D>(p, sh, wait, mq, mk, mv, s_q, s_ring, lane, n);
+            Cursor at;
+            load_role<D>(p, sh, wait, mq, mk, mv, s_q, s_ring, lane, at);
             __syncwarp();
             if (*reinterpret_cast<volatile int *>(&sh.abort)) {
                 // let the copies in flight land before the CTA's memory goes (bounded)
                 const uint64_t t0 = global_timer_ns();
-                for (uint32_t i = n > (uint32_t)p.stages ? n - p.stages : 0; i < n; ++i)
-                    while (!mbar_test_wait(smem_u32(&sh.full[i % p.stages]), (i / p.stages) & 1) &&
+                for (uint32_t i = 0; i < (uint32_t)p.stages; ++i)  // (a stage not yet used this time round completed before)
+                    while (!mbar_test_wait(smem_u32(&sh.full[i]), at.phase ^ (i >= at.stage)) &&
                            global_timer_ns() - t0 < 2000000ull) {
                     }
                 while (global_timer_ns() - t0 < 50000ull) {
