@@ -12,11 +12,11 @@
 // (128 x 128 x 2 x 128 operations and 128 x 128 exponentials take about the same time).
 //
 // Warps 0-3 and 4-7: softmax of tile 0 and 1, one row a thread: S from TMEM to registers, maximum,
-// exponentials, P as fp16 back into S's columns (the second product's A operand), and the epilogue.
-// Warp 8 issues the MMAs: P(j-1) V(j-1) then Q K(j) per tile, so S's columns are free when they are
-// written.  Warp 9 loads: Q as one box of [tokens][G heads][64 values] per 64 values, K and V page
-// by page (TMA, 128-byte swizzle) into a ring of blocks of BN keys; V stays as it lies in the cache
-// and is the MMA's MN-major B operand.
+// exponentials, P as fp16 back into S's columns (the second product's A operand) in two halves, and the
+// epilogue.  Warp 8 issues the MMAs: P(j-1) V(j-1) then Q K(j) per tile, so S's columns are free when
+// they are written.  Warps 9 and 10 load K and V page by page (TMA, 128-byte swizzle) into rings of
+// blocks of BN keys, warp 9 also Q, as one box of [tokens][G heads][64 values] per 64 values; V stays as
+// it lies in the cache and is the MMA's MN-major B operand.
 //
 // Work: an item is a row tile of one key head, a unit one of its key blocks.  Items go whole to
 // the CTAs, longest first in snake order, when that balances; else (few items, long caches) every
@@ -34,7 +34,8 @@ namespace {
 constexpr float kBias = 4.0f;  // weights reach 2^(kBias + kLag) < 65504: fp16's relative precision reaches further down
 constexpr float kLag = 8.0f;
 constexpr int kPolyEvery = 4;  // every so many pairs of exponentials one by polynomial
-constexpr int kThreads = 384;
+constexpr int kThreads = 384;  // 8 softmax warps, MMA, K and Q loads, V loads, one idle
+constexpr int kWarpMma = 8, kWarpK = 9, kWarpV = 10;
 constexpr int kSortTiles = 512;
 // A join costs about as much as this many blocks: whole items unless the longest is that much
 // longer than an even share.
@@ -47,7 +48,8 @@ struct Cfg {
     static constexpr int CH = D / 64;              // 128-byte wide pieces of a row
     static constexpr uint32_t Q_TILE = 128 * D * 2;
     static constexpr uint32_t STAGE = BN * D * 2;
-    static constexpr int MAX_STAGES = 8;
+    static constexpr int MAX_STAGES = 4;  // of K, and of V
+    static constexpr int SOFTMAX_WARPS = 4 * NT;
     static constexpr uint32_t S_COL = BN;          // TMEM columns: S slots, then O
     static constexpr uint32_t O_COL = 256;
     static constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((128u >> 4) << 24);
@@ -59,7 +61,7 @@ struct PrefillParams {
     float scale_log2;
     int group, tpt;   // query heads of a key head; tokens of an MMA tile
     int box_rows;     // keys of one K/V box: the smaller of a page and a block
-    int stages;
+    int k_stages, v_stages;
     unsigned long long timeout_ns;
     int inject;
 };
@@ -276,18 +278,23 @@ struct Walk {
 constexpr int kSegs = 4;  // segments on their way from the loader to the other roles
 
 struct Shared {
-    unsigned long long full[8], empty[8], q_full, q_empty, s_full[2], p_ready[2][2], o_full[2], pv_done, tail, join, never;
-    unsigned long long seg_full[kSegs], seg_empty[kSegs];
+    unsigned long long k_full[4], k_empty[4], v_full[4], v_empty[4], q_full, q_empty, s_full[2], p_ready[2][2], o_full[2];
+    unsigned long long pv_done, tail, join, never, seg_full[kSegs], seg_empty[kSegs];
     Segment seg[kSegs];
     uint32_t tmem;
     int abort, last;
-    long long red[kThreads / 32];
-    int red_max[kThreads / 32];
     Plan plan;
 };
 
 static_assert(sizeof(Shared) <= 1024, "a CTA has 227 KB of shared memory");
 constexpr size_t kSmem = 226 * 1024;  // dynamic
+
+// What the plan is made with, in the ring's memory.
+struct PlanScratch {
+    long long red[kThreads / 32];
+    int red_max[kThreads / 32];
+    int nbs[1];  // blocks of every row tile
+};
 
 // Place in the ring: advanced block by block (a division by the number of stages would cost more than
 // the rest of an MMA's issue).
@@ -325,12 +332,13 @@ struct Waiter {
     }
 };
 
-// The CTA's plan, by all its threads.  scratch: at least 4 bytes per row tile.
+// The CTA's plan, by all its threads.
 template <int D>
-__device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, int *seq_tiles, unsigned short *order, int *nbs) {
+__device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, int *seq_tiles, unsigned short *order, PlanScratch &scratch) {
     using C = Cfg<D>;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = p.a.cache.n_seqs;
     const int per = C::NT * p.tpt;
+    int *nbs = scratch.nbs;
     {
         const int chunk = (S + kThreads - 1) / kThreads, s0 = tid * chunk;
         int sum = 0;
@@ -348,10 +356,10 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
             const int o = __shfl_up_sync(0xffffffffu, run, d);
             if (lane >= d) run += o;
         }
-        if (lane == 31) sh.red[warp] = run;
+        if (lane == 31) scratch.red[warp] = run;
         __syncthreads();
         int base = run - sum;
-        for (int w = 0; w < warp; ++w) base += (int)sh.red[w];
+        for (int w = 0; w < warp; ++w) base += (int)scratch.red[w];
         for (int s = s0; s < s0 + chunk && s < S; ++s) seq_tiles[s] += base;
         if (tid == kThreads - 1) seq_tiles[S] = base + sum;
         __syncthreads();
@@ -375,14 +383,14 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         if (lane >= d) run += o;
         most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
     }
-    if (lane == 31) sh.red[warp] = run;
-    if (lane == 0) sh.red_max[warp] = most;
+    if (lane == 31) scratch.red[warp] = run;
+    if (lane == 0) scratch.red_max[warp] = most;
     __syncthreads();
     long long before = run - sum, total = 0;
     for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) before += sh.red[w];
-        total += sh.red[w];
-        most = max(most, sh.red_max[w]);
+        if (w < warp) before += scratch.red[w];
+        total += scratch.red[w];
+        most = max(most, scratch.red_max[w]);
     }
     total *= heads;
     const int whole = most <= total / (int)gridDim.x + kJoinBlocks;
@@ -425,63 +433,69 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
     __syncthreads();
 }
 
-// Loads of one CTA, by a warp: segments to the other roles, Q, K and V to shared memory.  `at`: the
-// ring's next block.
-template <int D>
+// Loads of one CTA by a warp each: the K warp hands the segments to the other roles and loads Q and K,
+// the V warp loads V (two warps, because a block of 16-position pages is 16 copies or more, which one warp
+// issues no faster than the MMAs read it).  `at`: the ring's next block.
+template <int D, bool V>
 __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, const Waiter &wait, const CUtensorMap &mq,
-                                          const CUtensorMap &mk, const CUtensorMap &mv, unsigned char *s_q,
-                                          unsigned char *s_ring, int lane, Cursor &at) {
+                                          const CUtensorMap &m, unsigned char *s_q, unsigned char *s_ring, int lane, Cursor &at) {
     using C = Cfg<D>;
     constexpr int NT = C::NT, BN = C::BN, CH = C::CH;
     const AttnLaunch &a = p.a;
-    const int boxes = (BN / p.box_rows) * CH;
+    const int boxes = (BN / p.box_rows) * CH, stages = V ? p.v_stages : p.k_stages;
     const int sub = lane / CH, piece = lane % CH;  // this lane's box of a block
     uint32_t tails = 0;
     Walk<D> walk(p, sh.plan);
     for (uint32_t k = 0;; ++k) {
         Segment s;
-        const bool have = walk.next(s);
         Segment &rec = sh.seg[k % kSegs];
-        if (!wait(sh.seg_empty[k % kSegs], ((k / kSegs) & 1) ^ 1)) return;
-        if (lane == 0) {
+        if (V) {
+            if (!wait(sh.seg_full[k % kSegs], (k / kSegs) & 1)) return;
+            s = rec;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.seg_empty[k % kSegs]));
+        } else {
+            const bool have = walk.next(s);
+            if (!wait(sh.seg_empty[k % kSegs], ((k / kSegs) & 1) ^ 1)) return;
             s.bad = 0;
             s.live = have;
-            rec = s;
-            mbar_arrive(smem_u32(&sh.seg_full[k % kSegs]));
+            if (lane == 0) {
+                rec = s;
+                mbar_arrive(smem_u32(&sh.seg_full[k % kSegs]));
+            }
+            __syncwarp();
         }
-        __syncwarp();
-        if (!have) return;
-        const int subs = s.n_tok > p.tpt ? NT : 1;
+        if (!s.live) return;
         const int32_t *table = a.cache.table + (long long)s.seq * a.cache.table_stride;
         // The page of this lane's box of block i; n_pages, out of range, where no token sees the box
         // (the copy fills it with zeros) or the table names no page.
         auto page_of = [&](int i) {
             const int j = kv_block(s.blocks, i) * BN + sub * p.box_rows;
-            if (lane >= boxes || !tile_sees(s, j, p.box_rows)) return a.cache.n_pages;
+            if (lane >= boxes || i >= s.b1 || !tile_sees(s, j, p.box_rows)) return a.cache.n_pages;
             const int q = __ldg(table + (j >> a.cache.page_shift));
             if (kv_page_ok(a.cache, q)) return q;
-            rec.bad = 1;
+            if (!V) *reinterpret_cast<volatile int *>(&rec.bad) = 1;
             return a.cache.n_pages;
         };
-        // block i of the segment's K (kv = 0) or V (1) into the ring
-        auto load = [&](int i, int kv, int page) {
+        int page = page_of(s.b0);
+        for (int i = s.b0; i < s.b1; ++i) {
+            const int next = page_of(i + 1);  // a block ahead
             const uint32_t st = at.stage;
-            if (!wait(sh.empty[st], at.phase ^ 1)) return false;
-            at.next(p.stages);
+            if (!wait((V ? sh.v_empty : sh.k_empty)[st], at.phase ^ 1)) return;
+            at.next(stages);
             const int j0 = kv_block(s.blocks, i) * BN;
             unsigned char *to = s_ring + (size_t)st * C::STAGE;
+            unsigned long long &full = (V ? sh.v_full : sh.k_full)[st];
             // V rows past the sequence's end may hold anything, and 0 * NaN is NaN: zeroed once they landed
-            const bool tail = kv == 1 && j0 + BN > s.len;
-            const uint32_t bar = smem_u32(tail ? &sh.tail : &sh.full[st]);
+            const bool tail = V && j0 + BN > s.len;
+            const uint32_t bar = smem_u32(tail ? &sh.tail : &full);
             if (lane == 0) mbar_arrive_expect_tx(bar, C::STAGE);
             __syncwarp();
-            if (lane < boxes) {
-                const int j = j0 + sub * p.box_rows;
-                tma4(smem_u32(to) + piece * (BN * 128) + sub * p.box_rows * 128, kv ? &mv : &mk, 64 * piece,
-                     j & ((1 << a.cache.page_shift) - 1), s.head, page, bar);
-            }
+            if (lane < boxes)
+                tma4(smem_u32(to) + piece * (BN * 128) + sub * p.box_rows * 128, &m, 64 * piece,
+                     (j0 + sub * p.box_rows) & ((1 << a.cache.page_shift) - 1), s.head, page, bar);
             if (tail) {
-                if (!wait(sh.tail, tails & 1)) return false;
+                if (!wait(sh.tail, tails & 1)) return;
                 ++tails;
                 for (int e = lane + max(0, s.len - j0) * 8; e < BN * 8; e += 32)
 #pragma unroll
@@ -489,53 +503,45 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
                         *reinterpret_cast<uint4 *>(to + c * (BN * 128) + e * 16) = make_uint4(0, 0, 0, 0);
                 fence_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.full[st]));
+                if (lane == 0) mbar_arrive(smem_u32(&full));
             }
             __syncwarp();
-            return true;
-        };
-        int page = page_of(s.b0);  // of the block whose K is loaded next
-        if (!load(s.b0, 0, page)) return;
-        if (!wait(sh.q_empty, (k & 1) ^ 1)) return;
-        if (lane == 0) mbar_arrive_expect_tx(smem_u32(&sh.q_full), (uint32_t)(subs * p.tpt * p.group * D * 2));
-        __syncwarp();
-        if (lane < subs * CH)
-            tma3(smem_u32(s_q) + sub * C::Q_TILE + piece * (128 * 128), &mq, 64 * piece, s.head * p.group,
-                 s.row0 + sub * p.tpt, smem_u32(&sh.q_full));
-        __syncwarp();
-        // the rest in the order in which the MMAs read it, pages looked up a block ahead
-        if (NT == 2) {
-            for (int i = s.b0; i < s.b1; ++i) {
-                const int next = i + 1 < s.b1 ? page_of(i + 1) : 0;
-                if (!load(i, 1, page)) return;
-                page = next;
-                if (i + 1 < s.b1 && !load(i + 1, 0, page)) return;
-            }
-        } else {
-            int page1 = s.b0 + 1 < s.b1 ? page_of(s.b0 + 1) : 0;
-            if (s.b0 + 1 < s.b1 && !load(s.b0 + 1, 0, page1)) return;
-            for (int i = s.b0; i < s.b1; ++i) {
-                const int next = i + 2 < s.b1 ? page_of(i + 2) : 0;
-                if (!load(i, 1, page)) return;
-                page = page1;
-                page1 = next;
-                if (i + 2 < s.b1 && !load(i + 2, 0, page1)) return;
+            page = next;
+            if (!V && i == s.b0) {
+                const int subs = s.n_tok > p.tpt ? NT : 1;
+                if (!wait(sh.q_empty, (k & 1) ^ 1)) return;
+                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&sh.q_full), (uint32_t)(subs * p.tpt * p.group * D * 2));
+                __syncwarp();
+                if (lane < subs * CH)
+                    tma3(smem_u32(s_q) + sub * C::Q_TILE + piece * (128 * 128), &mq, 64 * piece, s.head * p.group,
+                         s.row0 + sub * p.tpt, smem_u32(&sh.q_full));
+                __syncwarp();
             }
         }
     }
 }
 
+// After an early stop: let a warp's copies in flight land before the CTA's memory goes (bounded).
+__device__ __forceinline__ void drain(unsigned long long *full, int stages, const Cursor &at) {
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t i = 0; i < (uint32_t)stages; ++i)  // (a stage not yet used this time round completed before)
+        while (!mbar_test_wait(smem_u32(full + i), at.phase ^ (i >= at.stage)) && global_timer_ns() - t0 < 2000000ull) {
+        }
+    while (global_timer_ns() - t0 < 50000ull) {
+    }
+}
+
 // The MMAs of one CTA, by a converged warp, one elected lane issuing.
 template <int D>
-__device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, const Waiter &wait, uint32_t q0, uint32_t ring,
-                                         uint32_t tmem) {
+__device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, const Waiter &wait, uint32_t q0, uint32_t k_ring,
+                                         uint32_t v_ring, uint32_t tmem) {
     using C = Cfg<D>;
     constexpr int NT = C::NT, BN = C::BN;
     constexpr uint32_t kStep = C::STAGE >> 4;
-    Cursor at;                // the ring's next block to read
+    Cursor ka, va;            // the rings' next blocks to read
     uint32_t np[2] = {0, 0};  // P's begun of each slot
     if (p.inject && !wait(sh.never, 0)) return;
-    const uint32_t q_lo = desc_lo(q0, 16), k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, BN * 128);
+    const uint32_t q_lo = desc_lo(q0, 16), k_lo = desc_lo(k_ring, 16), v_lo = desc_lo(v_ring, BN * 128);
     // S slot = Q tile t times the K block in ring stage st
     auto mma_s = [&](int t, int slot, uint32_t st) {
         const uint32_t kb = k_lo + st * kStep, qb = q_lo + t * (C::Q_TILE >> 4);
@@ -547,7 +553,7 @@ __device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, con
     };
     // O tile t (+)= half h of the slot's P times its keys' rows of the V block in ring stage st
     auto mma_o = [&](int t, int slot, uint32_t st, bool first, int h) {
-        const uint32_t vb = v_lo + st * kStep + h * (BN / 32) * 128, pb = tmem + slot * C::S_COL + h * (BN / 32) * 8;
+        const uint32_t vb = v_lo + st * kStep + h * (BN / 32) * 128, pb = tmem + slot * C::S_COL + h * (BN / 4);
 #pragma unroll
         for (int e = 0; e < BN / 32; ++e)
             mma_ts(tmem + C::O_COL + t * D, pb + e * 8, vb + e * 128, C::IDESC_O, !(first && h == 0 && e == 0));
@@ -562,74 +568,45 @@ __device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, con
         __syncwarp();
         if (elect_one()) mbar_arrive(smem_u32(&sh.seg_empty[k % kSegs]));
         if (!wait(sh.q_full, k & 1)) return;
-        if (NT == 2) {
-            // ring: K0 V0 K1 V1 ...; V(j-1) and K(j) are read together
-            uint32_t v = 0;
-            for (int j = 0; j <= nb; ++j) {
-                if (j > 0) {
-                    v = at.stage;
-                    if (!wait(sh.full[v], at.phase)) return;
-                    at.next(p.stages);
-                }
-                const uint32_t kk = at.stage;
-                if (j < nb) {
-                    if (!wait(sh.full[kk], at.phase)) return;
-                    at.next(p.stages);
-                }
-                for (int t = 0; t < subs; ++t) {
-                    if (j > 0) {
-                        if (!wait_p(t, 0)) return;
-                        fence_after();
-                        if (elect_one()) mma_o(t, t, v, j == 1, 0);
-                        __syncwarp();
-                        if (!wait_p(t, 1)) return;
-                    }
+        for (int j = -(3 - NT); j < nb; ++j) {
+            // PV of block j, S of block j + 3 - NT (a tile a slot: the next; one tile: the next but one, whose slot
+            // is free then)
+            const int js = j + 3 - NT;
+            const uint32_t v = va.stage, kk = ka.stage;
+            if (j >= 0) {
+                if (!wait(sh.v_full[v], va.phase)) return;
+                va.next(p.v_stages);
+            }
+            if (js < nb) {
+                if (!wait(sh.k_full[kk], ka.phase)) return;
+                ka.next(p.k_stages);
+            }
+            for (int t = 0; t < subs; ++t) {
+                const int slot = NT == 2 ? t : j & 1;
+                if (j >= 0) {
+                    if (!wait_p(slot, 0)) return;
                     fence_after();
-                    if (elect_one()) {
-                        if (j > 0) mma_o(t, t, v, false, 1);
-                        if (j < nb) mma_s(t, t, kk);
-                        else commit(smem_u32(&sh.o_full[t]));
+                    if (elect_one()) mma_o(t, slot, v, j == 0, 0);
+                    __syncwarp();
+                    if (!wait_p(slot, 1)) return;
+                }
+                fence_after();
+                if (elect_one()) {
+                    if (j >= 0) {
+                        mma_o(t, slot, v, false, 1);
+                        if (j == nb - 1) commit(smem_u32(&sh.o_full[t]));
+                        else if (NT == 1) commit(smem_u32(&sh.pv_done));
+                        if (t == subs - 1) commit(smem_u32(&sh.v_empty[v]));
+                    }
+                    if (js < nb) {
+                        mma_s(t, slot, kk);
                         if (t == subs - 1) {
-                            if (j > 0) commit(smem_u32(&sh.empty[v]));
-                            if (j < nb) commit(smem_u32(&sh.empty[kk]));
-                            if (j == nb - 1) commit(smem_u32(&sh.q_empty));
+                            commit(smem_u32(&sh.k_empty[kk]));
+                            if (js == nb - 1) commit(smem_u32(&sh.q_empty));
                         }
                     }
-                    __syncwarp();
                 }
-            }
-        } else {
-            // ring: K0 K1 V0 K2 V1 ... K(i) V(i-2) ... V(nb-1)
-            for (int i = -2; i < nb; ++i) {
-                if (i >= 0) {
-                    const uint32_t v = at.stage;
-                    if (!wait(sh.full[v], at.phase)) return;
-                    at.next(p.stages);
-                    if (!wait_p(i & 1, 0)) return;
-                    fence_after();
-                    if (elect_one()) mma_o(0, i & 1, v, i == 0, 0);
-                    __syncwarp();
-                    if (!wait_p(i & 1, 1)) return;
-                    fence_after();
-                    if (elect_one()) {
-                        mma_o(0, i & 1, v, false, 1);
-                        commit(smem_u32(i == nb - 1 ? &sh.o_full[0] : &sh.pv_done));
-                        commit(smem_u32(&sh.empty[v]));
-                    }
-                    __syncwarp();
-                }
-                if (i + 2 < nb) {
-                    const uint32_t kk = at.stage;
-                    if (!wait(sh.full[kk], at.phase)) return;
-                    at.next(p.stages);
-                    fence_after();
-                    if (elect_one()) {
-                        mma_s(0, i & 1, kk);
-                        commit(smem_u32(&sh.empty[kk]));
-                        if (i + 2 == nb - 1) commit(smem_u32(&sh.q_empty));
-                    }
-                    __syncwarp();
-                }
+                __syncwarp();
             }
         }
     }
@@ -725,13 +702,14 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                         for (int e = 0; e < 32; ++e) x[32 * c + e] = (bits >> e & 1) ? x[32 * c + e] : -INFINITY;
                     }
                 }
-                float mx[2] = {x[0], x[1]};
+                float mx[4];
 #pragma unroll
-                for (int e = 2; e < BN; e += 4) {
-                    mx[0] = max3(mx[0], x[e], x[e + 1]);
-                    if (e + 3 < BN) mx[1] = max3(mx[1], x[e + 2], x[e + 3]);
-                }
-                const float top = fmaxf(mx[0], mx[1]) * p.scale_log2;
+                for (int u = 0; u < 4; ++u) mx[u] = fmaxf(x[2 * u], x[2 * u + 1]);
+#pragma unroll
+                for (int e = 8; e < BN; e += 8)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) mx[u] = max3(mx[u], x[e + 2 * u], x[e + 2 * u + 1]);
+                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;
                 const bool raise = top > m + kLag;  // the first score above -inf raises from -inf
                 if (__any_sync(0xffffffffu, raise)) {
                     const float to = raise ? top : m;
@@ -877,41 +855,44 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
     __shared__ Shared sh;
     const AttnLaunch &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    unsigned char *s_q = smem, *s_ring = smem + C::NT * C::Q_TILE;
-    int *seq_tiles = reinterpret_cast<int *>(s_ring + (size_t)p.stages * C::STAGE);
+    unsigned char *s_q = smem, *s_k = smem + C::NT * C::Q_TILE, *s_v = s_k + (size_t)p.k_stages * C::STAGE;
+    int *seq_tiles = reinterpret_cast<int *>(s_v + (size_t)p.v_stages * C::STAGE);
     unsigned short *order = reinterpret_cast<unsigned short *>(seq_tiles + a.cache.n_seqs + 1);
 
     pdl_launch_dependents();
     if (tid == 0) {
-        for (int i = 0; i < p.stages; ++i) {
-            mbar_init(smem_u32(&sh.full[i]), 1);
-            mbar_init(smem_u32(&sh.empty[i]), 1);
+        auto init = [](unsigned long long &bar, uint32_t count) { mbar_init(smem_u32(&bar), count); };
+        for (int i = 0; i < C::MAX_STAGES; ++i) {
+            init(sh.k_full[i], 1);
+            init(sh.k_empty[i], 1);
+            init(sh.v_full[i], 1);
+            init(sh.v_empty[i], 1);
         }
-        mbar_init(smem_u32(&sh.q_full), 1);
-        mbar_init(smem_u32(&sh.q_empty), 1);
+        init(sh.q_full, 1);
+        init(sh.q_empty, 1);
         for (int t = 0; t < 2; ++t) {
-            mbar_init(smem_u32(&sh.s_full[t]), 1);
-            mbar_init(smem_u32(&sh.p_ready[t][0]), 4);
-            mbar_init(smem_u32(&sh.p_ready[t][1]), 4);
-            mbar_init(smem_u32(&sh.o_full[t]), 1);
+            init(sh.s_full[t], 1);
+            init(sh.p_ready[t][0], 4);
+            init(sh.p_ready[t][1], 4);
+            init(sh.o_full[t], 1);
         }
-        mbar_init(smem_u32(&sh.pv_done), 1);
-        mbar_init(smem_u32(&sh.tail), 1);
-        mbar_init(smem_u32(&sh.join), 4 * C::NT);
-        mbar_init(smem_u32(&sh.never), 1);
+        init(sh.pv_done, 1);
+        init(sh.tail, 1);
+        init(sh.join, C::SOFTMAX_WARPS);
+        init(sh.never, 1);
         for (int i = 0; i < kSegs; ++i) {
-            mbar_init(smem_u32(&sh.seg_full[i]), 1);
-            mbar_init(smem_u32(&sh.seg_empty[i]), 4 * C::NT + 1);
+            init(sh.seg_full[i], 1);
+            init(sh.seg_empty[i], C::SOFTMAX_WARPS + 2);
         }
         mbar_init_fence();
         sh.abort = 0;
     }
-    if (warp == 8) {
+    if (warp == kWarpMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     pdl_wait();
-    make_plan<D>(p, sh, seq_tiles, order, reinterpret_cast<int *>(s_ring));
+    make_plan<D>(p, sh, seq_tiles, order, *reinterpret_cast<PlanScratch *>(s_k));
     fence_async();  // the ring's memory goes from the plan to the TMA
     fence_before();
     __syncthreads();
@@ -919,24 +900,20 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
     const uint32_t tmem = sh.tmem;
     const Waiter wait{sh, p.timeout_ns, a.status};
 
-    if (warp >= 8) {
+    if (warp >= kWarpMma) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 9) {
+        if (warp == kWarpK) {
             Cursor at;
-            load_role<D>(p, sh, wait, mq, mk, mv, s_q, s_ring, lane, at);
+            load_role<D, false>(p, sh, wait, mq, mk, s_q, s_k, lane, at);
             __syncwarp();
-            if (*reinterpret_cast<volatile int *>(&sh.abort)) {
-                // let the copies in flight land before the CTA's memory goes (bounded)
-                const uint64_t t0 = global_timer_ns();
-                for (uint32_t i = 0; i < (uint32_t)p.stages; ++i)  // (a stage not yet used this time round completed before)
-                    while (!mbar_test_wait(smem_u32(&sh.full[i]), at.phase ^ (i >= at.stage)) &&
-                           global_timer_ns() - t0 < 2000000ull) {
-                    }
-                while (global_timer_ns() - t0 < 50000ull) {
-                }
-            }
-        } else if (warp == 8) {
-            mma_role<D>(p, sh, wait, smem_u32(s_q), smem_u32(s_ring), tmem);
+            if (*reinterpret_cast<volatile int *>(&sh.abort)) drain(sh.k_full, p.k_stages, at);
+        } else if (warp == kWarpV) {
+            Cursor at;
+            load_role<D, true>(p, sh, wait, mq, mv, s_q, s_v, lane, at);
+            __syncwarp();
+            if (*reinterpret_cast<volatile int *>(&sh.abort)) drain(sh.v_full, p.v_stages, at);
+        } else if (warp == kWarpMma) {
+            mma_role<D>(p, sh, wait, smem_u32(s_q), smem_u32(s_k), smem_u32(s_v), tmem);
             __syncwarp();
             if (*reinterpret_cast<volatile int *>(&sh.abort)) {
                 // let the MMAs in flight end before the accumulators go (bounded)
@@ -949,12 +926,12 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        if (warp < 4 * C::NT) softmax_role<D>(p, sh, wait, tmem);
+        if (warp < C::SOFTMAX_WARPS) softmax_role<D>(p, sh, wait, tmem);
     }
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == kWarpMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 // ------------------------------------------------------------------ host
@@ -991,9 +968,10 @@ cudaError_t launch(PrefillParams &p, cudaStream_t stream) {
     // most row tiles: one per sequence more than the rows fill
     const size_t tables = (size_t)(a.cache.n_seqs + 1) * 4 + (size_t)kSortTiles * 2;
     const size_t room = kSmem - tables - C::NT * C::Q_TILE;
-    p.stages = (int)(room / C::STAGE);
-    if (p.stages > C::MAX_STAGES) p.stages = C::MAX_STAGES;
-    const size_t smem = C::NT * C::Q_TILE + (size_t)p.stages * C::STAGE + tables;
+    const int stages = (int)(room / C::STAGE);  // K, which is waited for longest, gets the odd one
+    p.k_stages = (stages + 1) / 2 < C::MAX_STAGES ? (stages + 1) / 2 : C::MAX_STAGES;
+    p.v_stages = stages / 2 < C::MAX_STAGES ? stages / 2 : C::MAX_STAGES;
+    const size_t smem = C::NT * C::Q_TILE + (size_t)(p.k_stages + p.v_stages) * C::STAGE + tables;
 
     CUtensorMap mq, mk, mv;
     const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)a.M};
