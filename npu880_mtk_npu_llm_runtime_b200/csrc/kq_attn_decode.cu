@@ -87,29 +87,6 @@ __device__ __forceinline__ float sum_over_keys(float v) {
     return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
 
-// Total units cut into `parts` contiguous shares that differ by one at most.
-struct Shares {
-    long long q;          // total / parts
-    unsigned r, parts;    // total % parts
-    float inv;            // about parts / total
-    __device__ __forceinline__ Shares(long long total, int n) : parts((unsigned)n) {
-        if (total < 0xffffffffll) {  // 32-bit division where it will do
-            q = (unsigned)total / parts;
-        } else {
-            q = total / n;
-        }
-        r = (unsigned)(total - q * n);
-        inv = (float)n / (float)total;
-    }
-    __device__ __forceinline__ long long begin(int c) const { return q * c + (r * (unsigned)c) / parts; }
-    __device__ __forceinline__ int of(long long u) const {
-        int c = min((int)((float)u * inv), (int)parts - 1);
-        while (c + 1 < (int)parts && begin(c + 1) <= u) ++c;
-        while (c > 0 && begin(c) > u) --c;
-        return c;
-    }
-};
-
 struct Item {
     int seq, vhead, cost;  // sequence, item of the sequence (key head x splits), kBegin + its units
     long long begin;       // where its cost begins; its first unit stands kBegin later

@@ -9,7 +9,9 @@
 // 128-row MMA tile holds 128 / G tokens and short prompts fill it too.  A CTA takes NT = 2 such
 // tiles (heads of 64 and 128; 1 for 256) over the same key blocks: while the softmax of one tile
 // runs, the tensor core works for the other.  Bound by the tensor pipe and the exponentials alike
-// (128 x 128 x 2 x 128 operations and 128 x 128 exponentials take about the same time).
+// (128 x 128 x 2 x 128 operations and 128 x 128 exponentials take about the same time).  A share of the
+// exponentials by polynomial on the FMA pipe made it slower (a quarter: 294 us against 289): the issue
+// slots and, in long runs, the power are as scarce.
 //
 // Warps 0-3 and 4-7: softmax of tile 0 and 1, one row a thread: S from TMEM to registers, maximum,
 // exponentials, P as fp16 back into S's columns (the second product's A operand) in two halves, and the
@@ -33,7 +35,6 @@ namespace {
 
 constexpr float kBias = 4.0f;  // weights reach 2^(kBias + kLag) < 65504: fp16's relative precision reaches further down
 constexpr float kLag = 8.0f;
-constexpr int kPolyEvery = 4;  // every so many pairs of exponentials one by polynomial
 constexpr int kThreads = 384;  // 8 softmax warps, MMA, K and Q loads, V loads, one idle
 constexpr int kWarpMma = 8, kWarpK = 9, kWarpV = 10;
 constexpr int kSortTiles = 512;
@@ -64,6 +65,7 @@ struct PrefillParams {
     int k_stages, v_stages;
     unsigned long long timeout_ns;
     int inject;
+    int wide;         // rows of out start at multiples of 32 bytes
 };
 
 // ------------------------------------------------------------------ PTX
@@ -146,26 +148,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// 2^x without the special-function unit, which alone takes as long over a block's exponentials as the
-// tensor core over its products: x = n + r with n the nearest integer (Cody and Waite's reduction, n
-// from the low bits of x + 1.5 2^23), 2^r on [-1/2, 1/2] by the polynomial of degree 4 of least
-// relative error (2.6e-6, fitted; the result is rounded to 11 bits), n added to the exponent.  x is at
-// most a few; below -126 it gives 2^-126 (0 in fp16), and a NaN leaves a value past fp16's range.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.0f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.0f));
-    const float2 magic = make_float2(12582912.0f, 12582912.0f), minus = make_float2(-1.0f, -1.0f);
-    const float2 t = __fadd2_rn(x, magic);
-    const float2 r = __ffma2_rn(__fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f)), minus, x);
-    float2 y = make_float2(0.00957010128f, 0.00957010128f);
-    y = __ffma2_rn(y, r, make_float2(0.0559178603f, 0.0559178603f));
-    y = __ffma2_rn(y, r, make_float2(0.240247448f, 0.240247448f));
-    y = __ffma2_rn(y, r, make_float2(0.693121815f, 0.693121815f));
-    y = __ffma2_rn(y, r, make_float2(0.999999261f, 0.999999261f));
-    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
-}
-
 // ------------------------------------------------------------------ work
 
 // What the CTA's roles walk: the same segments (an item, or a range of its blocks) in the same order.
@@ -174,9 +156,9 @@ struct Plan {
     const unsigned short *order;     // whole items: row tiles, longest first (nullptr: last first)
     int tiles;                       // row tiles of all sequences
     int whole;                       // items go whole
-    int parts;                       // else: CTAs that share the units
+    Shares shares;                   // else: the CTAs' shares of the units
     int start_tile;                  // else: the tile of this CTA's first unit, and that tile's first unit
-    long long start_begin, total, c0, c1;
+    long long start_begin, c0, c1;
 };
 
 struct Segment {
@@ -232,23 +214,25 @@ template <int D>
 struct Walk {
     const PrefillParams &p;
     const Plan &plan;
-    int k = 0;            // whole items: the CTA's next
+    unsigned k = 0;       // whole items: the CTA's next
     long long unit;       // else: the next unit
     int tile;
     long long begin;
     __device__ Walk(const PrefillParams &pp, const Plan &pl)
         : p(pp), plan(pl), unit(pl.c0), tile(pl.start_tile), begin(pl.start_begin) {}
     __device__ bool next(Segment &s) {
-        const int heads = p.a.cache.kv_heads;
+        const unsigned heads = p.a.cache.kv_heads;
         if (plan.whole) {
-            const long long G = gridDim.x, c = blockIdx.x;
-            const long long idx = k * G + ((k & 1) ? G - 1 - c : c);
-            if (k * G >= (long long)plan.tiles * heads) return false;
-            ++k;
-            if (idx >= (long long)plan.tiles * heads) return next(s);
-            const int rank = (int)(idx / heads);
-            s.head = (int)(idx % heads);
-            s.tile = plan.order ? plan.order[rank] : plan.tiles - 1 - rank;
+            const unsigned G = gridDim.x, c = blockIdx.x, items = plan.tiles * heads;
+            unsigned idx;
+            do {
+                if (k * G >= items) return false;
+                idx = k * G + ((k & 1) ? G - 1 - c : c);
+                ++k;
+            } while (idx >= items);
+            const unsigned rank = idx / heads;
+            s.head = (int)(idx - rank * heads);
+            s.tile = plan.order ? plan.order[rank] : plan.tiles - 1 - (int)rank;
             const int seq = seq_of_tile(plan.seq_tiles, p.a.cache.n_seqs, s.tile);
             tile_of<D>(p, seq, s.tile - plan.seq_tiles[seq], s);
             s.begin = 0;
@@ -258,9 +242,9 @@ struct Walk {
         const int seq = seq_of_tile(plan.seq_tiles, p.a.cache.n_seqs, tile);
         tile_of<D>(p, seq, tile - plan.seq_tiles[seq], s);
         s.tile = tile;
-        const long long r = unit - begin;
-        s.head = (int)(r / s.nb);
-        s.b0 = (int)(r % s.nb);
+        const unsigned r = (unsigned)(unit - begin);  // below blocks x heads of a tile: 2^24 x 2^8 at most
+        s.head = (int)(r / (unsigned)s.nb);
+        s.b0 = (int)(r - (unsigned)s.head * (unsigned)s.nb);
         s.begin = begin + (long long)s.head * s.nb;
         const long long left = plan.c1 - unit;
         s.b1 = s.nb - s.b0 < left ? s.nb : s.b0 + (int)left;
@@ -393,30 +377,45 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         most = max(most, scratch.red_max[w]);
     }
     total *= heads;
-    const int whole = most <= total / (int)gridDim.x + kJoinBlocks;
-    const int parts = (int)min((long long)gridDim.x, total);
-    const bool sorted = whole && tiles <= kSortTiles;
-    if (sorted) {
+    // Whole items in snake order, unless the fullest CTA would get more than an even share and a join.
+    const int G = gridDim.x;
+    const Shares even(total > 0 ? total : 1, G);
+    const bool sorted = tiles <= kSortTiles;
+    bool whole = (long long)tiles * heads >= 32ll * G;  // (so many that the order evens out)
+    if (!whole && most <= even.q + kJoinBlocks && sorted) {
         for (int i = tid; i < tiles; i += kThreads) {
             int rank = 0;
             for (int j = 0; j < tiles; ++j) rank += nbs[j] > nbs[i] || (nbs[j] == nbs[i] && j < i);
             order[rank] = (unsigned short)i;
         }
+        __syncthreads();
+        int fits = 1;
+        for (int c = tid; c < G; c += kThreads) {
+            int sum = 0;
+            for (int k = 0; k * G < tiles * heads; ++k) {
+                const unsigned idx = k * G + ((k & 1) ? G - 1 - c : c);
+                if (idx < (unsigned)(tiles * heads)) sum += nbs[order[idx / (unsigned)heads]];
+            }
+            fits &= sum <= even.q + kJoinBlocks;
+        }
+        whole = __syncthreads_and(fits);
     }
     if (tid == 0) {
         Plan &pl = sh.plan;
         pl.seq_tiles = seq_tiles;
-        pl.order = sorted ? order : nullptr;
+        pl.order = sorted && (long long)tiles * heads < 32ll * G ? order : nullptr;
         pl.tiles = tiles;
         pl.whole = whole;
-        pl.parts = parts;
-        pl.total = total;
         pl.c0 = pl.c1 = 0;
         pl.start_tile = 0;
         pl.start_begin = 0;
-        if (!whole && (int)blockIdx.x < parts) {
-            pl.c0 = part_begin(total, parts, blockIdx.x);
-            pl.c1 = part_begin(total, parts, blockIdx.x + 1);
+        const int parts = (int)min((long long)G, total);
+        if (!whole) {
+            pl.shares = parts == G ? even : Shares(total, parts);
+            if ((int)blockIdx.x < parts) {
+                pl.c0 = pl.shares.begin(blockIdx.x);
+                pl.c1 = pl.shares.begin(blockIdx.x + 1);
+            }
         }
     }
     __syncthreads();
@@ -628,20 +627,30 @@ __device__ __forceinline__ void mend_rows(const PrefillParams &p, const Segment 
     }
 }
 
-// 32 values of a row, rounded, to out (where `write`); true when one is not finite
-__device__ __forceinline__ bool put32(const float *o, uint16_t *out, bool write) {
-    bool odd = false;
+// 32 values of a row, times `by`, rounded, to out (where `write`).  `odd` turns NaN when one is not
+// finite (0 times it is NaN).  With rows that allow it 32 bytes a store: a warp's lanes write to 32
+// rows, so a 16-byte store would fill half a sector at each.
+__device__ __forceinline__ void put32(const float *o, float by, uint16_t *out, bool write, bool wide, float2 &odd) {
     uint32_t h[16];
+    const float2 by2 = make_float2(by, by), zero = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        odd |= !(fabsf(o[2 * e]) <= 65504.0f) || !(fabsf(o[2 * e + 1]) <= 65504.0f);
-        h[e] = f2_to_h2(o[2 * e], o[2 * e + 1]);
+        const float2 v = __fmul2_rn(make_float2(o[2 * e], o[2 * e + 1]), by2);
+        odd = __ffma2_rn(v, zero, odd);
+        h[e] = f2_to_h2(v.x, v.y);
     }
-    if (write)
+    if (!write) return;
+    if (wide) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + 16 * e), "r"(h[8 * e]), "r"(h[8 * e + 1]),
+                         "r"(h[8 * e + 2]), "r"(h[8 * e + 3]), "r"(h[8 * e + 4]), "r"(h[8 * e + 5]), "r"(h[8 * e + 6]), "r"(h[8 * e + 7])
+                         : "memory");
+    } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             *reinterpret_cast<uint4 *>(out + 8 * e) = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
-    return odd;
+    }
 }
 
 // Softmax and epilogue of row tile t, by 128 threads with a row each.
@@ -744,12 +753,8 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             float2 w = __ffma2_rn(make_float2(x[32 * c + 2 * e], x[32 * c + 2 * e + 1]), scale2, off2);
-                            if (e % kPolyEvery == kPolyEvery - 1) {
-                                w = exp2_poly(w);
-                            } else {
-                                w.x = exp2_fast(w.x);
-                                w.y = exp2_fast(w.y);
-                            }
+                            w.x = exp2_fast(w.x);
+                            w.y = exp2_fast(w.y);
                             sum[e & 1] = __fadd2_rn(sum[e & 1], w);
                             h[e] = f2_to_h2(w.x, w.y);
                         }
@@ -768,37 +773,33 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
             fence_after();
             if (*reinterpret_cast<const volatile int *>(&s.bad)) l = NAN;  // mended below
             if (whole) {
-                const float inv = 1.0f / l;
-                bool odd = m == -INFINITY;
+                float2 odd = make_float2(0.0f, 0.0f);
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     float o[32];
                     tmem_ld32(o_base + 32 * c, o);
                     wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] *= inv;
-                    odd |= put32(o, out + 32 * c, mine);
+                    put32(o, 1.0f / l, out + 32 * c, mine, p.wide, odd);
                 }
-                mend_rows<D>(p, s, mine && odd, tok, head, lane);
+                mend_rows<D>(p, s, mine && (m == -INFINITY || !(odd.x + odd.y == 0.0f)), tok, head, lane);
             } else {
-                // this CTA's part: [value][row], then m and l
-                float *part = a.parts + (size_t)(2 * blockIdx.x + (b0 == 0)) * part_rows * (D + 2) + t * 128 + r;
+                // this CTA's part: [value / 4][row][4], then (m, l) of each row
+                float4 *part = reinterpret_cast<float4 *>(a.parts + (size_t)(2 * blockIdx.x + (b0 == 0)) * part_rows * (D + 2)) + t * 128 + r;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     float o[32];
                     tmem_ld32(o_base + 32 * c, o);
                     wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) part[(size_t)(32 * c + e) * part_rows] = o[e];
+                    for (int e = 0; e < 8; ++e) part[(8 * c + e) * part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
-                part[(size_t)D * part_rows] = m;
-                part[(size_t)(D + 1) * part_rows] = l;
+                reinterpret_cast<float2 *>(part - (t * 128 + r) + D / 4 * part_rows)[t * 128 + r] = make_float2(m, l);
             }
         }
         if (!whole) {
             // the last CTA that brings a part of the item joins them in order
-            const int first = part_of(sh.plan.total, sh.plan.parts, s.begin);
-            const int last = part_of(sh.plan.total, sh.plan.parts, s.begin + s.nb - 1);
+            const int first = sh.plan.shares.of(s.begin);
+            const int last = sh.plan.shares.of(s.begin + s.nb - 1);
             if (!together()) return;
             if (tid == 0) {
                 // after the barrier: the release covers all of the CTA's rows
@@ -810,34 +811,55 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
             if (!together()) return;
             if (join && active) {
                 auto part_at = [&](int c) {
-                    return a.parts + (size_t)(2 * c + (c == first)) * part_rows * (D + 2) + t * 128 + r;
+                    return reinterpret_cast<const float4 *>(a.parts + (size_t)(2 * c + (c == first)) * part_rows * (D + 2));
                 };
+                auto stat_at = [&](int c) { return __ldcg(reinterpret_cast<const float2 *>(part_at(c) + D / 4 * part_rows) + t * 128 + r); };
                 float M = -INFINITY, L = 0.0f;
-                for (int c = first; c <= last; ++c) M = fmaxf(M, __ldcg(part_at(c) + (size_t)D * part_rows));
+#pragma unroll 4
                 for (int c = first; c <= last; ++c) {
-                    const float mc = __ldcg(part_at(c) + (size_t)D * part_rows);
-                    const float lc = __ldcg(part_at(c) + (size_t)(D + 1) * part_rows);
+                    const float2 ml = stat_at(c);
+                    const float top = fmaxf(M, ml.x);
                     // a part without a score above -inf adds nothing; NaN (a NaN score, a missing page) stays
-                    L += mc == -INFINITY ? (lc != lc ? lc : 0.0f) : exp2_fast(mc - M) * lc;
+                    L = L * (M == -INFINITY ? 1.0f : exp2_fast(M - top)) +
+                        (ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.0f) : exp2_fast(ml.x - top) * ml.y);
+                    M = top;
                 }
                 const float inv = 1.0f / L;
-                bool odd = M == -INFINITY || !(fabsf(inv) <= 3e38f);
+                float2 odd = make_float2(0.0f, 0.0f);
+                // 32 values of each part in turn, the next ones on their way meanwhile
+                const int n = last - first + 1;
+                float4 ahead[8];
+                auto fetch = [&](int c0, int i) {
+                    const float4 *part = part_at(first + i) + c0 / 4 * part_rows + t * 128 + r;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) ahead[e] = __ldcg(part + e * part_rows);
+                };
+                fetch(0, 0);
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
                     float o[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0.0f;
 #pragma unroll 1
-                    for (int c = first; c <= last; ++c) {
-                        const float *part = part_at(c);
-                        const float mc = __ldcg(part + (size_t)D * part_rows);
-                        const float w = mc == -INFINITY ? 0.0f : exp2_fast(mc - M) * inv;
+                    for (int i = 0; i < n; ++i) {
+                        float4 v[8];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] += w * __ldcg(part + (size_t)(c0 + e) * part_rows);
+                        for (int e = 0; e < 8; ++e) v[e] = ahead[e];
+                        const float mc = stat_at(first + i).x;
+                        if (i + 1 < n) fetch(c0, i + 1);
+                        else if (c0 + 32 < D) fetch(c0 + 32, 0);
+                        const float w = mc == -INFINITY ? 0.0f : exp2_fast(mc - M);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            o[4 * e] += w * v[e].x;
+                            o[4 * e + 1] += w * v[e].y;
+                            o[4 * e + 2] += w * v[e].z;
+                            o[4 * e + 3] += w * v[e].w;
+                        }
                     }
-                    odd |= put32(o, out + c0, mine);
+                    put32(o, inv, out + c0, mine, p.wide, odd);
                 }
-                mend_rows<D>(p, s, mine && odd, tok, head, lane);
+                mend_rows<D>(p, s, mine && (M == -INFINITY || !(odd.x + odd.y == 0.0f)), tok, head, lane);
             }
         }
         __syncwarp();
@@ -860,6 +882,9 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
     unsigned short *order = reinterpret_cast<unsigned short *>(seq_tiles + a.cache.n_seqs + 1);
 
     pdl_launch_dependents();
+    if (tid == 32) {
+        for (const CUtensorMap *m : {&mq, &mk, &mv}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+    }
     if (tid == 0) {
         auto init = [](unsigned long long &bar, uint32_t count) { mbar_init(smem_u32(&bar), count); };
         for (int i = 0; i < C::MAX_STAGES; ++i) {
@@ -1026,6 +1051,7 @@ cudaError_t launch_attn_prefill(const AttnLaunch &L, cudaStream_t stream) {
     p.tpt = 128 / p.group;
     p.timeout_ns = L.timeout_ns;
     p.inject = L.inject;
+    p.wide = kv_aligned(L.out, 32) && L.out_stride % 16 == 0;
     switch (L.cache.head_dim) {
         case 64: return launch<64>(p, stream);
         case 128: return launch<128>(p, stream);

@@ -101,15 +101,29 @@ KQ_HD KvRows kv_rows(int start, int end, int M, bool &bad) {
     return r;
 }
 
-// Share c of `total` units over `parts`: [part_begin(c), part_begin(c + 1)).
-KQ_HD long long part_begin(long long total, int parts, int c) { return total * c / parts; }
-// The part that holds unit u.
-KQ_HD int part_of(long long total, int parts, long long u) {
-    int c = (int)(u * parts / total);
-    while (c + 1 < parts && part_begin(total, parts, c + 1) <= u) ++c;
-    while (c > 0 && part_begin(total, parts, c) > u) --c;
-    return c;
-}
+// Total units cut into `parts` contiguous shares that differ by one at most.
+struct Shares {
+    long long q;          // total / parts
+    unsigned r, parts;    // total % parts
+    float inv;            // about parts / total
+    KQ_HD Shares() {}
+    KQ_HD Shares(long long total, int n) : parts((unsigned)n) {
+        if (total < 0xffffffffll) {  // 32-bit division where it will do
+            q = (unsigned)total / parts;
+        } else {
+            q = total / n;
+        }
+        r = (unsigned)(total - q * n);
+        inv = (float)n / (float)total;
+    }
+    KQ_HD long long begin(int c) const { return q * c + (r * (unsigned)c) / parts; }
+    KQ_HD int of(long long u) const {
+        int c = (int)((float)u * inv) < (int)parts - 1 ? (int)((float)u * inv) : (int)parts - 1;
+        while (c + 1 < (int)parts && begin(c + 1) <= u) ++c;
+        while (c > 0 && begin(c) > u) --c;
+        return c;
+    }
+};
 
 // ------------------------------------------------------------------ checks (host)
 

@@ -24,8 +24,8 @@ int sees(int p, int len, int window, int sinks, int j) { return kv_sees(kv_span(
 int count(int p, int len, int window, int sinks) { return kv_count(kv_span(p, len, window, sinks)); }
 int nth(int p, int len, int window, int sinks, int e) { return kv_nth(kv_span(p, len, window, sinks), e); }
 int blocks(int kept, int lo, int hi, int B, int *o) { KvBlocks b = kv_blocks(kept, lo, hi, B); for (int i = 0; i < b.count; ++i) o[i] = kv_block(b, i); return b.count; }
-long long begin_of(long long total, int parts, int c) { return part_begin(total, parts, c); }
-int part(long long total, int parts, long long u) { return part_of(total, parts, u); }
+long long begin_of(long long total, int parts, int c) { return Shares(total, parts).begin(c); }
+int part(long long total, int parts, long long u) { return Shares(total, parts).of(u); }
 long long row(int n_pages, int shift, int heads, int dim, int page, int head, int slot) {
     KvView v{}; v.n_pages = n_pages; v.page_shift = shift; v.kv_heads = heads; v.head_dim = dim; return kv_row(v, page, head, slot); }
 int length(int stride, int shift, int len, int *bad) { KvView v{}; v.table_stride = stride; v.page_shift = shift; bool b = false; int r = kv_length(v, len, b); *bad = b; return r; }
