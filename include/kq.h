@@ -321,6 +321,30 @@ int kq_attn_decode_async(kq_ctx *ctx, const kq_kv_cache *cache, const kq_attn *a
  * sequences are left as they were. */
 int kq_attn_prefill_async(kq_ctx *ctx, const kq_kv_cache *cache, const kq_attn *a);
 
+/* The attention block of a layer, the counterpart of kq_run_ffn_async (the engine's ENG:7950-8261
+ * around its attention):  x_out = x_in + W_o . attention(q, cache)  with q, k, v = W . rmsnorm(x_in,
+ * gamma), the append of k and v, and kq_attn_decode_async (q_start NULL) or kq_attn_prefill_async. */
+typedef struct kq_attn_layer {
+    const kq_weight *q, *k, *v, *o;    /* [heads * D][hidden], [kv_heads * D][hidden] twice, [hidden][heads * D] */
+    const uint16_t *gamma;             /* fp16 [hidden] */
+    const uint16_t *q_gamma, *k_gamma; /* fp16 [head_dim] per-head norms, NULL: none */
+    const kq_rope *rope;               /* NULL: none */
+    const kq_kv_cache *cache;
+    int heads;
+    int window, sinks;                 /* as in kq_attn */
+    float scale;
+    float eps;                         /* of the per-head norms */
+} kq_attn_layer;
+/* M rows of x_in / x_out (fp16 [M][hidden]); seq_dev and pos_dev as in kq_kv_append_async, kv_len_dev
+ * and q_start_dev as in kq_attn (kv_len counts the appended rows).  A row of no sequence comes out as
+ * it went in.  One eager call at the largest M sizes the scratch; then a call allocates nothing and
+ * can be captured into a CUDA graph, which keeps reading x_in, the tables and the lengths where they
+ * were.  As for every call of this library, the work of one context (its graphs included) shares
+ * that context's scratch: let no two run at the same time on different streams. */
+int kq_run_attn_async(kq_ctx *ctx, const kq_attn_layer *layer, int M, const int32_t *seq_dev, const int32_t *pos_dev,
+                      const int32_t *kv_len_dev, const int32_t *q_start_dev, const uint16_t *x_in_dev,
+                      uint16_t *x_out_dev);
+
 /* ---------------------------------------------------------------- LM head */
 
 /* Full-vocabulary LM head over M normalised fp16 rows x [M][K]: logits (fp16 [M][rows], may be

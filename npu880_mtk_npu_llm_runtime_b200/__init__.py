@@ -46,6 +46,7 @@ EXPORTS = (
     "kq_rmsnorm_fp16_rows", "kq_swiglu_fp16_rows", "kq_rmsnorm_q8k_async", "kq_swiglu_q8k_async",
     "kq_run_ffn", "kq_run_ffn_async",
     "kq_rope_init", "kq_qk_norm_rope_async", "kq_kv_append_async", "kq_attn_decode_async", "kq_attn_prefill_async",
+    "kq_run_attn_async",
     "kq_lm_head_argmax", "kq_lm_head_argmax_async", "kq_lm_head_argmax_noalloc", "kq_eval_indexed_rows_argmax",
     "kq_dequant_rows", "kq_dequant_rows_async", "kq_embed_rows", "kq_embed_rows_async",
     "kq_gguf_open", "kq_gguf_open_memory", "kq_gguf_close", "kq_gguf_info", "kq_gguf_tensor_count",
@@ -112,6 +113,13 @@ class AttnStruct(C.Structure):
                 ("window", C.c_int), ("sinks", C.c_int), ("scale", C.c_float)]
 
 
+class AttnLayerStruct(C.Structure):
+    """kq_attn_layer: the weights, norms and cache of a layer's attention block."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("gamma", C.c_void_p),
+                ("q_gamma", C.c_void_p), ("k_gamma", C.c_void_p), ("rope", C.c_void_p), ("cache", C.c_void_p),
+                ("heads", C.c_int), ("window", C.c_int), ("sinks", C.c_int), ("scale", C.c_float), ("eps", C.c_float)]
+
+
 _vp, _i, _u32, _sz, _u64 = C.c_void_p, C.c_int, C.c_uint32, C.c_size_t, C.c_uint64
 _LIB = None
 
@@ -160,6 +168,7 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "kq_kv_append_async": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, C.c_float]),
         "kq_attn_decode_async": (_i, [_vp, _vp, _vp]),
         "kq_attn_prefill_async": (_i, [_vp, _vp, _vp]),
+        "kq_run_attn_async": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
         "kq_lm_head_argmax": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp]),
         "kq_lm_head_argmax_async": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
         "kq_lm_head_argmax_noalloc": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp]),
@@ -335,6 +344,26 @@ class Weight:
         if self.handle:
             self.ctx.L.kq_weight_free(self.ctx.handle, self.handle)
             self.handle = None
+
+
+class AttnLayer:
+    """kq_attn_layer: q, k, v and o weights, the norms' gammas (fp16 CUDA tensors), rotation and cache."""
+
+    def __init__(self, q: Weight, k: Weight, v: Weight, o: Weight, gamma, cache: KvCache, rope: Rope | None = None,
+                 q_gamma=None, k_gamma=None, window: int = 0, sinks: int = 0, scale: float = 0.0, eps: float = 1e-6):
+        import torch
+        dim = cache.struct.head_dim
+        for t, n, what in ((gamma, q.cols, "gamma"), (q_gamma, dim, "q_gamma"), (k_gamma, dim, "k_gamma")):
+            if t is None and what != "gamma":
+                continue
+            if t.dtype != torch.float16 or not t.is_contiguous() or t.numel() != n or t.device != cache.device:
+                raise ValueError(f"{what}: {n} fp16 values side by side on the cache's device are needed")
+        s = self.struct = AttnLayerStruct(q=q.handle, k=k.handle, v=v.handle, o=o.handle, gamma=_dp(gamma),
+                                          q_gamma=_dp(q_gamma), k_gamma=_dp(k_gamma), rope=rope and rope.ref,
+                                          cache=cache.ref, heads=q.rows // dim, window=window, sinks=sinks, scale=scale,
+                                          eps=eps)
+        self.cache, self.hidden, self.ref = cache, q.cols, C.addressof(s)
+        self.keep = (q, k, v, o, gamma, q_gamma, k_gamma, rope)
 
 
 class Context:
@@ -579,6 +608,19 @@ class Context:
         """attention of the sequences' last rows (a.q_start)"""
         self._here(a.cache)
         self.check(self.L.kq_attn_prefill_async(self.handle, a.cache.ref, a.ref))
+
+    def run_attn_async(self, layer: AttnLayer, seq, pos, kv_len, x_dev, out_dev, q_start=None):
+        """x + W_o . attention over the rows' keys and the cache (decode: one row per sequence; with q_start, prefill)"""
+        n_seqs, M = layer.cache.struct.n_seqs, x_dev.shape[0]
+        for t in (x_dev, out_dev):
+            if tuple(t.shape) != (M, layer.hidden) or t.element_size() != 2 or not t.is_contiguous():
+                raise ValueError(f"x and out: contiguous 16-bit tensors [rows, {layer.hidden}] are needed")
+        for t in (x_dev, out_dev, seq, pos, kv_len, q_start, layer.cache.k):
+            if t is not None and t.device.index != self.device:
+                raise ValueError(f"a tensor lives on {t.device}, the context on device {self.device}")
+        self.check(self.L.kq_run_attn_async(
+            self.handle, layer.ref, M, _ints(seq, "sequences", M), _ints(pos, "positions", M), _ints(kv_len, "kv_len", n_seqs),
+            None if q_start is None else _ints(q_start, "q_start", n_seqs + 1), _dp(x_dev), _dp(out_dev)))
 
     # ---- several GPUs: the gather in the LM head GEMV (kq_peer_*, kq_gemm_peer_gather_async)
     def peer_region_bytes(self, M: int, row_stride: int) -> int:

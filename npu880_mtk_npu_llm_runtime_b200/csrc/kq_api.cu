@@ -1266,6 +1266,75 @@ extern "C" int kq_attn_prefill_async(kq_ctx *c, const kq_kv_cache *cache, const 
     return KQ_OK;
 }
 
+extern "C" int kq_run_attn_async(kq_ctx *c, const kq_attn_layer *l, int M, const int32_t *seq, const int32_t *pos,
+                                 const int32_t *kv_len, const int32_t *q_start, const uint16_t *x_in, uint16_t *x_out) {
+    if (!c || !l || !l->q || !l->k || !l->v || !l->o || !l->gamma || !l->cache || !x_in || !x_out)
+        return fail(c, KQ_ERR_INVALID_ARGUMENT, "NULL argument");
+    for (const kq_weight *w : {l->q, l->k, l->v, l->o})
+        if (int r = check_weight_device(c, w)) return r;
+    const char *why = "";
+    if (int r = kq::check_cache(l->cache, &why)) return fail(c, r, "%s", why);
+    const int D = l->cache->head_dim, hidden = l->q->cols;
+    if (l->heads < 1 || l->heads > KQ_MAX_HEADS) return fail(c, KQ_ERR_SHAPE, "heads = %d", l->heads);
+    const int qd = l->heads * D, kd = l->cache->kv_heads * D, rows = qd + 2 * kd;
+    if (l->q->rows != qd || l->k->rows != kd || l->v->rows != kd || l->k->cols != hidden || l->v->cols != hidden ||
+        l->o->cols != qd || l->o->rows != hidden)
+        return fail(c, KQ_ERR_SHAPE, "attention weights do not chain: q %dx%d k %dx%d v %dx%d o %dx%d, %d and %d heads of %d",
+                    l->q->rows, l->q->cols, l->k->rows, l->k->cols, l->v->rows, l->v->cols, l->o->rows, l->o->cols, l->heads,
+                    l->cache->kv_heads, D);
+    if (int r = validate_mk(c, M, hidden)) return r;
+    if (int r = validate_mk(c, M, qd)) return r;
+    const OnDevice on(c->device);
+    // scratch: xn [M][hidden] | q, k, v rows side by side | attention's output | q8k(xn) | q8_0(xn)
+    auto al = [](size_t v) { return (v + 255) & ~(size_t)255; };
+    const size_t xnb = al((size_t)M * hidden * 2), qkvb = al((size_t)M * rows * 2), ab = al((size_t)M * qd * 2);
+    const size_t q8b = al((size_t)M * (hidden / 256) * sizeof(kq::BlockQ8K));
+    const size_t q80b = al((size_t)M * (hidden / 32) * sizeof(kq::BlockQ80));
+    if (int r = ensure(c, c->misc, xnb + qkvb + ab + q8b + q80b)) return r;
+    uint8_t *base = static_cast<uint8_t *>(c->misc.p);
+    uint16_t *xn = reinterpret_cast<uint16_t *>(base), *qkv = reinterpret_cast<uint16_t *>(base + xnb);
+    uint16_t *att = reinterpret_cast<uint16_t *>(base + xnb + qkvb);
+    void *q8 = base + xnb + qkvb + ab, *q80 = base + xnb + qkvb + ab + q8b;
+    // every refusal before the first launch
+    kq_heads hq{qkv, (size_t)rows, qkv, (size_t)rows, l->heads, l->q_gamma};
+    kq_heads hk{qkv + qd, (size_t)rows, nullptr, 0, l->cache->kv_heads, l->k_gamma};
+    kq_heads hv{qkv + qd + kd, (size_t)rows, nullptr, 0, l->cache->kv_heads, nullptr};
+    kq_attn at{qkv, (size_t)rows, att, (size_t)qd, l->heads, M, kv_len, q_start, l->window, l->sinks, l->scale};
+    if (int r = kq::check_append(l->cache, l->rope, M, seq, pos, &hq, &hk, &hv, &why)) return fail(c, r, "%s", why);
+    if (int r = kq::check_attn(l->cache, &at, q_start != nullptr, &why)) return fail(c, r, "%s", why);
+    if (!(l->eps >= 0.0f)) return fail(c, KQ_ERR_INVALID_ARGUMENT, "eps must not be negative");
+
+    KQ_CUDA(c, kq::launch_rmsnorm_q8k(x_in, l->gamma, xn, q8, M, hidden, c->stream, c->pdl));
+    const bool any_q80 = l->q->type == KQ_TYPE_Q8_0 || l->k->type == KQ_TYPE_Q8_0 || l->v->type == KQ_TYPE_Q8_0;
+    if (any_q80) KQ_CUDA(c, kq::launch_quantize(KQ_TYPE_Q8_0, xn, hidden, M, hidden, q80, c->stream));
+    kq_task t[3] = {};
+    const kq_weight *w[3] = {l->q, l->k, l->v};
+    const int at_row[3] = {0, qd, qd + kd};
+    for (int i = 0; i < 3; ++i) {
+        t[i].w = w[i];
+        t[i].rows = w[i]->rows;
+        t[i].dst = qkv + at_row[i];
+        t[i].dst_stride = rows;
+    }
+    if (int r = run_gemv(c, t, 3, M, hidden, nullptr, 0, q8, any_q80 ? q80 : nullptr)) return r;
+    if (int r = kq_kv_append_async(c, l->cache, l->rope, M, seq, pos, &hq, &hk, &hv, l->eps)) return r;
+    if (q_start) {
+        // rows of no sequence: attention leaves them, and zeros here leave x_in there
+        KQ_CUDA(c, cudaMemsetAsync(att, 0, (size_t)M * qd * 2, c->stream));
+        if (int r = kq_attn_prefill_async(c, l->cache, &at)) return r;
+    } else if (int r = kq_attn_decode_async(c, l->cache, &at)) {
+        return r;
+    }
+    kq_task o{};
+    o.w = l->o;
+    o.rows = hidden;
+    o.dst = x_out;
+    o.dst_stride = hidden;
+    o.residual = x_in;
+    o.res_stride = hidden;
+    return run_gemv(c, &o, 1, M, qd, reinterpret_cast<const __half *>(att), qd, nullptr, nullptr);
+}
+
 // =================================================================== LM head
 
 extern "C" int kq_lm_head_argmax_async(kq_ctx *c, const kq_weight *w, const uint16_t *x, int M, uint16_t *logits,

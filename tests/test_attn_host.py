@@ -235,7 +235,8 @@ def test_no_context_is_refused():
 
 def test_structs_have_the_header_layout(tmp_path):
     """the ctypes mirrors of the attention structs against the C compiler's offsets"""
-    mirrors = {"kq_rope": kq.RopeStruct, "kq_kv_cache": kq.KvCacheStruct, "kq_heads": kq.HeadsStruct, "kq_attn": kq.AttnStruct}
+    mirrors = {"kq_rope": kq.RopeStruct, "kq_kv_cache": kq.KvCacheStruct, "kq_heads": kq.HeadsStruct, "kq_attn": kq.AttnStruct,
+               "kq_attn_layer": kq.AttnLayerStruct}
     src = "#include <stddef.h>\n#include <stdio.h>\n#include \"kq.h\"\nint main(void) {\n"
     for name, S in mirrors.items():
         for f, _ in S._fields_:
