@@ -21,11 +21,13 @@ activation is quantized to Q8_K inside the kernel and the 9728 fp32 outputs are 
 sharded over the ranks and the logit slices all-gathered with NCCL, and (record p2p_gather) with
 the gather inside the GEMV over NVLink.  --config ffn / prefill / decode run configs 2-4
 (--tokens M; --ffn-fused 0 times the FFN block's four launches instead of the persistent kernel).
+prefill and decode leave the attention core out (o takes q's output) unless --context N puts it in:
+every layer's attention block with a paged cache of N earlier tokens per sequence.
 --impl reference times the reference engine's own CPU path (oracle/_ref, built from its
 sources) on this host on the same workload.
 
 python bench.py [--gpus N] [--steps K] [--warmup W] [--impl ours|reference]
-                [--config gemv|lm_head|ffn|prefill|decode] [--tokens M]
+                [--config gemv|lm_head|ffn|prefill|decode] [--tokens M] [--context N]
 """
 from __future__ import annotations
 
@@ -547,7 +549,7 @@ METRIC_FFN = "tree-verify FFN block weight GB/s (Q4_K gate/up, Q6_K down)"
 METRIC_PREFILL = "prefill GEMM TOPS (36-layer Q4_K_M stack, int8 tensor cores)"
 METRIC_DECODE = "batched decode tok/s (64 sequences, 36-layer Q5_K/Q8_0 stack + sharded LM head)"
 
-HIDDEN, FFN_DIM, Q_DIM, KV_DIM, VOCAB = 2560, 9728, 4096, 1024, 151936
+HIDDEN, FFN_DIM, Q_DIM, KV_DIM, VOCAB, HEAD_DIM = 2560, 9728, 4096, 1024, 151936, 128
 
 
 def stack_layout(kind):
@@ -736,9 +738,10 @@ def run_stack(args, rank, world, local_rank):
     elif args.config in ("prefill", "decode"):
         # configs 3 and 4: the decoder stack's matrix products chained layer by layer through the
         # producers.  Per layer: RMSNorm + Q8_K (and Q8_0 for Q8_0 weights) -> q / k / v (one
-        # dispatch) -> o over q's output with the residual (the attention core is outside the
-        # path, so q's output stands in for its result) -> the FFN block (RMSNorm, gate / up,
-        # SwiGLU, down + residual).  Config 3 (prefill, M tokens): at N GPUs the FFN rows are
+        # dispatch) -> o over q's output with the residual (q's output stands in for the attention
+        # core's result; with --context the whole attention block: per-head norms, rotation, append to
+        # a paged cache, attention over it) -> the FFN block (RMSNorm, gate / up, SwiGLU, down +
+        # residual).  Config 3 (prefill, M tokens): at N GPUs the FFN rows are
         # sharded (shard.RowShardedFfn), the projections replicated.  Config 4 (decode, 64
         # sequences): the sequences split over the ranks, then the final RMSNorm, an all-gather of
         # the normalised rows, each rank's vocabulary slice of the LM head for all rows, and the
@@ -787,6 +790,29 @@ def run_stack(args, rank, world, local_rank):
                for lay in layers]
         o_tasks = [[ctx.make_tasks([dict(w=lay["o"], dst=dst, residual=src)]) for (src, dst) in ((h_a, h_mid), (h_b, h_mid))]
                    for lay in layers]
+        attn, attn_args = None, None
+        if args.context is not None:
+            # prefill: one prompt of M rows behind the context; decode: M sequences of one row each
+            seqs, new, page = (1, M, 64) if prefill else (M, 1, 64)
+            total = args.context + new
+            per_seq = -(-total // page)
+            gen = torch.Generator(device=dev)
+            gen.manual_seed(3903 + rank)
+            head = torch.from_numpy((1.0 + 0.1 * np.random.default_rng(3904).standard_normal(HEAD_DIM)).astype(np.float16)).to(dev)
+            rope = kq.Rope(HEAD_DIM, base=1e6)
+            attn = []
+            for lay in layers:
+                ck, cv = (torch.empty((seqs * per_seq, KV_DIM // HEAD_DIM, page, HEAD_DIM), dtype=f16, device=dev)
+                          .normal_(generator=gen) for _ in range(2))
+                table = torch.randperm(seqs * per_seq, generator=gen, device=dev).int().view(seqs, per_seq)
+                attn.append(kq.AttnLayer(lay["q"], lay["k"], lay["v"], lay["o"], g_attn.view(f16), kq.KvCache(ck, cv, table),
+                                         rope=rope, q_gamma=head, k_gamma=head))
+            i32 = dict(dtype=torch.int32, device=dev)
+            row = torch.arange(M, **i32)
+            attn_args = dict(seq=torch.zeros(M, **i32) if prefill else row,
+                             pos=args.context + (row if prefill else torch.zeros(M, **i32)),
+                             kv_len=torch.full((seqs,), total, **i32),
+                             q_start=torch.tensor([0, M], **i32) if prefill else None)
         rk = None
         if sharded_ffn:
             rk = shard.RowShardedFfn(ctx, plan, rank, M, dev)
@@ -798,11 +824,15 @@ def run_stack(args, rank, world, local_rank):
         def run_layers():
             src, dst = h_a, h_b
             for li, lay in enumerate(layers):
-                ctx.rmsnorm_q8k_async(src, g_attn, xn, M, HIDDEN, qx)
-                if need_q80:
-                    ctx.quantize_q8_0_async(xn, M, HIDDEN, qx0)
-                ctx.gemm_multi_q8_async(qx, qx0, M, HIDDEN, qkv[li])
-                ctx.gemm_multi_async(qo, M, Q_DIM, o_tasks[li][0 if src is h_a else 1])
+                if attn is not None:
+                    ctx.run_attn_async(attn[li], attn_args["seq"], attn_args["pos"], attn_args["kv_len"], src, h_mid,
+                                       q_start=attn_args["q_start"])
+                else:
+                    ctx.rmsnorm_q8k_async(src, g_attn, xn, M, HIDDEN, qx)
+                    if need_q80:
+                        ctx.quantize_q8_0_async(xn, M, HIDDEN, qx0)
+                    ctx.gemm_multi_q8_async(qx, qx0, M, HIDDEN, qkv[li])
+                    ctx.gemm_multi_async(qo, M, Q_DIM, o_tasks[li][0 if src is h_a else 1])
                 if rk is not None:
                     gu, dn = ffn_tasks[li][0]
                     rk.forward(h_mid, g_ffn, dst, gu, dn, gather)
@@ -815,7 +845,7 @@ def run_stack(args, rank, world, local_rank):
             def step(i):
                 h_a.copy_(x_dev)
                 run_layers()
-            launches_per_step = L * (5 + (7 if sharded_ffn else 4)) + 1
+            launches_per_step = L * (5 + (7 if sharded_ffn else 4) + (2 if attn else 0)) + 1
         else:
             v0, vrows = shard.vocab_slice(rank, world, VOCAB)
             lm_host = synth.gen_weights(synth.TYPE_Q6_K, VOCAB, HIDDEN, 4100)[v0:v0 + vrows]
@@ -849,7 +879,7 @@ def run_stack(args, rank, world, local_rank):
                 pv = pair_all.view(world, 2, SEQ)
                 r_ = torch.argmax(pv[:, 0, :], dim=0)       # first rank with the maximum = first row
                 best.copy_(pv[:, 1, :][r_, cols].long())
-            launches_per_step = L * (5 + 4 + (1 if need_q80 else 0)) + 4
+            launches_per_step = L * (5 + 4 + (1 if need_q80 else 0) + (2 if attn else 0)) + 4
 
         steps = args.steps
         warmup = max(3, args.warmup)
@@ -909,8 +939,9 @@ def run_stack(args, rank, world, local_rank):
                 result = dict(common, **{
                     "metric": METRIC_PREFILL, "value": round(value, 2), "unit": "TOPS", "scaling": "strong",
                     "config": {"workload": f"config3: {L}-layer Q4_K_M stack (q/k/o/gate/up Q4_K, v/down Q6_K) at "
-                                           f"M={M}, layers chained through RMSNorm / SwiGLU (attention core outside "
-                                           f"the path: o takes q's output)",
+                                           f"M={M}, layers chained through RMSNorm / SwiGLU "
+                                           + ("(attention core outside the path: o takes q's output)" if attn is None else
+                                              f"and the attention block, {args.context} earlier tokens"),
                                "m": M, "layers": L, "ops_per_step": ops, "weight_bytes_per_rank": rank_wbytes,
                                "l2": f"inputs larger than L2: {rank_wbytes / 2**20:.0f} MiB of weights per rank",
                                "parallelism": "replicas x1" if world == 1 else
@@ -929,7 +960,9 @@ def run_stack(args, rank, world, local_rank):
                 result = dict(common, **{
                     "metric": METRIC_DECODE, "value": round(value, 1), "unit": "tok/s", "scaling": "strong",
                     "config": {"workload": f"config4: {SEQ} sequences x 1 token, {L}-layer stack (q/o/gate/up Q5_K, "
-                                           f"k/v/down Q8_0) chained through RMSNorm / SwiGLU + final norm + Q6_K LM head "
+                                           f"k/v/down Q8_0) chained through RMSNorm / SwiGLU "
+                                           + ("" if attn is None else f"and the attention block at {args.context} earlier tokens ")
+                                           + f"+ final norm + Q6_K LM head "
                                            f"{VOCAB}x{HIDDEN} vocab-sharded with the argmax merged on the device",
                                "rows_per_rank": M, "layers": L, "weight_bytes_per_step_per_rank": rank_wbytes,
                                "parallelism": f"batch-split x{world}, LM head vocab-split + NCCL all-gathers",
@@ -1027,6 +1060,8 @@ def main():
     ap.add_argument("--config", choices=["gemv", "lm_head", "ffn", "prefill", "decode"], default="gemv")
     # (not "--m": torchrun's own parser takes it for an abbreviation of its options)
     ap.add_argument("--tokens", "--m", dest="tokens", type=int, default=0, help="tokens (ffn: 8/16/32/64 or 512/2048, prefill: 512/2048)")
+    ap.add_argument("--context", type=int, default=None, help="prefill / decode: run the attention block with this many "
+                                                              "earlier tokens per sequence (default: no attention core)")
     ap.add_argument("--ffn-fused", type=int, default=1, help="ffn: 1 = the persistent FFN kernel where it applies "
                                                               "(1-2 tokens), 0 = the four launches")
     ap.add_argument("--layers", type=int, default=36)
