@@ -79,8 +79,8 @@ int kq_synchronize(kq_ctx *ctx);
 const char *kq_last_error(const kq_ctx *ctx);
 /* Options: "pdl" -- programmatic dependent launch between consecutive kernels (default 1);
  * "timeout_ms" / "timeout_us" -- limit of every device-side wait (default 1000 ms);
- * "inject_timeout" -- failure-path test: matrix-product kernels first wait on a barrier that
- * nothing completes, so the wait runs out, the kernel returns early and the call reports
+ * "inject_timeout" -- failure-path test: matrix-product and prefill attention kernels first wait on a
+ * barrier that nothing completes, so the wait runs out, the kernel returns early and the call reports
  * KQ_ERR_TIMEOUT (default 0);
  * "gemm_path" -- products of more than 8 activation rows: 0 chooses by a cost model, 1 always
  * the weight-row-major tensor-core kernel (tcgen05; weight rows as the MMA's A operand), 2 always
@@ -227,7 +227,7 @@ int kq_run_ffn_async(kq_ctx *ctx, const kq_weight *gate, const kq_weight *up, co
  * ENG:7787-7915 (QK-norm, RoPE, active-window GQA).
  *
  * Rows of heads: fp16, one head's head_dim values after another, rows `stride` elements apart
- * (stride >= heads * head_dim, a multiple of 8; the address a multiple of 16 bytes), so that q, k
+ * (stride >= heads * head_dim, a multiple of 8, at most 2^38; the address a multiple of 16 bytes), so that q, k
  * and v can be views into one buffer.  head_dim is 64, 128 or 256. */
 #define KQ_MAX_HEAD_DIM 256
 #define KQ_MAX_HEADS 256         /* heads of a row */
@@ -336,8 +336,9 @@ typedef struct kq_attn_layer {
     float eps;                         /* of the per-head norms */
 } kq_attn_layer;
 /* M rows of x_in / x_out (fp16 [M][hidden]); seq_dev and pos_dev as in kq_kv_append_async, kv_len_dev
- * and q_start_dev as in kq_attn (kv_len counts the appended rows).  A row of no sequence comes out as
- * it went in.  One eager call at the largest M sizes the scratch; then a call allocates nothing and
+ * and q_start_dev as in kq_attn (kv_len counts the appended rows; without q_start row i is sequence i,
+ * so seq_dev[i] is i, or -1 for padding).  x_out may not overlap x_in.  A row of no sequence comes out
+ * as it went in.  One eager call at the largest M sizes the scratch; then a call allocates nothing and
  * can be captured into a CUDA graph, which keeps reading x_in, the tables and the lengths where they
  * were.  As for every call of this library, the work of one context (its graphs included) shares
  * that context's scratch: let no two run at the same time on different streams. */

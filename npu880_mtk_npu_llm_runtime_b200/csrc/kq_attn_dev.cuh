@@ -29,65 +29,80 @@ __device__ __forceinline__ int kv_page(const KvView &c, int seq, int j, int *sta
 }
 
 // One row of one head by a warp: out = sum_j softmax_j(scale q.k_j) v_j over exactly the keys of
-// `span`, everything in fp32, four keys at a time (lane i holds values [i D/32, (i+1) D/32) of the
-// head).  No key outside the span is read.
+// `span`, everything in fp32, 32 keys at a time: a lane takes a key for the scores, and values
+// [lane D/32, (lane + 1) D/32) of the row for the sum.  No key outside the span is read.
 template <int D>
 __device__ __noinline__ void attn_row(const KvView &c, int seq, int kv_head, KvSpan span, const uint16_t *q,
                                       uint16_t *out, float scale, int lane, int *status) {
-    constexpr int W = D / 64;  // 32-bit words per lane
-    constexpr int U = 4;
-    float2 qv[W], acc[W];
+    constexpr int W = D / 64;  // 32-bit words of a row per lane
+    constexpr int U = 8;       // rows of V on their way at once
+    float2 acc[W];
     const int mask = (1 << c.page_shift) - 1;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-        qv[i] = h2_to_f2(reinterpret_cast<const uint32_t *>(q)[lane * W + i]);
-        qv[i].x *= scale;
-        qv[i].y *= scale;
-        acc[i] = make_float2(0.0f, 0.0f);
-    }
-    float m = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < W; ++i) acc[i] = make_float2(0.0f, 0.0f);
+    float m = -INFINITY, sum = 0.0f;  // sum: this lane's keys
     const int n = kv_count(span);
-    int seen = 0;  // keys that were there
-    for (int e0 = 0; e0 < n; e0 += U) {
-        float s[U];
-        long long at[U];
+    bool seen = false;
+    for (int e0 = 0; e0 < n; e0 += 32) {
+        long long at = -1;
+        float s = 0.0f;
+        if (e0 + lane < n) {
+            const int j = kv_nth(span, e0 + lane), page = kv_page(c, seq, j, status);
+            if (page >= 0) at = kv_row(c, page, kv_head, j & mask);
+        }
+        if (at >= 0) {
+#pragma unroll 4
+            for (int i = 0; i < D / 8; ++i) {
+                const uint4 k = *reinterpret_cast<const uint4 *>(c.k + at + 8 * i);
+                const uint4 x = *reinterpret_cast<const uint4 *>(q + 8 * i);
+                const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, xw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            at[u] = -1;
-            s[u] = 0.0f;
-            if (e0 + u < n) {
-                const int j = kv_nth(span, e0 + u);
-                const int page = kv_page(c, seq, j, status);
-                if (page >= 0) at[u] = kv_row(c, page, kv_head, j & mask) / 2 + lane * W;
+                for (int u = 0; u < 4; ++u) {
+                    const float2 a = h2_to_f2(kw[u]), b = h2_to_f2(xw[u]);
+                    s = fmaf(a.x, b.x, fmaf(a.y, b.y, s));
+                }
             }
-            if (at[u] >= 0) {
+            s *= scale;
+        }
+        const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+        seen |= there != 0;
+        float top = at >= 0 ? s : -INFINITY;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        top = fmaxf(m, top);
+        // before the first score above -inf there is nothing to rescale; a NaN score stays NaN
+        const float old = (m == -INFINITY) ? 1.0f : __expf(m - top);
+        const float w = (at < 0 || s == -INFINITY) ? 0.0f : __expf(s - top);
+        m = top;
+        sum = sum * old + w;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            acc[i].x *= old;
+            acc[i].y *= old;
+        }
+        for (int i0 = 0; i0 < 32 && (there >> i0); i0 += U) {
+            uint32_t v[U][W];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long long row = __shfl_sync(0xffffffffu, at, i0 + u);
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    v[u][i] = row >= 0 ? reinterpret_cast<const uint32_t *>(c.v + row)[lane * W + i] : 0u;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float wu = __shfl_sync(0xffffffffu, w, i0 + u);
 #pragma unroll
                 for (int i = 0; i < W; ++i) {
-                    const float2 k = h2_to_f2(reinterpret_cast<const uint32_t *>(c.k)[at[u] + i]);
-                    s[u] += qv[i].x * k.x + qv[i].y * k.y;
+                    const float2 x = h2_to_f2(v[u][i]);
+                    acc[i].x = fmaf(wu, x.x, acc[i].x);
+                    acc[i].y = fmaf(wu, x.y, acc[i].y);
                 }
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], d);
-            if (at[u] < 0) continue;  // uniform over the warp
-            ++seen;
-            const float mn = fmaxf(m, s[u]);
-            // before the first score above -inf there is nothing to rescale; a NaN score stays NaN
-            const float old = (m == -INFINITY) ? 0.0f : __expf(m - mn);
-            const float w = (s[u] == -INFINITY) ? 0.0f : __expf(s[u] - mn);
-            sum = sum * old + w;
-            m = mn;
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const float2 v = h2_to_f2(reinterpret_cast<const uint32_t *>(c.v)[at[u] + i]);
-                acc[i].x = acc[i].x * old + w * v.x;
-                acc[i].y = acc[i].y * old + w * v.y;
-            }
-        }
     }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     const float inv = seen ? 1.0f / sum : 0.0f;  // scores all -inf: 0 / 0, NaN as in the formula
 #pragma unroll
     for (int i = 0; i < W; ++i)

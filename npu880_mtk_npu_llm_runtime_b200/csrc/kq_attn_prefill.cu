@@ -266,7 +266,7 @@ struct Shared {
     unsigned long long pv_done, tail, join, never, seg_full[kSegs], seg_empty[kSegs];
     Segment seg[kSegs];
     uint32_t tmem;
-    int abort, last;
+    int abort, last, mending;  // mending: warps that compute rows key by key, which may take long
     Plan plan;
 };
 
@@ -306,7 +306,7 @@ struct Waiter {
             if (polls & 63) continue;
             if (*reinterpret_cast<volatile int *>(&sh.abort)) return false;
             const uint64_t now = global_timer_ns();
-            if (t0 == 0) t0 = now;
+            if (t0 == 0 || *reinterpret_cast<volatile int *>(&sh.mending)) t0 = now;
             if (now - t0 > timeout_ns) {
                 *reinterpret_cast<volatile int *>(&sh.abort) = 1;
                 report_error(status, DEV_ERR_TIMEOUT);
@@ -613,10 +613,14 @@ __device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, con
 
 // Rows of a warp whose plain result does not stand: computed key by key, over exactly their own
 // keys.  These see nothing (zeros), or have a value that is not finite: a weight of 0 times an
-// infinity that only other rows see is NaN in the matrix product; or a page is missing.
+// infinity that only other rows see is NaN in the matrix product; or a page is missing.  (A row whose
+// sum is NaN saw a NaN score: all NaN, which stands.)
 template <int D>
-__device__ __forceinline__ void mend_rows(const PrefillParams &p, const Segment &s, bool odd, int tok, int head, int lane) {
+__device__ __forceinline__ void mend_rows(const PrefillParams &p, Shared &sh, const Segment &s, bool odd, int tok, int head,
+                                          int lane) {
     uint32_t todo = __ballot_sync(0xffffffffu, odd);
+    if (!todo) return;
+    if (lane == 0) atomicAdd(&sh.mending, 1);
     while (todo) {
         const int src = __ffs(todo) - 1;
         todo &= todo - 1;
@@ -625,6 +629,8 @@ __device__ __forceinline__ void mend_rows(const PrefillParams &p, const Segment 
         attn_row<D>(p.a.cache, s.seq, s.head, kv_span(s.pos0 + tk, s.len, p.a.window, p.a.sinks),
                     p.a.q + row * p.a.q_stride + hd * D, p.a.out + row * p.a.out_stride + hd * D, p.a.scale, lane, p.a.status);
     }
+    __syncwarp();
+    if (lane == 0) atomicSub(&sh.mending, 1);
 }
 
 // 32 values of a row, times `by`, rounded, to out (where `write`).  `odd` turns NaN when one is not
@@ -771,7 +777,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
             ++no;
             npv += b1 - b0 - 1;
             fence_after();
-            if (*reinterpret_cast<const volatile int *>(&s.bad)) l = NAN;  // mended below
+            const bool bad = *reinterpret_cast<const volatile int *>(&s.bad) != 0;
             if (whole) {
                 float2 odd = make_float2(0.0f, 0.0f);
 #pragma unroll 1
@@ -781,7 +787,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                     wait_ld();
                     put32(o, 1.0f / l, out + 32 * c, mine, p.wide, odd);
                 }
-                mend_rows<D>(p, s, mine && (m == -INFINITY || !(odd.x + odd.y == 0.0f)), tok, head, lane);
+                mend_rows<D>(p, sh, s, mine && (bad || m == -INFINITY || (l == l && !(odd.x + odd.y == 0.0f))), tok, head, lane);
             } else {
                 // this CTA's part: [value / 4][row][4], then (m, l) of each row
                 float4 *part = reinterpret_cast<float4 *>(a.parts + (size_t)(2 * blockIdx.x + (b0 == 0)) * part_rows * (D + 2)) + t * 128 + r;
@@ -793,7 +799,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
 #pragma unroll
                     for (int e = 0; e < 8; ++e) part[(8 * c + e) * part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
-                reinterpret_cast<float2 *>(part - (t * 128 + r) + D / 4 * part_rows)[t * 128 + r] = make_float2(m, l);
+                reinterpret_cast<float2 *>(part - (t * 128 + r) + D / 4 * part_rows)[t * 128 + r] = make_float2(bad ? NAN : m, l);  // NaN: a page is missing
             }
         }
         if (!whole) {
@@ -815,11 +821,13 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                 };
                 auto stat_at = [&](int c) { return __ldcg(reinterpret_cast<const float2 *>(part_at(c) + D / 4 * part_rows) + t * 128 + r); };
                 float M = -INFINITY, L = 0.0f;
+                bool missing = false;
 #pragma unroll 4
                 for (int c = first; c <= last; ++c) {
                     const float2 ml = stat_at(c);
+                    missing |= ml.x != ml.x;
                     const float top = fmaxf(M, ml.x);
-                    // a part without a score above -inf adds nothing; NaN (a NaN score, a missing page) stays
+                    // a part without a score above -inf adds nothing; NaN (a NaN score) stays
                     L = L * (M == -INFINITY ? 1.0f : exp2_fast(M - top)) +
                         (ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.0f) : exp2_fast(ml.x - top) * ml.y);
                     M = top;
@@ -859,7 +867,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                     }
                     put32(o, inv, out + c0, mine, p.wide, odd);
                 }
-                mend_rows<D>(p, s, mine && (M == -INFINITY || !(odd.x + odd.y == 0.0f)), tok, head, lane);
+                mend_rows<D>(p, sh, s, mine && (missing || M == -INFINITY || (L == L && !(odd.x + odd.y == 0.0f))), tok, head, lane);
             }
         }
         __syncwarp();
@@ -911,6 +919,7 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
         }
         mbar_init_fence();
         sh.abort = 0;
+        sh.mending = 0;
     }
     if (warp == kWarpMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)));

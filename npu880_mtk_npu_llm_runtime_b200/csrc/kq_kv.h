@@ -197,7 +197,7 @@ inline int check_head_rows(const void *p, size_t stride, int heads, int head_dim
         *why = "heads out of range";
         return KQ_ERR_SHAPE;
     }
-    if (stride < (size_t)heads * (size_t)head_dim || stride % 8 || stride > ((size_t)1 << 40)) {
+    if (stride < (size_t)heads * (size_t)head_dim || stride % 8 || stride > ((size_t)1 << 38)) {
         *why = "a row stride must be at least heads * head_dim and a multiple of 8";
         return KQ_ERR_INVALID_ARGUMENT;
     }

@@ -647,3 +647,106 @@ def test_prefill_long_cache(kqctx, D, H, K, seqs, window):
         kqctx.attn_prefill_async(a)
     kqctx.synchronize()
     assert (out == first).all()
+
+
+@pytest.mark.parametrize("where", ["value", "key", "query"])
+def test_prefill_nonfinite_early(kqctx, where):
+    """a value that almost every row sees: their rows hold it as in the formula, in reasonable time"""
+    rng = np.random.default_rng(12)
+    D, n = 128, 1500
+    p = R.Paged(rng, [n], 2, 16, D)
+    q = rng.standard_normal((n, 4, D)).astype(np.float16)
+    if where == "value":
+        p.v[p.table[0, 0], 1, 5, 3] = np.inf
+    elif where == "key":
+        p.k[p.table[0, 0], 1, 5, 3] = np.nan
+    else:
+        q[5:, 2:, 3] = np.nan
+    out = dev(np.zeros_like(q))
+    kqctx.attn_prefill_async(kq.Attention(cache_of(p), dev(q), out, dev(np.array([n], np.int32)), q_start=dev(np.array([0, n], np.int32))))
+    kqctx.synchronize()
+    got = out.cpu().numpy()
+    rows = [0, 3, 4, 5, 6, 127, 128, 700, n - 1]
+    want, tol = R.expect(p, q, [(i, 0, i, n) for i in rows], 0, 0)
+    close(got[rows][:, :2], want[:, :2], tol[:, :2])               # the other key head
+    close(got[:5], *R.expect(p, q, [(i, 0, i, n) for i in range(5)], 0, 0))
+    if where == "value":
+        assert not np.isfinite(got[5:, 2:, 3]).any()
+        keep = np.delete(np.arange(D), 3)
+        close(got[rows][:, 2:][..., keep], want[:, 2:][..., keep], tol[:, 2:][..., keep])
+    else:
+        assert np.isnan(got[5:, 2:]).all()
+
+
+def test_many_sequences_prefill(kqctx):
+    rng = np.random.default_rng(13)
+    for D, count in ((64, 4096), (128, 1000), (256, 4096)):
+        lens = [int(x) for x in rng.integers(0, 30, count)]
+        rows = [int(rng.integers(0, 2)) if count == 4096 else int(rng.integers(0, 9)) for _ in lens]
+        p = R.Paged(rng, lens, 1, 16, D)
+        start = np.cumsum([0] + rows).astype(np.int32)
+        M = int(start[-1])
+        assert M <= 4096
+        q = rng.standard_normal((M, 2, D)).astype(np.float16)
+        out = dev(np.full_like(q, SENTINEL))
+        kqctx.attn_prefill_async(kq.Attention(cache_of(p), dev(q), out, dev(np.array(lens, np.int32)), q_start=dev(start)))
+        kqctx.synchronize()
+        want, tol = R.expect(p, q, [(start[s] + i, s, lens[s] - rows[s] + i, lens[s]) for s in range(count) for i in range(rows[s])], 0, 0)
+        close(out.cpu().numpy(), want, tol, D)
+
+
+def test_offsets_past_32_bits(kqctx):
+    """pages at the far end of a cache of more than 2^32 values"""
+    import torch
+    rng = np.random.default_rng(14)
+    D, K, page, n, pages = 128, 8, 256, 600, 16500
+    assert (pages - 4) * K * page * D > 2 ** 32
+    p = R.Paged(rng, [0], K, page, D)
+    p.keys[0], p.values[0] = (rng.standard_normal((n, K, D)).astype(np.float16) for _ in range(2))
+    table = np.array([[pages - 2, pages - 4, pages - 1]], np.int32)
+    ck, cv = (torch.empty((pages, K, page, D), dtype=torch.float16, device="cuda") for _ in range(2))
+    cache = kq.KvCache(ck, cv, dev(table))
+    h = dev(np.concatenate([p.keys[0].reshape(n, -1), p.values[0].reshape(n, -1)], 1))
+    seq, pos = dev(np.zeros(n, np.int32)), dev(np.arange(n, dtype=np.int32))
+    kqctx.kv_append_async(cache, None, seq, pos, kq.Heads(h[:, :K * D], K), kq.Heads(h[:, K * D:], K))
+    q = rng.standard_normal((3, 16, D)).astype(np.float16)
+    lens = dev(np.array([n], np.int32))
+    o1, o2 = dev(np.zeros_like(q)), dev(np.zeros_like(q[:1]))
+    kqctx.attn_prefill_async(kq.Attention(cache, dev(q), o1, lens, q_start=dev(np.array([0, 3], np.int32))))
+    kqctx.attn_decode_async(kq.Attention(cache, dev(q[2:]), o2, lens))
+    kqctx.synchronize()
+    want, tol = R.expect(p, q, [(i, 0, n - 3 + i, n) for i in range(3)], 0, 0)
+    close(o1.cpu().numpy(), want, tol)
+    close(o2.cpu().numpy(), want[2:], tol[2:])
+    del ck, cv, cache
+
+
+def test_two_contexts_at_once(kqctx):
+    """two contexts on two streams, their kernels in flight together"""
+    import torch
+    rng = np.random.default_rng(15)
+    D, n = 128, 700
+    work = []
+    for i in range(2):
+        ctx, stream = kq.Context(0), torch.cuda.Stream()
+        ctx.set_stream(stream.cuda_stream)
+        p = R.Paged(rng, [n, 3000], 2, 16, D)
+        q = rng.standard_normal((n + 2, 8, D)).astype(np.float16)
+        o1, o2 = dev(np.zeros_like(q)), dev(np.zeros_like(q[:2]))
+        lens = dev(np.array([n, 3000], np.int32))
+        cache = cache_of(p)
+        work.append((ctx, p, q, o1, o2, kq.Attention(cache, dev(q), o1, lens, q_start=dev(np.array([0, n, n + 2], np.int32))),
+                     kq.Attention(cache, dev(q[n:]), o2, lens), stream))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for w in work:
+            w[0].attn_prefill_async(w[5])
+            w[0].attn_decode_async(w[6])
+    for ctx, p, q, o1, o2, _, _, _ in work:
+        ctx.synchronize()
+        rows = [(0, 0, 0, n), (350, 0, 350, n), (n - 1, 0, n - 1, n), (n, 1, 2998, 3000), (n + 1, 1, 2999, 3000)]
+        want, tol = R.expect(p, q, rows, 0, 0)
+        close(o1.cpu().numpy()[[r[0] for r in rows]], want, tol)
+        want, tol = R.expect(p, q, [(n, 0, n - 1, n), (n + 1, 1, 2999, 3000)], 0, 0)
+        close(o2.cpu().numpy(), want, tol)
+        ctx.close()
