@@ -41,6 +41,7 @@ constexpr int kSortTiles = 512;
 // A join costs about as much as this many blocks: whole items unless the longest is that much
 // longer than an even share.
 constexpr int kJoinBlocks = 8;
+constexpr int kJoinAhead = 3;  // parts whose values a join has on their way at once
 
 template <int D>
 struct Cfg {
@@ -266,6 +267,7 @@ struct Shared {
     unsigned long long pv_done, tail, join, never, seg_full[kSegs], seg_empty[kSegs];
     Segment seg[kSegs];
     uint32_t tmem;
+    uint32_t odd[8];  // rows of each softmax warp to be mended after a join
     int abort, last, mending;  // mending: warps that compute rows key by key, which may take long
     Plan plan;
 };
@@ -277,6 +279,7 @@ constexpr size_t kSmem = 226 * 1024;  // dynamic
 struct PlanScratch {
     long long red[kThreads / 32];
     int red_max[kThreads / 32];
+    float red_split[kThreads / 32];
     int nbs[1];  // blocks of every row tile
 };
 
@@ -352,6 +355,7 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
     const int chunk = (tiles + kThreads - 1) / kThreads, i0 = tid * chunk;
     long long sum = 0;
     int most = 0;
+    float split = 0.0f;
     for (int i = i0; i < i0 + chunk && i < tiles; ++i) {
         Segment s;
         const int seq = seq_of_tile(seq_tiles, S, i);
@@ -359,6 +363,8 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         nbs[i] = s.nb;
         sum += s.nb;
         most = max(most, s.nb);
+        // an item's blocks times what joining a part of it costs, in blocks: its rows' bytes and a latency
+        split = fmaxf(split, s.nb * (s.n_tok * p.group * (D / 54000.0f) + 0.17f));
     }
     long long run = sum;
 #pragma unroll
@@ -366,15 +372,20 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         const long long o = __shfl_up_sync(0xffffffffu, run, d);
         if (lane >= d) run += o;
         most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+        split = fmaxf(split, __shfl_xor_sync(0xffffffffu, split, d));
     }
     if (lane == 31) scratch.red[warp] = run;
-    if (lane == 0) scratch.red_max[warp] = most;
+    if (lane == 0) {
+        scratch.red_max[warp] = most;
+        scratch.red_split[warp] = split;
+    }
     __syncthreads();
     long long before = run - sum, total = 0;
     for (int w = 0; w < kThreads / 32; ++w) {
         if (w < warp) before += scratch.red[w];
         total += scratch.red[w];
         most = max(most, scratch.red_max[w]);
+        split = fmaxf(split, scratch.red_split[w]);
     }
     total *= heads;
     // Whole items in snake order, unless the fullest CTA would get more than an even share and a join.
@@ -409,7 +420,10 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         pl.c0 = pl.c1 = 0;
         pl.start_tile = 0;
         pl.start_begin = 0;
-        const int parts = (int)min((long long)G, total);
+        // Split: shares of x blocks take x and joining an item of n blocks (n / x) c blocks' time, least at
+        // x = sqrt(n c); more CTAs than that would spend longer joining than they save.
+        const float x = fmaxf(sqrtf(split), 1.0f);
+        const int parts = (int)fmaxf(fminf((float)G, (float)total / x), 1.0f);
         if (!whole) {
             pl.shares = parts == G ? even : Shares(total, parts);
             if ((int)blockIdx.x < parts) {
@@ -797,7 +811,8 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                     tmem_ld32(o_base + 32 * c, o);
                     wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) part[(8 * c + e) * part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    for (int e = 0; e < 8; ++e)
+                        if (mine) part[(8 * c + e) * part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
                 reinterpret_cast<float2 *>(part - (t * 128 + r) + D / 4 * part_rows)[t * 128 + r] = make_float2(bad ? NAN : m, l);  // NaN: a page is missing
             }
@@ -816,58 +831,74 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
             const bool join = sh.last != 0;
             if (!together()) return;
             if (join && active) {
+                // A tile of 32 or 64 rows gives its other warps shares of the values.
+                const int rows = min(s.n_tok - t * p.tpt, p.tpt) * p.group;
+                const int span_warps = rows <= 32 ? 1 : rows <= 64 ? 2 : 4, shares = 4 / span_warps;
+                const int jr = (warp & (span_warps - 1)) * 32 + lane;  // this thread's row of the tile
+                const bool on = jr < rows;
+                const int jtok = t * p.tpt + jr / p.group, jhead = s.head * p.group + jr % p.group;
+                uint16_t *jout = a.out + (long long)(s.row0 + jtok) * a.out_stride + jhead * D;
                 auto part_at = [&](int c) {
                     return reinterpret_cast<const float4 *>(a.parts + (size_t)(2 * c + (c == first)) * part_rows * (D + 2));
                 };
-                auto stat_at = [&](int c) { return __ldcg(reinterpret_cast<const float2 *>(part_at(c) + D / 4 * part_rows) + t * 128 + r); };
+                auto stat_at = [&](int c) { return __ldcg(reinterpret_cast<const float2 *>(part_at(c) + D / 4 * part_rows) + t * 128 + jr); };
                 float M = -INFINITY, L = 0.0f;
                 bool missing = false;
-#pragma unroll 4
-                for (int c = first; c <= last; ++c) {
-                    const float2 ml = stat_at(c);
-                    missing |= ml.x != ml.x;
-                    const float top = fmaxf(M, ml.x);
-                    // a part without a score above -inf adds nothing; NaN (a NaN score) stays
-                    L = L * (M == -INFINITY ? 1.0f : exp2_fast(M - top)) +
-                        (ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.0f) : exp2_fast(ml.x - top) * ml.y);
-                    M = top;
-                }
-                const float inv = 1.0f / L;
                 float2 odd = make_float2(0.0f, 0.0f);
-                // 32 values of each part in turn, the next ones on their way meanwhile
-                const int n = last - first + 1;
-                float4 ahead[8];
-                auto fetch = [&](int c0, int i) {
-                    const float4 *part = part_at(first + i) + c0 / 4 * part_rows + t * 128 + r;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) ahead[e] = __ldcg(part + e * part_rows);
-                };
-                fetch(0, 0);
-#pragma unroll 1
-                for (int c0 = 0; c0 < D; c0 += 32) {
-                    float o[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-#pragma unroll 1
-                    for (int i = 0; i < n; ++i) {
-                        float4 v[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = ahead[e];
-                        const float mc = stat_at(first + i).x;
-                        if (i + 1 < n) fetch(c0, i + 1);
-                        else if (c0 + 32 < D) fetch(c0 + 32, 0);
-                        const float w = mc == -INFINITY ? 0.0f : exp2_fast(mc - M);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            o[4 * e] += w * v[e].x;
-                            o[4 * e + 1] += w * v[e].y;
-                            o[4 * e + 2] += w * v[e].z;
-                            o[4 * e + 3] += w * v[e].w;
-                        }
+                if (on) {
+#pragma unroll 8
+                    for (int c = first; c <= last; ++c) {
+                        const float2 ml = stat_at(c);
+                        missing |= ml.x != ml.x;
+                        const float top = fmaxf(M, ml.x);
+                        // a part without a score above -inf adds nothing; NaN (a NaN score) stays
+                        L = L * (M == -INFINITY ? 1.0f : exp2_fast(M - top)) +
+                            (ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.0f) : exp2_fast(ml.x - top) * ml.y);
+                        M = top;
                     }
-                    put32(o, inv, out + c0, mine, p.wide, odd);
+                    const float inv = 1.0f / L;
+                    for (int c0 = 32 * ((warp & 3) / span_warps); c0 < D; c0 += 32 * shares) {
+                        float o[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+#pragma unroll 1
+                        for (int c = first; c <= last; c += kJoinAhead) {
+                            float4 v[kJoinAhead][8];
+                            float w[kJoinAhead];
+#pragma unroll
+                            for (int i = 0; i < kJoinAhead; ++i) {
+                                const int cc = min(c + i, last);
+                                const float4 *part = part_at(cc) + c0 / 4 * part_rows + t * 128 + jr;
+                                w[i] = stat_at(cc).x;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) v[i][e] = __ldcg(part + e * part_rows);
+                            }
+#pragma unroll
+                            for (int i = 0; i < kJoinAhead; ++i) {
+                                if (c + i > last) break;
+                                w[i] = w[i] == -INFINITY ? 0.0f : exp2_fast(w[i] - M);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    o[4 * e] += w[i] * v[i][e].x;
+                                    o[4 * e + 1] += w[i] * v[i][e].y;
+                                    o[4 * e + 2] += w[i] * v[i][e].z;
+                                    o[4 * e + 3] += w[i] * v[i][e].w;
+                                }
+                            }
+                        }
+                        put32(o, inv, jout + c0, true, p.wide, odd);
+                    }
                 }
-                mend_rows<D>(p, sh, s, mine && (missing || M == -INFINITY || (L == L && !(odd.x + odd.y == 0.0f))), tok, head, lane);
+                __syncwarp();
+                const uint32_t wrong = __ballot_sync(0xffffffffu, on && (missing || M == -INFINITY || (L == L && !(odd.x + odd.y == 0.0f))));
+                if (lane == 0 && wrong) atomicOr(&sh.odd[t * 4 + (warp & (span_warps - 1))], wrong);
+            }
+            if (join) {
+                if (!together()) return;  // all values are written
+                const uint32_t wrong = sh.odd[warp];
+                __syncwarp();
+                if (lane == 0) sh.odd[warp] = 0;  // (every warp has read its own before the next join's first meeting)
+                mend_rows<D>(p, sh, s, wrong >> lane & 1, tok, head, lane);
             }
         }
         __syncwarp();
@@ -920,6 +951,7 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
         mbar_init_fence();
         sh.abort = 0;
         sh.mending = 0;
+        for (int i = 0; i < 8; ++i) sh.odd[i] = 0;
     }
     if (warp == kWarpMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)));
