@@ -297,7 +297,12 @@ int kq_kv_append_async(kq_ctx *ctx, const kq_kv_cache *cache, const kq_rope *rop
  * key j when 0 <= j <= p and, with a window, j > p - window or j < sinks (the first tokens stay
  * visible).  A row that sees no key gets zeros.  Keys that a row does not see have no effect on it,
  * whatever they hold.  Lengths past the table's reach count as its reach, negative ones as 0, and
- * the next kq_synchronize reports KQ_ERR_SHAPE. */
+ * the next kq_synchronize reports KQ_ERR_SHAPE.
+ *
+ * The first call of a context allocates its scratch (about 40 MB, one size for all shapes), so make
+ * one before capturing.  A graph holds on to the addresses it was captured with, and the work of one
+ * context shares its scratch: let no two of its calls or graphs run at the same time on different
+ * streams.  After KQ_ERR_TIMEOUT make an eager call before a graph is replayed. */
 typedef struct kq_attn {
     const uint16_t *q;          /* rows of heads * head_dim, after norm and rotation */
     size_t q_stride;

@@ -750,3 +750,70 @@ def test_two_contexts_at_once(kqctx):
         want, tol = R.expect(p, q, [(n, 0, n - 1, n), (n + 1, 1, 2999, 3000)], 0, 0)
         close(o2.cpu().numpy(), want, tol)
         ctx.close()
+
+
+def test_rows_at_any_16_bytes(kqctx):
+    """q and out as views that begin 16 bytes into their rows, rows a multiple of 8 values apart"""
+    import torch
+    rng = np.random.default_rng(16)
+    for D, H, K in ((64, 6, 2), (128, 4, 4), (256, 3, 1)):
+        lens = [70, 33]
+        p = R.Paged(rng, lens, K, 16, D)
+        q = rng.standard_normal((40, H, D)).astype(np.float16)
+        width = H * D + 24
+        qb, ob = (torch.full((40, width), SENTINEL, dtype=torch.float16, device="cuda") for _ in range(2))
+        qv, ov = qb[:, 8:8 + H * D], ob[:, 16:16 + H * D]
+        qv.copy_(dev(q.reshape(40, -1)))
+        n = dev(np.array(lens, np.int32))
+        a = kq.Attention(cache_of(p), qv, ov, n, q_start=dev(np.array([0, 30, 40], np.int32)), heads=H)
+        kqctx.attn_prefill_async(a)
+        kqctx.synchronize()
+        want, tol = R.expect(p, q, [(i, 0, 40 + i, 70) for i in range(30)] + [(30 + i, 1, 23 + i, 33) for i in range(10)], 0, 0)
+        close(ov.cpu().numpy().reshape(40, H, D), want, tol)
+        kqctx.attn_decode_async(kq.Attention(a.cache, qv[:2], ov[:2], n, heads=H))
+        kqctx.synchronize()
+        want, tol = R.expect(p, q, [(0, 0, 69, 70), (1, 1, 32, 33)], 0, 0)
+        close(ov[:2].cpu().numpy().reshape(2, H, D), want, tol)
+        assert (ob[:, :16] == SENTINEL).all() and (ob[:, 16 + H * D:] == SENTINEL).all()
+
+
+def test_prefill_in_a_graph(kqctx):
+    """a captured prompt call replayed with other row ranges and lengths: whole items, then items that are split"""
+    import torch
+    rng = np.random.default_rng(17)
+    D, H, K, M, stride = 128, 4, 2, 200, 300
+    ctx, stream = kq.Context(0), torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    try:
+        lens = [4600, 500]
+        p = R.Paged(rng, lens, K, 16, D, stride=stride)
+        q = rng.standard_normal((M, H, D)).astype(np.float16)
+        out = dev(np.zeros_like(q))
+        start, n = dev(np.zeros(3, np.int32)), dev(np.zeros(2, np.int32))
+        a = kq.Attention(cache_of(p), dev(q), out, n, q_start=start)
+        torch.cuda.synchronize()
+        ctx.attn_prefill_async(a)                                  # sizes the scratch: nothing to do yet
+        ctx.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            ctx.attn_prefill_async(a)
+        for s, b in (([0, 100, 200], [100, 300]), ([0, 7, 9], [4600, 500]), ([0, 0, 150], [0, 500]), ([5, 60, 60], [4100, 0])):
+            out.fill_(SENTINEL)
+            start.copy_(dev(np.array(s, np.int32)))
+            n.copy_(dev(np.array(b, np.int32)))
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                g.replay()
+                g.replay()
+            ctx.synchronize()
+            rows = [(s[i] + j, i, b[i] - (s[i + 1] - s[i]) + j, b[i]) for i in range(2) for j in range(s[i + 1] - s[i])]
+            got = out.cpu().numpy()
+            rest = np.setdiff1d(np.arange(M), [r[0] for r in rows])
+            assert (got[rest] == SENTINEL).all()
+            pick = rows[:: max(1, len(rows) // 20)]
+            want, tol = R.expect(p, q, pick, 0, 0)
+            close(got[[r[0] for r in pick]], want, tol, (s, b))
+        del g
+    finally:
+        torch.cuda.synchronize()
+        ctx.close()
