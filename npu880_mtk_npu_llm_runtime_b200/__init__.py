@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 import numpy as np
 
@@ -238,10 +239,10 @@ def _rows(t, what: str, heads: int):
     return t.data_ptr(), stride, width // heads, t.shape[0]
 
 
-def _ints(t, what: str, n: int | None = None):
-    import torch
-    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() != n):
-        raise ValueError(f"{what}: a contiguous int32 CUDA tensor" + ("" if n is None else f" of {n}") + " is needed")
+def _ints(t, what: str, device: int, n: int | None = None):
+    """pointer of a contiguous int32 tensor of n values on CUDA device `device`"""
+    if t.dtype is not sys.modules["torch"].int32 or not t.is_contiguous() or t.get_device() != device or (n is not None and t.numel() != n):
+        raise ValueError(f"{what}: a contiguous int32 tensor" + ("" if n is None else f" of {n}") + f" on CUDA device {device} is needed")
     return t.data_ptr()
 
 
@@ -275,11 +276,12 @@ class KvCache:
                 raise ValueError(f"{what}: a contiguous fp16 CUDA tensor [pages, kv_heads, page_size, head_dim] is needed")
         if k.shape != v.shape or k.device != v.device or page_table.dim() != 2 or page_table.device != k.device:
             raise ValueError("k and v must have one shape, and the table two dimensions, on one device")
-        self.k, self.v, self.page_table, self.device = k, v, page_table, k.device
+        self.k, self.v, self.page_table, self.device, self.index = k, v, page_table, k.device, k.get_device()
         s = self.struct = KvCacheStruct()
-        s.k, s.v, s.page_table = k.data_ptr(), v.data_ptr(), _ints(page_table, "page_table")
+        s.k, s.v, s.page_table = k.data_ptr(), v.data_ptr(), _ints(page_table, "page_table", self.index)
         s.n_pages, s.kv_heads, s.page_size, s.head_dim = k.shape
         s.n_seqs, s.table_stride = page_table.shape
+        self.head_dim = s.head_dim
         self.ref = C.addressof(s)
 
 
@@ -302,7 +304,7 @@ class Heads:
         for t in (out, gamma):
             if t is not None and t.device != x.device:
                 raise ValueError("rows, out and gamma must be on one device")
-        self.device, self.keep, self.ref = x.device, (x, out, gamma), C.addressof(s)
+        self.index, self.keep, self.ref = x.get_device(), (x, out, gamma), C.addressof(s)
 
 
 class Attention:
@@ -319,12 +321,11 @@ class Attention:
         if (qd, od, om) != (dim, dim, s.M):
             raise ValueError(f"q and out must have the same rows of {heads} heads of {dim}")
         s.heads, s.window, s.sinks, s.scale = heads, window, sinks, scale
-        s.kv_len = _ints(kv_len, "kv_len", cache.struct.n_seqs)
+        s.kv_len = _ints(kv_len, "kv_len", cache.index, cache.struct.n_seqs)
         if q_start is not None:
-            s.q_start = _ints(q_start, "q_start", cache.struct.n_seqs + 1)
-        for t in (q, out, kv_len, q_start):
-            if t is not None and t.device != cache.device:
-                raise ValueError("q, out, kv_len and q_start must be on the cache's device")
+            s.q_start = _ints(q_start, "q_start", cache.index, cache.struct.n_seqs + 1)
+        if q.device != cache.device or out.device != cache.device:
+            raise ValueError("q and out must be on the cache's device")
         self.cache, self.keep, self.ref = cache, (q, out, kv_len, q_start), C.addressof(s)
 
 
@@ -573,8 +574,8 @@ class Context:
     # ---- attention over a paged cache (kq_rope, kq_kv_cache, kq_heads, kq_attn)
     def _here(self, *objects):
         for o in objects:
-            if o is not None and o.device.index != self.device:
-                raise ValueError(f"a tensor lives on {o.device}, the context on device {self.device}")
+            if o is not None and o.index != self.device:
+                raise ValueError(f"tensors on CUDA device {o.index}, the context on device {self.device}")
 
     def qk_norm_rope_async(self, rope: Rope | None, pos, q: Heads | None, k: Heads | None = None, eps: float = 1e-6):
         """per-head norm and rotation of q and k rows into their `out` in one launch"""
@@ -583,21 +584,22 @@ class Context:
             raise ValueError("q or k rows are needed")
         if q is not None and k is not None and (q.rows, q.head_dim) != (k.rows, k.head_dim):
             raise ValueError("q and k must have the same rows and head size")
-        self._here(q, k, pos)
-        p = None if pos is None else _ints(pos, "positions", h.rows)
+        self._here(q, k)
+        p = None if pos is None else _ints(pos, "positions", self.device, h.rows)
         self.check(self.L.kq_qk_norm_rope_async(self.handle, rope and rope.ref, h.head_dim, h.rows, p, q and q.ref,
                                                 k and k.ref, eps))
 
     def kv_append_async(self, cache: KvCache, rope: Rope | None, seq, pos, k: Heads, v: Heads, q: Heads | None = None,
                         eps: float = 1e-6):
         """row i's key (normed, rotated) and value to position pos[i] of sequence seq[i]; q into its `out`"""
+        rows, dim = k.rows, cache.head_dim
         for h in (k, v, q):
-            if h is not None and (h.rows, h.head_dim) != (k.rows, cache.struct.head_dim):
+            if h is not None and (h.rows != rows or h.head_dim != dim):
                 raise ValueError("q, k and v must have the same rows and the cache's head size")
-        self._here(cache, k, v, q, seq, pos)
-        self.check(self.L.kq_kv_append_async(self.handle, cache.ref, rope and rope.ref, k.rows,
-                                             _ints(seq, "sequences", k.rows), _ints(pos, "positions", k.rows),
-                                             q and q.ref, k.ref, v.ref, eps))
+        self._here(cache, k, v, q)
+        self.check(self.L.kq_kv_append_async(self.handle, cache.ref, rope and rope.ref, rows,
+                                             _ints(seq, "sequences", self.device, rows),
+                                             _ints(pos, "positions", self.device, rows), q and q.ref, k.ref, v.ref, eps))
 
     def attn_decode_async(self, a: Attention):
         """attention of one new token per sequence"""
@@ -615,12 +617,14 @@ class Context:
         for t in (x_dev, out_dev):
             if tuple(t.shape) != (M, layer.hidden) or t.element_size() != 2 or not t.is_contiguous():
                 raise ValueError(f"x and out: contiguous 16-bit tensors [rows, {layer.hidden}] are needed")
-        for t in (x_dev, out_dev, seq, pos, kv_len, q_start, layer.cache.k):
-            if t is not None and t.device.index != self.device:
-                raise ValueError(f"a tensor lives on {t.device}, the context on device {self.device}")
+            if t.get_device() != self.device:
+                raise ValueError(f"x and out must be on CUDA device {self.device}")
+        self._here(layer.cache)
+        dev = self.device
         self.check(self.L.kq_run_attn_async(
-            self.handle, layer.ref, M, _ints(seq, "sequences", M), _ints(pos, "positions", M), _ints(kv_len, "kv_len", n_seqs),
-            None if q_start is None else _ints(q_start, "q_start", n_seqs + 1), _dp(x_dev), _dp(out_dev)))
+            self.handle, layer.ref, M, _ints(seq, "sequences", dev, M), _ints(pos, "positions", dev, M),
+            _ints(kv_len, "kv_len", dev, n_seqs), None if q_start is None else _ints(q_start, "q_start", dev, n_seqs + 1),
+            _dp(x_dev), _dp(out_dev)))
 
     # ---- several GPUs: the gather in the LM head GEMV (kq_peer_*, kq_gemm_peer_gather_async)
     def peer_region_bytes(self, M: int, row_stride: int) -> int:
