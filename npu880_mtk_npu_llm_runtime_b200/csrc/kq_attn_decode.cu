@@ -19,7 +19,11 @@
 //   k slot stands for which dimension is free as long as Q's B fragment uses the same order;
 //   O^T = V^T P^T: lane (g, t) loads dimensions 8g.. of keys 2t, 2t+1, 2t+8, 2t+9 and pairs the
 //   keys of a dimension with byte permutes; P^T's fragment is S^T's transposed by movmatrix.
-// tcgen05 has nothing to add here: the tensor pipe idles either way while the bytes come in.
+// tcgen05 has nothing to add here: the tensor pipe (8.7% busy) idles either way while the bytes come in.
+//
+// 4 sequences x 131,072 keys, 8 key heads of 128 (2.15 GB): 331 us, 6.5 TB/s, 0.99 of a measured copy;
+// 64 sequences of 1..8,192 keys (239 MB): 49 us, of which 38 stream; 1 x 1,000 keys: 10 us, six dependent
+// memory latencies and the launch.  16 x 8,192 keys read 1.0004 x their bytes from DRAM.
 #include "kq_attn_dev.cuh"
 
 #include <mutex>

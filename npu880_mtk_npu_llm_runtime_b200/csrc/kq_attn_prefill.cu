@@ -2,7 +2,7 @@
 // tensor cores (tcgen05.mma kind::f16, accumulators in TMEM).
 //
 // out = sum_j w_j v_j / sum_j w_j,  w_j = 2^(x_j - m),  x_j = scale log2(e) q.k_j: one pass over
-// the keys with a running maximum.  m may lag behind the true maximum by up to 2^kLag (any m gives
+// the keys with a running maximum.  m may lag behind the true maximum by up to kLag (any m gives
 // the same quotient), so the accumulated rows are rescaled only when it falls further behind.
 //
 // Rows: the query heads that share a key head are packed side by side, row = token * G + head, so a
@@ -23,7 +23,12 @@
 // Work: an item is a row tile of one key head, a unit one of its key blocks.  Items go whole to
 // the CTAs, longest first in snake order, when that balances; else (few items, long caches) every
 // CTA takes an equal range of units, and the parts of an item that several CTAs share are joined
-// in order by the last of them.
+// in order by the last of them, no finer than the joins pay for (make_plan).
+//
+// 512 rows behind 32,256 keys, 32 / 8 heads of 128: 283 us, 970 TFLOP/s, at the power cap (1.47 GHz); tensor
+// pipe and exponential unit 60% busy.  A 2,048-token prompt: 45 us, of which 4 pass before the first
+// block and 2.5 in each item's epilogue; a block takes 1.75 us at 1.9 GHz, 0.6 of it MMAs that the
+// tile's own softmax waits for.
 #include "kq_attn_dev.cuh"
 
 #include <cuda.h>
