@@ -61,10 +61,11 @@ struct DecodeParams {
 };
 
 // The cache streams through: first to leave L2, so that what is used again (the kernel's code, the
-// tables, the parts) stays there.
+// tables, the parts) stays there.  (Not the read-only path: the kernel may be resident before the one
+// that appends the last rows has ended.)
 __device__ __forceinline__ uint4 load_stream(const uint16_t *p, uint64_t policy) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+    asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "l"(p), "l"(policy));
     return v;
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
         int sum = 0;
         for (int s = s0; s < s0 + chunk && s < S; ++s) {
             bool bad = false;
-            const int len = kv_length(a.cache, __ldg(a.kv_len + s), bad);
+            const int len = kv_length(a.cache, a.kv_len[s], bad);
             lens[s] = len;
             if (bad && blockIdx.x == 0) report_error(a.status, DEV_ERR_CACHE);
             const KvSpan sp = kv_span(len - 1, len, a.window, a.sinks);
@@ -260,11 +261,11 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
             l[b][0] = l[b][1] = 0.0f;
         }
         bool seen = false;
-        int next_page = __ldg(table + ((kv_block(blocks, t0) * kUnit) >> a.cache.page_shift));
+        int next_page = table[(kv_block(blocks, t0) * kUnit) >> a.cache.page_shift];
         for (int i = t0; i < t1; ++i) {
             const int j0 = kv_block(blocks, i) * kUnit;
             const int page = next_page;
-            if (i + 1 < t1) next_page = __ldg(table + ((kv_block(blocks, i + 1) * kUnit) >> a.cache.page_shift));
+            if (i + 1 < t1) next_page = table[(kv_block(blocks, i + 1) * kUnit) >> a.cache.page_shift];
             if (!kv_page_ok(a.cache, page)) {  // uniform: the unit counts as masked
                 if (lane == 0) report_error(a.status, DEV_ERR_CACHE);
                 continue;

@@ -22,7 +22,7 @@ __device__ __forceinline__ unsigned count_arrival(unsigned *count) {
 
 // The page that holds position j of sequence seq, or -1 (and an error) where the table names none.
 __device__ __forceinline__ int kv_page(const KvView &c, int seq, int j, int *status) {
-    const int page = __ldg(c.table + (long long)seq * c.table_stride + (j >> c.page_shift));
+    const int page = c.table[(long long)seq * c.table_stride + (j >> c.page_shift)];
     if (kv_page_ok(c, page)) return page;
     report_error(status, DEV_ERR_CACHE);
     return -1;

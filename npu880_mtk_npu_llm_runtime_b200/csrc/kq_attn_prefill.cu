@@ -185,9 +185,9 @@ template <int D>
 __device__ __forceinline__ void tile_of(const PrefillParams &p, int seq, int tile_in_seq, Segment &s) {
     using C = Cfg<D>;
     bool bad = false;
-    const KvRows rows = kv_rows(__ldg(p.a.q_start + seq), __ldg(p.a.q_start + seq + 1), p.a.M, bad);
+    const KvRows rows = kv_rows(p.a.q_start[seq], p.a.q_start[seq + 1], p.a.M, bad);
     s.seq = seq;
-    s.len = kv_length(p.a.cache, __ldg(p.a.kv_len + seq), bad);
+    s.len = kv_length(p.a.cache, p.a.kv_len[seq], bad);
     s.tok = tile_in_seq * C::NT * p.tpt;
     s.n_tok = min(C::NT * p.tpt, rows.n - s.tok);
     s.row0 = rows.begin + s.tok;
@@ -336,8 +336,8 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         int sum = 0;
         for (int s = s0; s < s0 + chunk && s < S; ++s) {
             bool bad = false;
-            const KvRows r = kv_rows(__ldg(p.a.q_start + s), __ldg(p.a.q_start + s + 1), p.a.M, bad);
-            kv_length(p.a.cache, __ldg(p.a.kv_len + s), bad);
+            const KvRows r = kv_rows(p.a.q_start[s], p.a.q_start[s + 1], p.a.M, bad);
+            kv_length(p.a.cache, p.a.kv_len[s], bad);
             if (bad && blockIdx.x == 0) report_error(p.a.status, DEV_ERR_CACHE);
             seq_tiles[s] = sum;
             sum += (r.n + per - 1) / per;
@@ -490,7 +490,7 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
         auto page_of = [&](int i) {
             const int j = kv_block(s.blocks, i) * BN + sub * p.box_rows;
             if (lane >= boxes || i >= s.b1 || !tile_sees(s, j, p.box_rows)) return a.cache.n_pages;
-            const int q = __ldg(table + (j >> a.cache.page_shift));
+            const int q = table[j >> a.cache.page_shift];
             if (kv_page_ok(a.cache, q)) return q;
             if (!V) *reinterpret_cast<volatile int *>(&rec.bad) = 1;
             return a.cache.n_pages;

@@ -86,13 +86,13 @@ __global__ __launch_bounds__(kThreads, kCtasPerSm) void kq_norm_rope(const __gri
     load(n0, ahead);
 
     int pos = 0, page = 0;
-    if (p.pos) pos = __ldg(p.pos + row);
+    if (p.pos) pos = p.pos[row];
     if (p.cache.table) {
-        const int seq = __ldg(p.seq + row);
+        const int seq = p.seq[row];
         if (seq < 0) return;  // padding
         bool ok = seq < p.cache.n_seqs && pos >= 0 && pos < kv_reach(p.cache);
         if (ok) {
-            page = __ldg(p.cache.table + (long long)seq * p.cache.table_stride + (pos >> p.cache.page_shift));
+            page = p.cache.table[(long long)seq * p.cache.table_stride + (pos >> p.cache.page_shift)];
             ok = kv_page_ok(p.cache, page);
         }
         if (!ok) {
