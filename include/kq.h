@@ -342,11 +342,12 @@ typedef struct kq_attn_layer {
 } kq_attn_layer;
 /* M rows of x_in / x_out (fp16 [M][hidden]); seq_dev and pos_dev as in kq_kv_append_async, kv_len_dev
  * and q_start_dev as in kq_attn (kv_len counts the appended rows; without q_start row i is sequence i,
- * so seq_dev[i] is i, or -1 for padding).  x_out may not overlap x_in.  A row of no sequence comes out
- * as it went in.  One eager call at the largest M sizes the scratch; then a call allocates nothing and
- * can be captured into a CUDA graph, which keeps reading x_in, the tables and the lengths where they
- * were.  As for every call of this library, the work of one context (its graphs included) shares
- * that context's scratch: let no two run at the same time on different streams. */
+ * so seq_dev[i] is i, or -1 with kv_len_dev[i] = 0 for padding).  x_out may not overlap x_in.  A row of no
+ * sequence (such padding, or a row outside the q_start ranges) comes out as it went in.  One eager call
+ * at the largest M sizes the scratch; then a call allocates nothing and can be captured into a CUDA
+ * graph, which keeps reading x_in, the tables and the lengths where they were.  As for every call of
+ * this library, the work of one context (its graphs included) shares that context's scratch: let no two
+ * run at the same time on different streams. */
 int kq_run_attn_async(kq_ctx *ctx, const kq_attn_layer *layer, int M, const int32_t *seq_dev, const int32_t *pos_dev,
                       const int32_t *kv_len_dev, const int32_t *q_start_dev, const uint16_t *x_in_dev,
                       uint16_t *x_out_dev);

@@ -363,8 +363,8 @@ class AttnLayer:
                                           q_gamma=_dp(q_gamma), k_gamma=_dp(k_gamma), rope=rope and rope.ref,
                                           cache=cache.ref, heads=q.rows // dim, window=window, sinks=sinks, scale=scale,
                                           eps=eps)
-        self.cache, self.hidden, self.ref = cache, q.cols, C.addressof(s)
-        self.keep = (q, k, v, o, gamma, q_gamma, k_gamma, rope)
+        self.cache, self.hidden, self.ref, self.weights = cache, q.cols, C.addressof(s), (q, k, v, o)
+        self.keep = (gamma, q_gamma, k_gamma, rope)
 
 
 class Context:
@@ -611,12 +611,16 @@ class Context:
         self._here(a.cache)
         self.check(self.L.kq_attn_prefill_async(self.handle, a.cache.ref, a.ref))
 
+    HALVES = ("torch.float16", "torch.int16", "torch.uint16")  # fp16, or its bits
+
     def run_attn_async(self, layer: AttnLayer, seq, pos, kv_len, x_dev, out_dev, q_start=None):
         """x + W_o . attention over the rows' keys and the cache (decode: one row per sequence; with q_start, prefill)"""
         n_seqs, M = layer.cache.struct.n_seqs, x_dev.shape[0]
+        if not all(w.handle for w in layer.weights):
+            raise ValueError("a weight of the layer was freed")
         for t in (x_dev, out_dev):
-            if tuple(t.shape) != (M, layer.hidden) or t.element_size() != 2 or not t.is_contiguous():
-                raise ValueError(f"x and out: contiguous 16-bit tensors [rows, {layer.hidden}] are needed")
+            if tuple(t.shape) != (M, layer.hidden) or str(t.dtype) not in self.HALVES or not t.is_contiguous():
+                raise ValueError(f"x and out: contiguous fp16 tensors [rows, {layer.hidden}] are needed")
             if t.get_device() != self.device:
                 raise ValueError(f"x and out must be on CUDA device {self.device}")
         self._here(layer.cache)

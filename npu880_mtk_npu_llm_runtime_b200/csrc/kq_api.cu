@@ -1156,8 +1156,13 @@ int attn_scratch(kq_ctx *c, kq::AttnLaunch &L) {
                                                             kq::attn_prefill_part_bytes(c->num_sms)))) return r;
     const bool clear = !c->attn_count.p || c->attn_dirty;
     if (int r = ensure(c, c->attn_count, sizeof(unsigned) * (size_t)c->num_sms)) return r;
-    if (clear) KQ_CUDA(c, cudaMemsetAsync(c->attn_count.p, 0, c->attn_count.cap, c->stream));
-    c->attn_dirty = false;
+    if (clear) {
+        KQ_CUDA(c, cudaMemsetAsync(c->attn_count.p, 0, c->attn_count.cap, c->stream));
+        // a capture has only recorded it: the counts stay as they are until the graph runs
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        KQ_CUDA(c, cudaStreamIsCapturing(c->stream, &cap));
+        c->attn_dirty = cap != cudaStreamCaptureStatusNone;
+    }
     L.parts = static_cast<float *>(c->attn_parts.p);
     L.count = static_cast<unsigned *>(c->attn_count.p);
     return KQ_OK;
@@ -1200,7 +1205,8 @@ extern "C" int kq_qk_norm_rope_async(kq_ctx *c, const kq_rope *rope, int head_di
     for (const kq_heads *h : {q, k})
         if (!r && h && M > 0) r = kq::check_heads(h, head_dim, 1, &why);
     if (r) return fail(c, r, "%s", why);
-    if (rope && rope->rot_dim > 0 && !pos) return fail(c, KQ_ERR_INVALID_ARGUMENT, "positions are NULL");
+    if ((rope && rope->rot_dim > 0 && !pos) || !kq::kv_aligned(pos, 4))
+        return fail(c, KQ_ERR_INVALID_ARGUMENT, "positions are NULL or not 4-byte aligned");
     if (!(eps >= 0.0f)) return fail(c, KQ_ERR_INVALID_ARGUMENT, "eps must not be negative");
     if (M == 0 || (!q && !k)) return KQ_OK;
     const OnDevice on(c->device);
@@ -1284,6 +1290,8 @@ extern "C" int kq_run_attn_async(kq_ctx *c, const kq_attn_layer *l, int M, const
                     l->cache->kv_heads, D);
     if (int r = validate_mk(c, M, hidden)) return r;
     if (int r = validate_mk(c, M, qd)) return r;
+    const uintptr_t xi = (uintptr_t)x_in, xo = (uintptr_t)x_out, xb = (uintptr_t)M * hidden * 2;
+    if (xi < xo + xb && xo < xi + xb) return fail(c, KQ_ERR_INVALID_ARGUMENT, "x_out may not overlap x_in");
     const OnDevice on(c->device);
     // scratch: xn [M][hidden] | q, k, v rows side by side | attention's output | q8k(xn) | q8_0(xn)
     auto al = [](size_t v) { return (v + 255) & ~(size_t)255; };

@@ -247,8 +247,8 @@ inline int check_append(const kq_kv_cache *c, const kq_rope *rope, int M, const 
         *why = "k and v must have the cache's kv_heads";
         return KQ_ERR_SHAPE;
     }
-    if (!seq || !pos) {
-        *why = "sequences or positions are NULL";
+    if (!seq || !pos || !kv_aligned(seq, 4) || !kv_aligned(pos, 4)) {
+        *why = "sequences or positions are NULL or not 4-byte aligned";
         return KQ_ERR_INVALID_ARGUMENT;
     }
     return KQ_OK;
@@ -256,8 +256,8 @@ inline int check_append(const kq_kv_cache *c, const kq_rope *rope, int M, const 
 
 inline int check_attn(const kq_kv_cache *c, const kq_attn *a, bool prefill, const char **why) {
     if (int r = check_cache(c, why)) return r;
-    if (!a || !a->kv_len || (prefill && !a->q_start)) {
-        *why = "the attention's description or its lengths are NULL";
+    if (!a || !a->kv_len || (prefill && !a->q_start) || !kv_aligned(a->kv_len, 4) || (prefill && !kv_aligned(a->q_start, 4))) {
+        *why = "the attention's description or its lengths are NULL or not 4-byte aligned";
         return KQ_ERR_INVALID_ARGUMENT;
     }
     if (int r = check_rows(a->M, why)) return r;
@@ -268,6 +268,10 @@ inline int check_attn(const kq_kv_cache *c, const kq_attn *a, bool prefill, cons
     if (a->M == 0) return KQ_OK;  // nothing to do: the rows may be NULL
     if (int r = check_head_rows(a->q, a->q_stride, a->heads, c->head_dim, why)) return r;
     if (int r = check_head_rows(a->out, a->out_stride, a->heads, c->head_dim, why)) return r;
+    if (a->q == a->out) {
+        *why = "out may not overlap q";
+        return KQ_ERR_INVALID_ARGUMENT;
+    }
     if (a->heads % c->kv_heads || a->heads / c->kv_heads > KQ_MAX_GROUP) {
         *why = "heads must be a multiple of kv_heads, at most KQ_MAX_GROUP times it";
         return KQ_ERR_SHAPE;

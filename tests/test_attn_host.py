@@ -177,7 +177,7 @@ def test_null_structs(host):
     (dict(out_stride=8), INVALID, INVALID), (dict(q=8), INVALID, INVALID), (dict(out=520), INVALID, INVALID), (dict(window=-1), INVALID, INVALID),
     (dict(sinks=4), INVALID, INVALID), (dict(window=8, sinks=-1), INVALID, INVALID), (dict(window=8, sinks=4), 0, 0),
     (dict(scale=-1.0), INVALID, INVALID), (dict(scale=float("nan")), INVALID, INVALID), (dict(scale=float("inf")), INVALID, INVALID),
-    (dict(scale=0.125), 0, 0),
+    (dict(scale=0.125), 0, 0), (dict(kv_len=66), INVALID, INVALID), (dict(q_start=65), 0, INVALID), (dict(out=256), INVALID, INVALID),
 ])
 def test_attention_refusals(host, change, decode, prefill):
     c, a = cache_struct(), attn_struct(**change)
@@ -187,6 +187,7 @@ def test_attention_refusals(host, change, decode, prefill):
 
 @pytest.mark.parametrize("change, status", [
     (dict(), 0), (dict(M=-1), SHAPE), (dict(M=4097), SHAPE), (dict(M=0), 0), (dict(seq=None), INVALID), (dict(pos=None), INVALID),
+    (dict(seq=66), INVALID), (dict(pos=65), INVALID),
     (dict(k=heads_struct(3)), SHAPE), (dict(v=heads_struct(1)), SHAPE), (dict(k=heads_struct(out=512, out_stride=512)), INVALID),
     (dict(v=heads_struct(gamma=64)), INVALID), (dict(k=heads_struct(gamma=64)), 0), (dict(k=heads_struct(gamma=72)), INVALID),
     (dict(k=heads_struct(in_=None)), INVALID), (dict(k=heads_struct(in_=260)), INVALID), (dict(k=heads_struct(in_stride=120)), INVALID),

@@ -817,3 +817,42 @@ def test_prefill_in_a_graph(kqctx):
     finally:
         torch.cuda.synchronize()
         ctx.close()
+
+
+def test_capture_between_a_timeout_and_the_next_call(kqctx):
+    """a graph captured after a call that stopped early has only recorded the clearing of the arrival counts: an
+    eager call before its first replay clears them itself, and the replay is right too"""
+    import torch
+    rng = np.random.default_rng(18)
+    D, H, K, n, new = 128, 8, 2, 6000, 20
+    ctx, stream = kq.Context(0), torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    try:
+        p = R.Paged(rng, [n], K, 16, D)
+        q = rng.standard_normal((new, H, D)).astype(np.float16)
+        out = dev(np.zeros_like(q))
+        a = kq.Attention(cache_of(p), dev(q), out, dev(np.array([n], np.int32)), q_start=dev(np.array([0, new], np.int32)))
+        torch.cuda.synchronize()
+        ctx.set_option("timeout_ms", 20)
+        ctx.set_option("inject_timeout", 1)
+        ctx.attn_prefill_async(a)
+        with pytest.raises(kq.KQError) as e:
+            ctx.synchronize()
+        assert e.value.status == -7
+        ctx.set_option("inject_timeout", 0)
+        ctx.set_option("timeout_ms", 1000)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            ctx.attn_prefill_async(a)
+        want, tol = R.expect(p, q, [(i, 0, n - new + i, n) for i in range(new)], 0, 0)
+        for call in (lambda: ctx.attn_prefill_async(a), g.replay, g.replay):
+            out.fill_(SENTINEL)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                call()
+            ctx.synchronize()
+            close(out.cpu().numpy(), want, tol)
+        del g, call
+    finally:
+        torch.cuda.synchronize()
+        ctx.close()

@@ -202,6 +202,12 @@ def test_block_refusals(kqctx):
     with pytest.raises(kq.KQError):                          # o is not [hidden][heads * D]
         bad.struct.o = b.w[1].handle
         kqctx.run_attn_async(bad, i3, i3, i3, x, torch.empty_like(x))
+    for y in (x, x.bfloat16()):                              # in place; another type
+        with pytest.raises((kq.KQError, ValueError)):
+            kqctx.run_attn_async(b.layer, i3, i3, i3, y, y)
+    both = torch.zeros((4, HIDDEN), dtype=torch.float16, device="cuda")
+    with pytest.raises(kq.KQError):                          # x_out lies over a part of x_in
+        kqctx.run_attn_async(b.layer, i3, i3, i3, both[:3], both[1:])
     for field, value in (("window", -1), ("sinks", 2), ("eps", -1.0), ("gamma", None), ("heads", 7), ("cache", None), ("q", None)):
         keep = getattr(b.layer.struct, field)
         setattr(b.layer.struct, field, value)
@@ -210,3 +216,5 @@ def test_block_refusals(kqctx):
         setattr(b.layer.struct, field, keep)
     kqctx.synchronize()
     b.free()
+    with pytest.raises(ValueError):                          # the layer's weights are gone
+        kqctx.run_attn_async(b.layer, i3, i3, i3, x, torch.empty_like(x))
