@@ -26,7 +26,7 @@
 // in order by the last of them, no finer than the joins pay for (make_plan).
 //
 // 512 rows behind 32,256 keys, 32 / 8 heads of 128: 283 us, 970 TFLOP/s, at the power cap (1.47 GHz); tensor
-// pipe and exponential unit 60% busy.  A 2,048-token prompt: 45 us, of which 4 pass before the first
+// pipe and exponential unit 60% busy.  A 2,048-token prompt: 43 us, of which 3.6 pass before the first
 // block and 2.5 in each item's epilogue; a block takes 1.75 us at 1.9 GHz, 0.6 of it MMAs that the
 // tile's own softmax waits for.
 #include "kq_attn_dev.cuh"
@@ -282,10 +282,11 @@ constexpr size_t kSmem = 226 * 1024;  // dynamic
 
 // What the plan is made with, in the ring's memory.
 struct PlanScratch {
-    long long red[kThreads / 32];
+    long long red[kThreads / 32], ends[kThreads / 32];
     int red_max[kThreads / 32];
     float red_split[kThreads / 32];
-    int nbs[1];  // blocks of every row tile
+    int rank[kSortTiles];  // of every row tile, the longest first
+    int nbs[1];            // blocks of every row tile
 };
 
 // Place in the ring: advanced block by block (a division by the number of stages would cost more than
@@ -324,7 +325,8 @@ struct Waiter {
     }
 };
 
-// The CTA's plan, by all its threads.
+// The CTA's plan, by all its threads (complete after the next barrier).  Every CTA makes its own: 2.6 us for one
+// prompt, 1.0 of it the lengths on their way; a launch before this one would take longer.
 template <int D>
 __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, int *seq_tiles, unsigned short *order, PlanScratch &scratch) {
     using C = Cfg<D>;
@@ -371,84 +373,109 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         // an item's blocks times what joining a part of it costs, in blocks: its rows' bytes and a latency
         split = fmaxf(split, s.nb * (s.n_tok * p.group * (D / 54000.0f) + 0.17f));
     }
-    long long run = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, run, d);
-        if (lane >= d) run += o;
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
-        split = fmaxf(split, __shfl_xor_sync(0xffffffffu, split, d));
-    }
-    if (lane == 31) scratch.red[warp] = run;
-    if (lane == 0) {
-        scratch.red_max[warp] = most;
-        scratch.red_split[warp] = split;
+    {
+        // (a thread's sum may pass 32 bits in all, not in halves of 16 bits and the rest)
+        const unsigned lo = __reduce_add_sync(0xffffffffu, (unsigned)(sum & 0xffff));
+        const unsigned hi = __reduce_add_sync(0xffffffffu, (unsigned)(sum >> 16));
+        most = __reduce_max_sync(0xffffffffu, most);
+        split = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(split)));  // (positive: ordered like its bits)
+        if (lane == 0) {
+            scratch.red[warp] = ((long long)hi << 16) + lo;
+            scratch.red_max[warp] = most;
+            scratch.red_split[warp] = split;
+        }
+        if (tid < kSortTiles - kThreads) scratch.rank[kThreads + tid] = 0;
+        scratch.rank[tid] = 0;
     }
     __syncthreads();
-    long long before = run - sum, total = 0;
+    long long total = 0;
     for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) before += scratch.red[w];
         total += scratch.red[w];
         most = max(most, scratch.red_max[w]);
         split = fmaxf(split, scratch.red_split[w]);
     }
     total *= heads;
     // Whole items in snake order, unless the fullest CTA would get more than an even share and a join.
-    const int G = gridDim.x;
+    const int G = gridDim.x, items = tiles * heads;
     const Shares even(total > 0 ? total : 1, G);
-    const bool sorted = tiles <= kSortTiles;
-    bool whole = (long long)tiles * heads >= 32ll * G;  // (so many that the order evens out)
-    if (!whole && most <= even.q + kJoinBlocks && sorted) {
-        for (int i = tid; i < tiles; i += kThreads) {
-            int rank = 0;
-            for (int j = 0; j < tiles; ++j) rank += nbs[j] > nbs[i] || (nbs[j] == nbs[i] && j < i);
-            order[rank] = (unsigned short)i;
-        }
-        __syncthreads();
-        int fits = 1;
-        for (int c = tid; c < G; c += kThreads) {
-            int sum = 0;
-            for (int k = 0; k * G < tiles * heads; ++k) {
-                const unsigned idx = k * G + ((k & 1) ? G - 1 - c : c);
-                if (idx < (unsigned)(tiles * heads)) sum += nbs[order[idx / (unsigned)heads]];
+    bool whole = items >= 32 * G, ordered = false;  // (so many that the order evens out)
+    if (!whole && most <= even.q + kJoinBlocks) {
+        // longest first: from the last tile on where no tile is longer than the next (one prompt), else by rank
+        bool rising = true;
+        for (int i = max(i0, 1); i < i0 + chunk && i < tiles; ++i) rising &= nbs[i - 1] <= nbs[i];
+        ordered = !__syncthreads_and(rising);
+        if (ordered && tiles <= kSortTiles) {
+            const int by = max(kThreads / tiles, 1);  // threads that share a tile's comparisons
+            for (int e = tid; e < tiles * by; e += kThreads) {
+                const int i = e % tiles, n = nbs[i];
+                int rank = 0;
+                for (int j = e / tiles; j < tiles; j += by) rank += nbs[j] > n || (nbs[j] == n && j < i);
+                atomicAdd(&scratch.rank[i], rank);
             }
-            fits &= sum <= even.q + kJoinBlocks;
+            __syncthreads();
+            for (int i = tid; i < tiles; i += kThreads) order[scratch.rank[i]] = (unsigned short)i;
+            __syncthreads();
+        }
+        int fits = !ordered || tiles <= kSortTiles;
+        for (int c = tid; fits && c < G; c += kThreads) {
+            int sum = 0;
+            for (int k = 0; k * G < items; ++k) {
+                const int idx = k * G + ((k & 1) ? G - 1 - c : c), rank = (unsigned)idx / (unsigned)heads;
+                if (idx < items) sum += nbs[ordered ? order[rank] : tiles - 1 - rank];
+            }
+            fits = sum <= even.q + kJoinBlocks;
         }
         whole = __syncthreads_and(fits);
     }
+    Plan &pl = sh.plan;
     if (tid == 0) {
-        Plan &pl = sh.plan;
         pl.seq_tiles = seq_tiles;
-        pl.order = sorted && (long long)tiles * heads < 32ll * G ? order : nullptr;
+        pl.order = ordered ? order : nullptr;
         pl.tiles = tiles;
         pl.whole = whole;
-        pl.c0 = pl.c1 = 0;
-        pl.start_tile = 0;
-        pl.start_begin = 0;
-        // Split: shares of x blocks take x and joining an item of n blocks (n / x) c blocks' time, least at
-        // x = sqrt(n c); more CTAs than that would spend longer joining than they save.
-        const float x = fmaxf(sqrtf(split), 1.0f);
-        const int parts = (int)fmaxf(fminf((float)G, (float)total / x), 1.0f);
-        if (!whole) {
-            pl.shares = parts == G ? even : Shares(total, parts);
-            if ((int)blockIdx.x < parts) {
-                pl.c0 = pl.shares.begin(blockIdx.x);
-                pl.c1 = pl.shares.begin(blockIdx.x + 1);
-            }
+    }
+    if (whole) {
+        if (tid == 0) {
+            pl.start_tile = 0;
+            pl.start_begin = pl.c0 = pl.c1 = 0;
+        }
+        return;
+    }
+    // Split: shares of x blocks take x and joining an item of n blocks (n / x) c blocks' time, least at
+    // x = sqrt(n c); more CTAs than that would spend longer joining than they save.
+    const float x = fmaxf(sqrtf(split), 1.0f);
+    const int parts = (int)fmaxf(fminf((float)G, (float)total / x), 1.0f);
+    const Shares shares = parts == G ? even : Shares(total > 0 ? total : 1, parts);
+    long long run = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, run, d);
+        if (lane >= d) run += o;
+    }
+    if (lane == 31) scratch.ends[warp] = run;
+    const bool mine = total > 0 && (int)blockIdx.x < parts;
+    const long long c0 = mine ? shares.begin(blockIdx.x) : 0, c1 = mine ? shares.begin(blockIdx.x + 1) : 0;
+    if (tid == 0) {
+        pl.shares = shares;
+        pl.c0 = c0;
+        pl.c1 = c1;
+        if (c1 <= c0) {
+            pl.start_tile = 0;
+            pl.start_begin = 0;
         }
     }
     __syncthreads();
-    if (!whole && sh.plan.c1 > sh.plan.c0) {
-        const long long c0 = sh.plan.c0;
+    if (c1 > c0) {
+        long long before = run - sum;
+        for (int w = 0; w < warp; ++w) before += scratch.ends[w];
         for (int i = i0; i < i0 + chunk && i < tiles; ++i) {
             if (before * heads <= c0 && c0 < (before + nbs[i]) * heads) {
-                sh.plan.start_tile = i;
-                sh.plan.start_begin = before * heads;
+                pl.start_tile = i;
+                pl.start_begin = before * heads;
             }
             before += nbs[i];
         }
     }
-    __syncthreads();
 }
 
 // Loads of one CTA by a warp each: the K warp hands the segments to the other roles and loads Q and K,
@@ -485,19 +512,32 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
         }
         if (!s.live) return;
         const int32_t *table = a.cache.table + (long long)s.seq * a.cache.table_stride;
-        // The page of this lane's box of block i; n_pages, out of range, where no token sees the box
-        // (the copy fills it with zeros) or the table names no page.
-        auto page_of = [&](int i) {
-            const int j = kv_block(s.blocks, i) * BN + sub * p.box_rows;
-            if (lane >= boxes || i >= s.b1 || !tile_sees(s, j, p.box_rows)) return a.cache.n_pages;
-            const int q = table[j >> a.cache.page_shift];
-            if (kv_page_ok(a.cache, q)) return q;
-            if (!V) *reinterpret_cast<volatile int *>(&rec.bad) = 1;
-            return a.cache.n_pages;
+        // This lane's box of block i in the table: read a block ahead, looked at when it is needed.
+        struct Entry {
+            int page;
+            bool sees;  // whether any token sees the box
         };
-        int page = page_of(s.b0);
+        auto entry_of = [&](int i) {
+            const int j = kv_block(s.blocks, i) * BN + sub * p.box_rows;
+            Entry e{0, lane < boxes && i < s.b1 && tile_sees(s, j, p.box_rows)};
+            if (e.sees) e.page = table[j >> a.cache.page_shift];
+            return e;
+        };
+        auto load_q = [&] {
+            const int subs = s.n_tok > p.tpt ? NT : 1;
+            if (!wait(sh.q_empty, (k & 1) ^ 1)) return false;
+            if (lane == 0) mbar_arrive_expect_tx(smem_u32(&sh.q_full), (uint32_t)(subs * p.tpt * p.group * D * 2));
+            __syncwarp();
+            if (lane < subs * CH)
+                tma3(smem_u32(s_q) + sub * C::Q_TILE + piece * (128 * 128), &mq, 64 * piece, s.head * p.group,
+                     s.row0 + sub * p.tpt, smem_u32(&sh.q_full));
+            __syncwarp();
+            return true;
+        };
+        Entry here = entry_of(s.b0);
+        if (!V && k == 0 && !load_q()) return;  // (later items' queries wait for room: not before their first keys)
         for (int i = s.b0; i < s.b1; ++i) {
-            const int next = page_of(i + 1);  // a block ahead
+            const Entry next = entry_of(i + 1);
             const uint32_t st = at.stage;
             if (!wait((V ? sh.v_empty : sh.k_empty)[st], at.phase ^ 1)) return;
             at.next(stages);
@@ -507,6 +547,11 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
             // V rows past the sequence's end may hold anything, and 0 * NaN is NaN: zeroed once they landed
             const bool tail = V && j0 + BN > s.len;
             const uint32_t bar = smem_u32(tail ? &sh.tail : &full);
+            // a box that no token sees, or whose page is missing: n_pages, out of range, is filled with zeros
+            const bool ok = here.sees && kv_page_ok(a.cache, here.page);
+            if (!V && here.sees && !ok) *reinterpret_cast<volatile int *>(&rec.bad) = 1;
+            const int page = ok ? here.page : a.cache.n_pages;
+            __syncwarp();
             if (lane == 0) mbar_arrive_expect_tx(bar, C::STAGE);
             __syncwarp();
             if (lane < boxes)
@@ -524,17 +569,8 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
                 if (lane == 0) mbar_arrive(smem_u32(&full));
             }
             __syncwarp();
-            page = next;
-            if (!V && i == s.b0) {
-                const int subs = s.n_tok > p.tpt ? NT : 1;
-                if (!wait(sh.q_empty, (k & 1) ^ 1)) return;
-                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&sh.q_full), (uint32_t)(subs * p.tpt * p.group * D * 2));
-                __syncwarp();
-                if (lane < subs * CH)
-                    tma3(smem_u32(s_q) + sub * C::Q_TILE + piece * (128 * 128), &mq, 64 * piece, s.head * p.group,
-                         s.row0 + sub * p.tpt, smem_u32(&sh.q_full));
-                __syncwarp();
-            }
+            here = next;
+            if (!V && k > 0 && i == s.b0 && !load_q()) return;
         }
     }
 }
