@@ -1155,7 +1155,7 @@ int attn_scratch(kq_ctx *c, kq::AttnLaunch &L) {
     if (int r = ensure(c, c->attn_parts, std::max(kq::attn_decode_part_bytes(c->num_sms),
                                                             kq::attn_prefill_part_bytes(c->num_sms)))) return r;
     const bool clear = !c->attn_count.p || c->attn_dirty;
-    if (int r = ensure(c, c->attn_count, sizeof(unsigned) * (size_t)c->num_sms)) return r;
+    if (int r = ensure(c, c->attn_count, sizeof(unsigned) * kq::attn_counts(c->num_sms))) return r;
     if (clear) {
         KQ_CUDA(c, cudaMemsetAsync(c->attn_count.p, 0, c->attn_count.cap, c->stream));
         // a capture has only recorded it: the counts stay as they are until the graph runs

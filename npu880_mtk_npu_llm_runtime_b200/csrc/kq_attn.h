@@ -47,5 +47,7 @@ size_t attn_prefill_part_bytes(int num_sms);
 cudaError_t launch_attn_prefill(const AttnLaunch &L, cudaStream_t stream);
 // kq_attn_decode.cu
 size_t attn_decode_part_bytes(int num_sms);
+// arrival counts: an item's, and its two groups' (see DecodeParams)
+inline size_t attn_counts(int num_sms) { return (size_t)3 * num_sms; }
 cudaError_t launch_attn_decode(const AttnLaunch &L, cudaStream_t stream);
 }  // namespace kq

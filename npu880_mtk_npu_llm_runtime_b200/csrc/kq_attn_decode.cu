@@ -27,6 +27,7 @@
 #include "kq_attn_dev.cuh"
 
 #include <mutex>
+#include <type_traits>
 
 namespace kq {
 
@@ -41,6 +42,9 @@ constexpr int kUnit = 16;  // keys of a unit; a page holds a multiple of it
 // would end last.
 constexpr int kBegin = 2;
 constexpr int kJoin = 3;
+constexpr int kFan = 12;  // parts that a thread joins one after another (148: two steps of 12)
+constexpr int kAhead = 6;  // of them on their way at once, ..
+constexpr int kFew = 3;    // .. but where there are no more than this one by one (less code to fetch)
 
 template <int D, int NB>
 struct Cfg {
@@ -56,8 +60,9 @@ struct DecodeParams {
     int group, rows, splits;  // query heads of a key head; of an item; items of a key head
     int part_floats;          // floats of a part: rows x (D + 2), to a multiple of 16 bytes
     int floats;               // shared memory before the tables
-    float *parts;             // [CTA][2] parts of rows x D values, then [rows][2] (m, l)
-    unsigned *count;          // [CTA] arrivals at the item that begins in a CTA and ends in a later one
+    float *parts;             // [2][CTA][2] parts (and joined ones) of rows x D values, then [rows][2] (m, l)
+    unsigned *count;          // [CTA] arrivals at the item that begins in a CTA and ends in a later one; then
+                              // [CTA][2] at the groups of its parts
 };
 
 // The cache streams through: first to leave L2, so that what is used again (the kernel's code, the
@@ -421,47 +426,64 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
     }
     if (before < 0 && after < 0) return;  // uniform over the CTA
 
-    // Items shared with other CTAs: the last to arrive joins their parts in unit order.
+    // Items shared with other CTAs: the last to arrive joins their parts in unit order.  Where a thread would have
+    // more than kFan of them one after another, the last of every fan CTAs joins those first (into a second set of
+    // parts), and the last of all what comes of that.
+    const int groups = elems < C::THREADS ? C::THREADS / elems : 1;  // threads left over share the parts
+    const int fan = kFan * groups, G = gridDim.x, me = blockIdx.x;
     int first[2] = {0, 0}, last[2] = {0, 0};
     if (before >= 0) {
         first[0] = shares.of(s_part[before].begin);
-        last[0] = s_part[before].end > c1 ? shares.of(s_part[before].end - 1) : (int)blockIdx.x;
+        last[0] = s_part[before].end > c1 ? shares.of(s_part[before].end - 1) : me;
     }
     if (after >= 0) {
-        first[1] = blockIdx.x;
+        first[1] = me;
         last[1] = shares.of(s_part[after].end - 1);
     }
+    const bool many[2] = {last[0] - first[0] >= kFew * groups, last[1] - first[1] >= kFew * groups};
     __syncthreads();
     if (tid < 2) {
         int is_last = 0;
         if ((tid ? after : before) >= 0) {
             const int f = tid ? first[1] : first[0], l = tid ? last[1] : last[0];
+            unsigned *count = p.count + f;
+            int others = l - f;
+            if (others >= fan) {
+                const int g0 = f + (me - f) / fan * fan;
+                count = p.count + G + 2 * g0 + (g0 == f);
+                others = min(fan - 1, l - g0);
+            }
             // after the barrier: the release covers the whole CTA's part
-            is_last = count_arrival(p.count + f) == (unsigned)(l - f);
-            if (is_last) p.count[f] = 0;  // for the next launch
+            is_last = count_arrival(count) == (unsigned)others;
+            if (is_last) *count = 0;  // for the next launch
         }
         s_last[tid] = is_last;
     }
     __syncthreads();
-    const int groups = elems < C::THREADS ? C::THREADS / elems : 1;  // threads left over share the parts
     float2 *s_ml = reinterpret_cast<float2 *>(s_parts + 4 * C::THREADS);
     float4 *s_v = reinterpret_cast<float4 *>(s_parts);
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        if (!s_last[which]) continue;  // uniform over the CTA
-        const PartInfo info = s_part[which ? after : before];
-        const int f = first[which], n = last[which] - f + 1;
+    // n parts, the i-th at part(i), `ahead` of them on their way at once; put(r, d, joint) takes every four values
+    auto join = [&](auto ahead, int n_rows, int n, auto part, auto put) {
+        constexpr int A = decltype(ahead)::value;
         for (int e0 = 0; e0 < elems; e0 += C::THREADS) {
             const int e = groups > 1 ? tid % elems : e0 + tid, grp = groups > 1 ? tid / elems : 0;
             const int r = e / (D / 4), d = 4 * (e % (D / 4));
-            const bool on = e < elems && grp < groups && r < info.n_rows;
+            const bool on = e < elems && grp < groups && r < n_rows;
             Joint jn;
             if (on) {
-#pragma unroll 4
-                for (int i = grp; i < n; i += groups) {
-                    const float *part = p.parts + (size_t)(2 * (f + i) + (i == 0)) * part_floats;
-                    jn.add(__ldcg(reinterpret_cast<const float2 *>(part + p.rows * D + 2 * r)),
-                           __ldcg(reinterpret_cast<const float4 *>(part + r * D + d)));
+#pragma unroll 1
+                for (int i = grp; i < n; i += A * groups) {
+                    float2 ml[A];
+                    float4 v[A];
+#pragma unroll
+                    for (int u = 0; u < A; ++u) {
+                        const float *from = part(A > 1 ? min(i + u * groups, n - 1) : i);
+                        ml[u] = __ldcg(reinterpret_cast<const float2 *>(from + p.rows * D + 2 * r));
+                        v[u] = __ldcg(reinterpret_cast<const float4 *>(from + r * D + d));
+                    }
+#pragma unroll
+                    for (int u = 0; u < A; ++u)
+                        if (u == 0 || i + u * groups < n) jn.add(ml[u], v[u]);
                 }
                 if (grp > 0) {
                     s_v[tid] = jn.v;
@@ -471,10 +493,61 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
             if (groups > 1) __syncthreads();
             if (on && grp == 0) {
                 for (int k = 1; k < groups; ++k) jn.add(s_ml[k * elems + e], s_v[k * elems + e]);
-                *reinterpret_cast<uint2 *>(a.out + info.seq * a.out_stride + (info.head0 + r) * D + d) = jn.result();
+                put(r, d, jn);
             }
         }
         __syncthreads();
+    };
+    if (many[0] || many[1]) {
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+            if (!s_last[which] || !(which ? many[1] : many[0])) continue;  // uniform over the CTA
+            const PartInfo info = s_part[which ? after : before];
+            const int f = which ? first[1] : first[0], l = which ? last[1] : last[0];
+            const bool two = l - f >= fan;
+            int at = f, step = 1, n = l - f + 1;  // the parts of CTAs at, at + step, ..; joined ones: G further on
+            float *to = nullptr;
+            if (two) {
+                at = f + (me - f) / fan * fan;
+                n = min(fan, l - at + 1);
+                to = p.parts + (size_t)(2 * (G + at) + (at == f)) * part_floats;
+            }
+            while (true) {
+                const int begins = at == f || at == G + f;  // the first part is of the CTA where the item begins
+                join(std::integral_constant<int, kAhead>(), info.n_rows, n,
+                     [&](int i) { return p.parts + (size_t)(2 * (at + step * i) + (i == 0 ? begins : 0)) * part_floats; },
+                     [&](int r, int d, const Joint &jn) {
+                         if (to) {
+                             *reinterpret_cast<float4 *>(to + r * D + d) = jn.v;
+                             if (d == 0) *reinterpret_cast<float2 *>(to + p.rows * D + 2 * r) = jn.mark();
+                         } else {
+                             *reinterpret_cast<uint2 *>(a.out + info.seq * a.out_stride + (info.head0 + r) * D + d) = jn.result();
+                         }
+                     });
+                if (!to) break;
+                if (tid == 0) {
+                    s_last[which] = count_arrival(p.count + f) == (unsigned)((l - f) / fan);
+                    if (s_last[which]) p.count[f] = 0;
+                }
+                __syncthreads();
+                if (!s_last[which]) break;
+                at = G + f;
+                step = fan;
+                n = (l - f) / fan + 1;
+                to = nullptr;
+            }
+        }
+    }
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        if (!s_last[which] || many[which]) continue;  // uniform over the CTA
+        const PartInfo info = s_part[which ? after : before];
+        const int f = first[which], n = last[which] - f + 1;
+        join(std::integral_constant<int, 1>(), info.n_rows, n,
+             [&](int i) { return p.parts + (size_t)(2 * (f + i) + (i == 0)) * part_floats; },
+             [&](int r, int d, const Joint &jn) {
+                 *reinterpret_cast<uint2 *>(a.out + info.seq * a.out_stride + (info.head0 + r) * D + d) = jn.result();
+             });
     }
 }
 
@@ -515,7 +588,7 @@ cudaError_t launch(DecodeParams &p, cudaStream_t stream) {
 
 }  // namespace
 
-size_t attn_decode_part_bytes(int num_sms) { return (size_t)2 * num_sms * KQ_MAX_GROUP * (KQ_MAX_HEAD_DIM + 2) * 4; }
+size_t attn_decode_part_bytes(int num_sms) { return (size_t)4 * num_sms * KQ_MAX_GROUP * (KQ_MAX_HEAD_DIM + 2) * 4; }
 
 cudaError_t launch_attn_decode(const AttnLaunch &L, cudaStream_t stream) {
     DecodeParams p{};

@@ -856,3 +856,28 @@ def test_capture_between_a_timeout_and_the_next_call(kqctx):
     finally:
         torch.cuda.synchronize()
         ctx.close()
+
+
+@pytest.mark.parametrize("D, G, K, lens, page", [
+    (128, 16, 1, [14368], 32), (128, 16, 1, [70001, 9], 64), (256, 8, 1, [30011], 16), (256, 16, 1, [25000], 64), (64, 16, 1, [50007], 64),
+    (64, 1, 1, [90001], 64), (128, 12, 2, [33333], 128), (256, 2, 1, [61000], 256),
+])
+def test_decode_few_items_of_many_parts(kqctx, D, G, K, lens, page):
+    """so few items that nearly every CTA has a part of one: parts joined in two steps, the same way every time"""
+    import torch
+    rng = np.random.default_rng(D + G)
+    p = R.Paged(rng, lens, K, page, D)
+    q = rng.standard_normal((len(lens), G * K, D)).astype(np.float16)
+    out = dev(np.zeros_like(q))
+    a = kq.Attention(cache_of(p), dev(q), out, dev(np.array(lens, np.int32)))
+    kqctx.attn_decode_async(a)
+    kqctx.synchronize()
+    first = out.cpu().numpy()
+    want, tol = R.expect(p, q, [(s, s, n - 1, n) for s, n in enumerate(lens)], 0, 0)
+    close(first, want, tol)
+    for _ in range(4):
+        out.fill_(SENTINEL)
+        torch.cuda.synchronize()
+        kqctx.attn_decode_async(a)
+        kqctx.synchronize()
+        assert (out.cpu().numpy() == first).all()
