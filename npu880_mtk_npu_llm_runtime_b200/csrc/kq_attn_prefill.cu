@@ -33,6 +33,7 @@
 
 #include <cuda.h>
 #include <mutex>
+#include <type_traits>
 
 namespace kq {
 
@@ -47,6 +48,10 @@ constexpr int kSortTiles = 512;
 // longer than an even share.
 constexpr int kJoinBlocks = 8;
 constexpr int kJoinAhead = 3;  // parts whose values a join has on their way at once
+// Parts are joined in two steps where there are more than kOneStep and together more than kOneStepRows rows (18
+// parts of 128 rows 68 us against 59, of 256 rows 74 against 63; but 18 of 32 rows 45.4 against 46.9, 12 of
+// 32 rows 23.4 against 25.6, 7 of 256 rows 40 against 49).
+constexpr int kOneStep = 8, kOneStepRows = 1024;
 
 template <int D>
 struct Cfg {
@@ -325,6 +330,12 @@ struct Waiter {
     }
 };
 
+// Sum over a warp of values below 2^43 (each half of it stays below 2^32).
+__device__ __forceinline__ long long sum_of_warp(long long v) {
+    const unsigned lo = __reduce_add_sync(0xffffffffu, (unsigned)(v & 0xffff));
+    return ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(v >> 16)) << 16) + lo;
+}
+
 // The CTA's plan, by all its threads (complete after the next barrier).  Every CTA makes its own: 2.6 us for one
 // prompt, 1.0 of it the lengths on their way; a launch before this one would take longer.
 template <int D>
@@ -352,8 +363,7 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         }
         if (lane == 31) scratch.red[warp] = run;
         __syncthreads();
-        int base = run - sum;
-        for (int w = 0; w < warp; ++w) base += (int)scratch.red[w];
+        const int base = run - sum + __reduce_add_sync(0xffffffffu, lane < warp ? (int)scratch.red[lane] : 0);
         for (int s = s0; s < s0 + chunk && s < S; ++s) seq_tiles[s] += base;
         if (tid == kThreads - 1) seq_tiles[S] = base + sum;
         __syncthreads();
@@ -374,13 +384,11 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         split = fmaxf(split, s.nb * (s.n_tok * p.group * (D / 54000.0f) + 0.17f));
     }
     {
-        // (a thread's sum may pass 32 bits in all, not in halves of 16 bits and the rest)
-        const unsigned lo = __reduce_add_sync(0xffffffffu, (unsigned)(sum & 0xffff));
-        const unsigned hi = __reduce_add_sync(0xffffffffu, (unsigned)(sum >> 16));
+        const long long warp_sum = sum_of_warp(sum);
         most = __reduce_max_sync(0xffffffffu, most);
         split = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(split)));  // (positive: ordered like its bits)
         if (lane == 0) {
-            scratch.red[warp] = ((long long)hi << 16) + lo;
+            scratch.red[warp] = warp_sum;
             scratch.red_max[warp] = most;
             scratch.red_split[warp] = split;
         }
@@ -388,13 +396,10 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         scratch.rank[tid] = 0;
     }
     __syncthreads();
-    long long total = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-        total += scratch.red[w];
-        most = max(most, scratch.red_max[w]);
-        split = fmaxf(split, scratch.red_split[w]);
-    }
-    total *= heads;
+    const bool a_warp = lane < kThreads / 32;  // each warp puts the warps' values together
+    const long long total = sum_of_warp(a_warp ? scratch.red[lane] : 0) * heads;
+    most = __reduce_max_sync(0xffffffffu, a_warp ? scratch.red_max[lane] : 0);
+    split = __uint_as_float(__reduce_max_sync(0xffffffffu, a_warp ? __float_as_uint(scratch.red_split[lane]) : 0u));
     // Whole items in snake order, unless the fullest CTA would get more than an even share and a join.
     const int G = gridDim.x, items = tiles * heads;
     const Shares even(total > 0 ? total : 1, G);
@@ -443,11 +448,10 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
     }
     // Split: shares of x blocks take x and joining an item of n blocks (n / x) c blocks' time, least at
     // x = sqrt(n c); more CTAs than that would spend longer joining than they save.
-    const float x = fmaxf(sqrtf(split), 1.0f);
-    const int parts = (int)fmaxf(fminf((float)G, (float)total / x), 1.0f);
+    const int parts = (int)fmaxf(fminf((float)G, (float)total * rsqrtf(fmaxf(split, 1.0f))), 1.0f);
     const Shares shares = parts == G ? even : Shares(total > 0 ? total : 1, parts);
     long long run = sum;
-#pragma unroll
+#pragma unroll 1
     for (int d = 1; d < 32; d <<= 1) {
         const long long o = __shfl_up_sync(0xffffffffu, run, d);
         if (lane >= d) run += o;
@@ -465,9 +469,8 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         }
     }
     __syncthreads();
-    if (c1 > c0) {
-        long long before = run - sum;
-        for (int w = 0; w < warp; ++w) before += scratch.ends[w];
+    if (c1 > c0) {  // (uniform over the CTA)
+        long long before = run - sum + sum_of_warp(lane < warp ? scratch.ends[lane] : 0);
         for (int i = i0; i < i0 + chunk && i < tiles; ++i) {
             if (before * heads <= c0 && c0 < (before + nbs[i]) * heads) {
                 pl.start_tile = i;
@@ -859,87 +862,113 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
             }
         }
         if (!whole) {
-            // the last CTA that brings a part of the item joins them in order
+            // The last CTA that brings a part of the item joins them in order; or, in two steps, the last of every
+            // `fan` CTAs joins theirs (in place of the first one's part) and the last of all what comes of that: a
+            // CTA reads a part of 256 rows in 1.5-2 us, and so has fan + n / fan of them on its way, not n.
             const int first = sh.plan.shares.of(s.begin);
-            const int last = sh.plan.shares.of(s.begin + s.nb - 1);
-            if (!together()) return;
-            if (tid == 0) {
-                // after the barrier: the release covers all of the CTA's rows
-                sh.last = count_arrival(a.count + first) == (unsigned)(last - first);
-                if (sh.last) a.count[first] = 0;  // for the next launch
-            }
-            if (!together()) return;
-            const bool join = sh.last != 0;
-            if (!together()) return;
-            if (join && active) {
-                // A tile of 32 or 64 rows gives its other warps shares of the values.
-                const int rows = min(s.n_tok - t * p.tpt, p.tpt) * p.group;
-                const int span_warps = rows <= 32 ? 1 : rows <= 64 ? 2 : 4, shares = 4 / span_warps;
-                const int jr = (warp & (span_warps - 1)) * 32 + lane;  // this thread's row of the tile
-                const bool on = jr < rows;
-                const int jtok = t * p.tpt + jr / p.group, jhead = s.head * p.group + jr % p.group;
-                uint16_t *jout = a.out + (long long)(s.row0 + jtok) * a.out_stride + jhead * D;
-                auto part_at = [&](int c) {
-                    return reinterpret_cast<const float4 *>(a.parts + (size_t)(2 * c + (c == first)) * part_rows * (D + 2));
-                };
-                auto stat_at = [&](int c) { return __ldcg(reinterpret_cast<const float2 *>(part_at(c) + D / 4 * part_rows) + t * 128 + jr); };
-                float M = -INFINITY, L = 0.0f;
-                bool missing = false;
-                float2 odd = make_float2(0.0f, 0.0f);
-                if (on) {
+            const int last = sh.plan.shares.of(s.begin + s.nb - 1), n = last - first + 1;
+            // A tile of 32 or 64 rows gives its other warps shares of the values.
+            const int rows = active ? min(s.n_tok - t * p.tpt, p.tpt) * p.group : 0;
+            const int span_warps = rows <= 32 ? 1 : rows <= 64 ? 2 : 4, shares = 4 / span_warps;
+            const int jr = (warp & (span_warps - 1)) * 32 + lane;  // this thread's row of the tile
+            const bool on = jr < rows;
+            auto part_at = [&](int c) { return reinterpret_cast<float4 *>(a.parts + (size_t)(2 * c + (c == first)) * part_rows * (D + 2)); };
+            auto stat_at = [&](int c) { return reinterpret_cast<float2 *>(part_at(c) + D / 4 * part_rows) + t * 128 + jr; };
+            // whether this CTA is the last of `others` + 1
+            auto arrive = [&](unsigned *count, int others, bool &join) {
+                if (!together()) return false;
+                if (tid == 0) {
+                    // after the barrier: the release covers all of the CTA's rows
+                    sh.last = count_arrival(count) == (unsigned)others;
+                    if (sh.last) *count = 0;  // for the next launch
+                }
+                if (!together()) return false;
+                join = sh.last != 0;
+                return together();
+            };
+            // The parts of CTAs from, from + step, .. to: 32 values of a row at a time to put(c0, o); the row's statistics.
+            auto join_parts = [&](int from, int to, auto step, float &M, float &L, bool &missing, auto put) {
+                M = -INFINITY;
+                L = 0.0f;
+                missing = false;
+                if (!on) return;
 #pragma unroll 8
-                    for (int c = first; c <= last; ++c) {
-                        const float2 ml = stat_at(c);
-                        missing |= ml.x != ml.x;
-                        const float top = fmaxf(M, ml.x);
-                        // a part without a score above -inf adds nothing; NaN (a NaN score) stays
-                        L = L * (M == -INFINITY ? 1.0f : exp2_fast(M - top)) +
-                            (ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.0f) : exp2_fast(ml.x - top) * ml.y);
-                        M = top;
-                    }
-                    const float inv = 1.0f / L;
-                    for (int c0 = 32 * ((warp & 3) / span_warps); c0 < D; c0 += 32 * shares) {
-                        float o[32];
+                for (int c = from; c <= to; c += step) {
+                    const float2 ml = __ldcg(stat_at(c));
+                    missing |= ml.x != ml.x;
+                    const float top = fmaxf(M, ml.x);
+                    // a part without a score above -inf adds nothing; NaN (a NaN score) stays
+                    L = L * (M == -INFINITY ? 1.0f : exp2_fast(M - top)) +
+                        (ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.0f) : exp2_fast(ml.x - top) * ml.y);
+                    M = top;
+                }
+                for (int c0 = 32 * ((warp & 3) / span_warps); c0 < D; c0 += 32 * shares) {
+                    float o[32];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
 #pragma unroll 1
-                        for (int c = first; c <= last; c += kJoinAhead) {
-                            float4 v[kJoinAhead][8];
-                            float w[kJoinAhead];
+                    for (int c = from; c <= to; c += kJoinAhead * step) {
+                        float4 v[kJoinAhead][8];
+                        float w[kJoinAhead];
 #pragma unroll
-                            for (int i = 0; i < kJoinAhead; ++i) {
-                                const int cc = min(c + i, last);
-                                const float4 *part = part_at(cc) + c0 / 4 * part_rows + t * 128 + jr;
-                                w[i] = stat_at(cc).x;
+                        for (int i = 0; i < kJoinAhead; ++i) {
+                            const int cc = min(c + i * step, to);
+                            const float4 *part = part_at(cc) + c0 / 4 * part_rows + t * 128 + jr;
+                            w[i] = __ldcg(stat_at(cc)).x;
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) v[i][e] = __ldcg(part + e * part_rows);
-                            }
+                            for (int e = 0; e < 8; ++e) v[i][e] = __ldcg(part + e * part_rows);
+                        }
 #pragma unroll
-                            for (int i = 0; i < kJoinAhead; ++i) {
-                                if (c + i > last) break;
-                                w[i] = w[i] == -INFINITY ? 0.0f : exp2_fast(w[i] - M);
+                        for (int i = 0; i < kJoinAhead; ++i) {
+                            if (c + i * step > to) break;
+                            w[i] = w[i] == -INFINITY ? 0.0f : exp2_fast(w[i] - M);
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    o[4 * e] += w[i] * v[i][e].x;
-                                    o[4 * e + 1] += w[i] * v[i][e].y;
-                                    o[4 * e + 2] += w[i] * v[i][e].z;
-                                    o[4 * e + 3] += w[i] * v[i][e].w;
-                                }
+                            for (int e = 0; e < 8; ++e) {
+                                o[4 * e] += w[i] * v[i][e].x;
+                                o[4 * e + 1] += w[i] * v[i][e].y;
+                                o[4 * e + 2] += w[i] * v[i][e].z;
+                                o[4 * e + 3] += w[i] * v[i][e].w;
                             }
                         }
-                        put32(o, inv, jout + c0, true, p.wide, odd);
                     }
+                    put(c0, o, L);
                 }
+            };
+            float M, L;
+            bool missing, join;
+            float2 odd = make_float2(0.0f, 0.0f);
+            const int jtok = t * p.tpt + jr / p.group, jhead = s.head * p.group + jr % p.group;
+            uint16_t *jout = a.out + (long long)(s.row0 + jtok) * a.out_stride + jhead * D;
+            auto result = [&](int c0, const float *o, float l) { put32(o, 1.0f / l, jout + c0, true, p.wide, odd); };
+            const std::integral_constant<int, 1> one;
+            if (n <= kOneStep || n * s.n_tok * p.group <= kOneStepRows) {
+                if (!arrive(a.count + first, n - 1, join)) return;
+                if (join) join_parts(first, last, one, M, L, missing, result);
+            } else {
+                const int fan = (int)ceilf(sqrtf((float)n)), g = ((int)blockIdx.x - first) / fan;
+                const int from = first + g * fan, to = min(from + fan - 1, last);
+                if (!arrive(a.count + (int)gridDim.x + 2 * from + (g == 0), to - from, join)) return;
+                if (join) {
+                    join_parts(from, to, 1, M, L, missing, [&](int c0, const float *o, float) {  // (nobody else reads these)
+                        float4 *part = part_at(from) + c0 / 4 * part_rows + t * 128 + jr;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) part[e * part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    });
+                    if (!together()) return;  // the row's other threads have read its old statistics
+                    if (on && (warp & 3) < span_warps) *stat_at(from) = make_float2(missing ? NAN : M, L);
+                    if (!arrive(a.count + first, (n - 1) / fan, join)) return;
+                    if (join) join_parts(first, first + (n - 1) / fan * fan, fan, M, L, missing, result);
+                }
+            }
+            if (join) {
                 __syncwarp();
                 const uint32_t wrong = __ballot_sync(0xffffffffu, on && (missing || M == -INFINITY || (L == L && !(odd.x + odd.y == 0.0f))));
                 if (lane == 0 && wrong) atomicOr(&sh.odd[t * 4 + (warp & (span_warps - 1))], wrong);
-            }
-            if (join) {
                 if (!together()) return;  // all values are written
-                const uint32_t wrong = sh.odd[warp];
+                const uint32_t mend = sh.odd[warp];
                 __syncwarp();
                 if (lane == 0) sh.odd[warp] = 0;  // (every warp has read its own before the next join's first meeting)
-                mend_rows<D>(p, sh, s, wrong >> lane & 1, tok, head, lane);
+                mend_rows<D>(p, sh, s, mend >> lane & 1, tok, head, lane);
             }
         }
         __syncwarp();

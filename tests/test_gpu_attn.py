@@ -881,3 +881,32 @@ def test_decode_few_items_of_many_parts(kqctx, D, G, K, lens, page):
         kqctx.attn_decode_async(a)
         kqctx.synchronize()
         assert (out.cpu().numpy() == first).all()
+
+
+@pytest.mark.parametrize("D, H, K, seqs, window", [
+    (128, 4, 1, [(60, 20000)], 0), (64, 16, 1, [(16, 26000)], 0), (256, 8, 1, [(32, 9000)], 0), (128, 16, 2, [(5, 21000), (30, 12000)], 0),
+    (128, 4, 1, [(64, 40001)], 30000),
+])
+def test_prefill_many_parts(kqctx, D, H, K, seqs, window):
+    """few rows over long caches: items in so many parts that they are joined in two steps, the same way every time"""
+    import torch
+    rng = np.random.default_rng(D + H)
+    lens = [n for _, n in seqs]
+    p = R.Paged(rng, lens, K, 64, D)
+    starts = np.cumsum([0] + [r for r, _ in seqs]).astype(np.int32)
+    q = rng.standard_normal((starts[-1], H, D)).astype(np.float16)
+    out = dev(np.zeros_like(q))
+    a = kq.Attention(cache_of(p), dev(q), out, dev(np.array(lens, np.int32)), q_start=dev(starts), window=window)
+    kqctx.attn_prefill_async(a)
+    kqctx.synchronize()
+    first = out.cpu().numpy()
+    rows = [(int(starts[s]) + i, s, n - r + i, n) for s, (r, n) in enumerate(seqs) for i in range(r)]
+    pick = rows[:: max(1, len(rows) // 12)]
+    want, tol = R.expect(p, q, pick, window, 0)
+    close(first[[r[0] for r in pick]], want, tol)
+    for _ in range(4):
+        out.fill_(SENTINEL)
+        torch.cuda.synchronize()
+        kqctx.attn_prefill_async(a)
+        kqctx.synchronize()
+        assert (out.cpu().numpy() == first).all()
