@@ -11,7 +11,8 @@
 // or ragged, load the SMs alike.  A warp works alone, without shared memory or barriers, and keeps
 // a whole unit (16 keys, 4 KB of K and 4 KB of V at D = 128) in flight in registers; the parts
 // of an item that several warps share meet in shared memory, those that several CTAs share in
-// global memory, joined in unit order by the last CTA that arrives.
+// global memory, joined in unit order by the last CTA that arrives (many parts in two steps: one
+// sequence of 14,000 keys, 16 query heads on one key head, 21 us where one step takes 77).
 //
 // The products run on mma.m16n8k16 with the keys (then the values' dimensions) as the 16 rows and
 // the query heads as the 8 columns, so a group of up to 8 heads wastes nothing of the registers:

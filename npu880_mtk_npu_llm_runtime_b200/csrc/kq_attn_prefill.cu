@@ -23,10 +23,11 @@
 // Work: an item is a row tile of one key head, a unit one of its key blocks.  Items go whole to
 // the CTAs, longest first in snake order, when that balances; else (few items, long caches) every
 // CTA takes an equal range of units, and the parts of an item that several CTAs share are joined
-// in order by the last of them, no finer than the joins pay for (make_plan).
+// in order by the last of them (in two steps where they are many), no finer than the joins pay for
+// (make_plan).
 //
 // 512 rows behind 32,256 keys, 32 / 8 heads of 128: 283 us, 970 TFLOP/s, at the power cap (1.47 GHz); tensor
-// pipe and exponential unit 60% busy.  A 2,048-token prompt: 43 us, of which 3.6 pass before the first
+// pipe and exponential unit 60% busy.  A 2,048-token prompt: 43 us, of which 3.3 pass before the first
 // block and 2.5 in each item's epilogue; a block takes 1.75 us at 1.9 GHz, 0.6 of it MMAs that the
 // tile's own softmax waits for.
 #include "kq_attn_dev.cuh"
@@ -336,7 +337,7 @@ __device__ __forceinline__ long long sum_of_warp(long long v) {
     return ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(v >> 16)) << 16) + lo;
 }
 
-// The CTA's plan, by all its threads (complete after the next barrier).  Every CTA makes its own: 2.6 us for one
+// The CTA's plan, by all its threads (complete after the next barrier).  Every CTA makes its own: 2.4 us for one
 // prompt, 1.0 of it the lengths on their way; a launch before this one would take longer.
 template <int D>
 __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, int *seq_tiles, unsigned short *order, PlanScratch &scratch) {
