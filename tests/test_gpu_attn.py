@@ -910,3 +910,52 @@ def test_prefill_many_parts(kqctx, D, H, K, seqs, window):
         kqctx.attn_prefill_async(a)
         kqctx.synchronize()
         assert (out.cpu().numpy() == first).all()
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+def test_special_values_in_many_parts(kqctx, prefill):
+    """items joined in two steps: a missing page is masked and reported, -inf scores weigh nothing, a NaN score
+    and an infinite value reach the rows that see them"""
+    rng = np.random.default_rng(19)
+    D, G, n, new, page = 128, 16, 30000, 10 if prefill else 1, 64
+    for what in ("page", "-inf", "all -inf", "nan", "inf"):
+        p = R.Paged(rng, [n], 1, page, D)
+        q = np.abs(rng.standard_normal((new, G, D))).astype(np.float16)
+        keep = np.arange(n)
+        if what == "page":
+            p.table[0, 201] = p.k.shape[0] + 5
+            keep = np.r_[0:201 * page, 202 * page:n]
+        elif what == "-inf":                              # a whole part's scores, and more
+            for i in range(100, 140):
+                p.k[p.table[0, i], 0] = -np.inf
+            keep = np.r_[0:100 * page, 140 * page:n]
+        elif what == "all -inf":
+            p.k[:] = -np.inf
+        elif what == "nan":
+            p.k[p.table[0, 77], 0, 5, 9] = np.nan
+        else:
+            p.v[p.table[0, 300], 0, 5, 9] = np.inf
+        p.keys[0], p.values[0] = p.keys[0][keep], p.values[0][keep]
+        out = dev(np.full_like(q, SENTINEL))
+        kv_len, start = dev(np.array([n], np.int32)), dev(np.array([0, new], np.int32))
+        if prefill:
+            kqctx.attn_prefill_async(kq.Attention(cache_of(p), dev(q), out, kv_len, q_start=start))
+        else:
+            kqctx.attn_decode_async(kq.Attention(cache_of(p), dev(q), out, kv_len))
+        if what == "page":
+            with pytest.raises(kq.KQError) as e:
+                kqctx.synchronize()
+            assert e.value.status == SHAPE
+        else:
+            kqctx.synchronize()
+        got = out.cpu().numpy()
+        if what in ("nan", "all -inf"):
+            assert np.isnan(got).all()
+            continue
+        m = len(keep)
+        want, tol = R.expect(p, q, [(i, 0, m - new + i, m) for i in range(new)], 0, 0)
+        cols = np.arange(D)
+        if what == "inf":
+            assert np.isinf(got[..., 9]).all()
+            cols = np.delete(cols, 9)
+        close(got[..., cols], want[..., cols], tol[..., cols], what)
