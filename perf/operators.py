@@ -210,13 +210,15 @@ _library = {}
 
 
 def _own(state, case):
-    """what a program that uses the library keeps: its context and the descriptions of its buffers"""
+    """what a program that uses the library keeps: a context for each stream, here of the stream on which
+    the inputs are made, and the descriptions of its buffers"""
     import npu880_mtk_npu_llm_runtime_b200 as kq
-    if "ctx" not in _library:
-        torch.cuda.init()
-        _library["ctx"] = kq.Context(torch.cuda.current_device())
-        _library["ctx"].set_stream(torch.cuda.current_stream().cuda_stream)
-    state["ctx"] = _library["ctx"]
+    torch.cuda.init()
+    at = (torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream)
+    if at not in _library:
+        _library[at] = kq.Context(at[0])
+        _library[at].set_stream(at[1])
+    state["ctx"] = _library[at]
     if "inv_freq" in state:
         state["rope"] = kq.Rope(case["rot"], base=case["base"], style=case["style"])
     if case["op"] != "norm_rope":
