@@ -322,8 +322,9 @@ typedef struct kq_attn {
 int kq_attn_decode_async(kq_ctx *ctx, const kq_kv_cache *cache, const kq_attn *a);
 /* Rows [q_start[s], q_start[s+1]) are sequence s's last tokens: with n of them the i-th stands at
  * position kv_len[s] - n + i (a negative one sees nothing).  q_start must not decrease and end at
- * or below M (else the sequence counts as having no rows, and KQ_ERR_SHAPE); rows outside the
- * sequences are left as they were. */
+ * or below M: a sequence for which it does counts as having no rows, and so does one whose rows begin
+ * in front of an earlier sequence's end, and KQ_ERR_SHAPE is reported; rows outside the sequences are
+ * left as they were. */
 int kq_attn_prefill_async(kq_ctx *ctx, const kq_kv_cache *cache, const kq_attn *a);
 
 /* The attention block of a layer, the counterpart of kq_run_ffn_async (the engine's ENG:7950-8261

@@ -348,9 +348,11 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
     {
         const int chunk = (S + kThreads - 1) / kThreads, s0 = tid * chunk;
         int sum = 0;
+        bool broken = false;
         for (int s = s0; s < s0 + chunk && s < S; ++s) {
             bool bad = false;
             const KvRows r = kv_rows(p.a.q_start[s], p.a.q_start[s + 1], p.a.M, bad);
+            broken |= bad;
             kv_length(p.a.cache, p.a.kv_len[s], bad);
             if (bad && blockIdx.x == 0) report_error(p.a.status, DEV_ERR_CACHE);
             seq_tiles[s] = sum;
@@ -363,7 +365,44 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
             if (lane >= d) run += o;
         }
         if (lane == 31) scratch.red[warp] = run;
-        __syncthreads();
+        if (__syncthreads_or(broken)) {
+            // q_start falls somewhere: what is valid for itself may overlap, and the tiles may then be more than the
+            // tables hold.  Once more, without the ranges that begin in front of an earlier one's end.
+            auto row_range = [&](int s, int limit) {
+                bool bad = false;
+                return kv_rows_behind(p.a.q_start[s], p.a.q_start[s + 1], p.a.M, limit, bad);
+            };
+            int end = 0;
+            for (int s = s0; s < s0 + chunk && s < S; ++s) {
+                const KvRows r = row_range(s, 0);
+                end = max(end, r.begin + r.n);
+            }
+#pragma unroll 1
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, end, d);
+                if (lane >= d) end = max(end, o);
+            }
+            if (lane == 31) scratch.red_max[warp] = end;
+            __syncthreads();
+            int limit = __shfl_up_sync(0xffffffffu, end, 1);
+            if (lane == 0) limit = 0;
+            for (int w = 0; w < warp; ++w) limit = max(limit, scratch.red_max[w]);
+            sum = 0;
+            for (int s = s0; s < s0 + chunk && s < S; ++s) {
+                seq_tiles[s] = sum;
+                sum += (row_range(s, limit).n + per - 1) / per;
+                const KvRows r = row_range(s, 0);
+                limit = max(limit, r.begin + r.n);
+            }
+            run = sum;
+#pragma unroll 1
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, run, d);
+                if (lane >= d) run += o;
+            }
+            if (lane == 31) scratch.red[warp] = run;
+            __syncthreads();
+        }
         const int base = run - sum + __reduce_add_sync(0xffffffffu, lane < warp ? (int)scratch.red[lane] : 0);
         for (int s = s0; s < s0 + chunk && s < S; ++s) seq_tiles[s] += base;
         if (tid == kThreads - 1) seq_tiles[S] = base + sum;

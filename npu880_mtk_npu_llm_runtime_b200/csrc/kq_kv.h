@@ -101,6 +101,19 @@ KQ_HD KvRows kv_rows(int start, int end, int M, bool &bad) {
     return r;
 }
 
+// The same where ranges overlap because q_start falls in between: rows before `limit` (the furthest end of the
+// sequences before s, each taken for itself) are another sequence's, so a range that begins there has none.
+// What is left is disjoint, M rows in all at most.
+KQ_HD KvRows kv_rows_behind(int start, int end, int M, int limit, bool &bad) {
+    KvRows r = kv_rows(start, end, M, bad);
+    if (r.n > 0 && r.begin < limit) {
+        bad = true;
+        r.begin = 0;
+        r.n = 0;
+    }
+    return r;
+}
+
 // Total units cut into `parts` contiguous shares that differ by one at most.
 struct Shares {
     long long q;          // total / parts
