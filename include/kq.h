@@ -314,7 +314,7 @@ typedef struct kq_attn {
     const int32_t *q_start;     /* prefill: [n_seqs + 1] first row of each sequence; decode: unused */
     int window;                 /* keys that a row sees, its own among them; 0: all */
     int sinks;                  /* first positions visible besides the window; 0 without a window */
-    float scale;                /* 0: 1 / sqrt(head_dim) */
+    float scale;                /* up to 1e24; 0: 1 / sqrt(head_dim) */
 } kq_attn;
 /* One new token per sequence: row s is sequence s at position kv_len[s] - 1 (M = n_seqs).  The keys
  * of all sequences are split evenly over the GPU and the parts joined in the same launch, in a

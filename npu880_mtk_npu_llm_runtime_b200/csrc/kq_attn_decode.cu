@@ -307,7 +307,7 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
                 }
                 // s[0], s[1]: key g, rows 2t, 2t+1; s[2], s[3]: key g+8
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] = (e < 2 ? k0 : k1) ? s[e] * p.scale_log2 : -INFINITY;
+                for (int e = 0; e < 4; ++e) s[e] = (e < 2 ? k0 : k1) ? __fmul_rn(s[e], p.scale_log2) : -INFINITY;
                 float al[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {

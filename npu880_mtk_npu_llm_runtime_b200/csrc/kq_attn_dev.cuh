@@ -62,7 +62,7 @@ __device__ __noinline__ void attn_row(const KvView &c, int seq, int kv_head, KvS
                     s = fmaf(a.x, b.x, fmaf(a.y, b.y, s));
                 }
             }
-            s *= scale;
+            s = __fmul_rn(s, scale);  // (one value: contracted into s - top below, large scores would not cancel)
         }
         const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
         seen |= there != 0;

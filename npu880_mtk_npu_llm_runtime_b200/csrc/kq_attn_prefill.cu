@@ -42,6 +42,10 @@ namespace {
 
 constexpr float kBias = 4.0f;  // weights reach 2^(kBias + kLag) < 65504: fp16's relative precision reaches further down
 constexpr float kLag = 8.0f;
+// The weights' exponents are one multiply-add from the scores, x scale - m in a single rounding, but m is a
+// rounded product itself: past 2^20 it is more than 1/16 off, from 2^28 on by more than fp16 holds.  Rows whose
+// maximum was ever larger are computed again key by key, where score and maximum are the same product.
+constexpr float kCoarse = 1048576.0f;
 constexpr int kThreads = 384;  // 8 softmax warps, MMA, K and Q loads, V loads, one idle
 constexpr int kWarpMma = 8, kWarpK = 9, kWarpV = 10;
 constexpr int kSortTiles = 512;
@@ -711,8 +715,8 @@ __device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, con
 
 // Rows of a warp whose plain result does not stand: computed key by key, over exactly their own
 // keys.  These see nothing (zeros), or have a value that is not finite: a weight of 0 times an
-// infinity that only other rows see is NaN in the matrix product; or a page is missing.  (A row whose
-// sum is NaN saw a NaN score: all NaN, which stands.)
+// infinity that only other rows see is NaN in the matrix product; or a page is missing; or their scores
+// are too large (kCoarse).  (Another row whose sum is NaN saw a NaN score: all NaN, which stands.)
 template <int D>
 __device__ __forceinline__ void mend_rows(const PrefillParams &p, Shared &sh, const Segment &s, bool odd, int tok, int head,
                                           int lane) {
@@ -792,6 +796,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
             const int b0 = s.b0, b1 = s.b1;
             const KvBlocks blocks = s.blocks;
             float m = -INFINITY, l = 0.0f;
+            bool coarse = false;  // see kCoarse
             for (int i = b0; i < b1; ++i) {
                 const int slot = NT == 2 ? t : (i - b0) & 1;
                 const uint32_t s_base = lane_base + slot * C::S_COL;
@@ -826,6 +831,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                 const bool raise = top > m + kLag;  // the first score above -inf raises from -inf
                 if (__any_sync(0xffffffffu, raise)) {
                     const float to = raise ? top : m;
+                    coarse |= raise && fabsf(top) > kCoarse;
                     const float alpha = m == to ? 1.0f : exp2_fast(m - to);
                     l *= alpha;
                     m = to;
@@ -885,7 +891,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                     wait_ld();
                     put32(o, 1.0f / l, out + 32 * c, mine, p.wide, odd);
                 }
-                mend_rows<D>(p, sh, s, mine && (bad || m == -INFINITY || (l == l && !(odd.x + odd.y == 0.0f))), tok, head, lane);
+                mend_rows<D>(p, sh, s, mine && (bad || coarse || m == -INFINITY || (l == l && !(odd.x + odd.y == 0.0f))), tok, head, lane);
             } else {
                 // this CTA's part: [value / 4][row][4], then (m, l) of each row
                 float4 *part = reinterpret_cast<float4 *>(a.parts + (size_t)(2 * blockIdx.x + (b0 == 0)) * part_rows * (D + 2)) + t * 128 + r;
@@ -898,7 +904,7 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                     for (int e = 0; e < 8; ++e)
                         if (mine) part[(8 * c + e) * part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
-                reinterpret_cast<float2 *>(part - (t * 128 + r) + D / 4 * part_rows)[t * 128 + r] = make_float2(bad ? NAN : m, l);  // NaN: a page is missing
+                reinterpret_cast<float2 *>(part - (t * 128 + r) + D / 4 * part_rows)[t * 128 + r] = make_float2(bad || coarse ? NAN : m, l);  // NaN: to be computed again
             }
         }
         if (!whole) {

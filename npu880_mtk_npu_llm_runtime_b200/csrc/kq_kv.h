@@ -293,8 +293,9 @@ inline int check_attn(const kq_kv_cache *c, const kq_attn *a, bool prefill, cons
         *why = "window and sinks must not be negative, and sinks needs a window";
         return KQ_ERR_INVALID_ARGUMENT;
     }
-    if (!(a->scale >= 0.0f) || a->scale > 1e30f) {
-        *why = "scale must be 0 or a positive finite number";
+    // (256 products of fp16's largest values stay below fp32's with it, so no finite score is lost)
+    if (!(a->scale >= 0.0f) || a->scale > 1e24f) {
+        *why = "scale must be 0 or a positive number up to 1e24";
         return KQ_ERR_INVALID_ARGUMENT;
     }
     return KQ_OK;

@@ -9,6 +9,7 @@ import subprocess
 import pytest
 
 from conftest import ROOT
+from test_attn_host import INVALID, attn_struct, cache_struct
 
 SOURCE = r'''
 #include "npu880_mtk_npu_llm_runtime_b200/csrc/kq_kv.h"
@@ -17,6 +18,7 @@ extern "C" {
 int rows(int start, int end, int M, int *begin) { bool b = false; KvRows r = kv_rows(start, end, M, b); *begin = r.begin; return r.n; }
 int rows_behind(int start, int end, int M, int limit, int *begin, int *bad) {
     bool b = false; KvRows r = kv_rows_behind(start, end, M, limit, b); *begin = r.begin; *bad = b; return r.n; }
+int c_attn(const kq_kv_cache *c, const kq_attn *a, int prefill) { const char *w; return check_attn(c, a, prefill != 0, &w); }
 }
 '''
 
@@ -63,3 +65,11 @@ def test_row_ranges_never_overlap(host):
         assert not wrong and got == [(a, b - a) for a, b in zip(q_start, q_start[1:])]
     assert ranges(host, [0, 20, 10, 30], 30)[0] == [(0, 20), (0, 0), (0, 0)]
     assert ranges(host, [5, 3, 10, 12], 30)[0] == [(0, 0), (3, 7), (10, 2)]
+
+
+@pytest.mark.parametrize("scale, status", [(0.0, 0), (-0.0, 0), (1e-40, 0), (1e24, 0), (1.1e24, INVALID), (1e30, INVALID)])
+def test_scales(host, scale, status):
+    """the largest scale keeps every finite score below fp32's largest number: 256 * 65504^2 * 1e24 / ln 2"""
+    assert 256 * 65504.0 ** 2 * 1e24 * 1.4427 < 3.4e38
+    for prefill in (0, 1):
+        assert host.c_attn(C.byref(cache_struct()), C.byref(attn_struct(scale=scale)), prefill) == status

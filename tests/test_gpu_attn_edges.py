@@ -44,3 +44,52 @@ def test_prefill_row_ranges_that_overlap(kqctx, D, H, starts):
     kqctx.attn_prefill_async(a)
     kqctx.synchronize()                                   # the context stays usable
     assert (out.cpu().numpy() == got).all()
+
+
+@pytest.mark.parametrize("D, G, scale, terms", [(64, 2, 0.0, 64), (128, 4, 0.0, 128), (256, 2, 0.0, 256), (128, 4, 0.0, 1), (128, 16, 1e24, 1), (64, 1, 1e24, 64)])
+@pytest.mark.parametrize("seqs", [[(70, 70), (3, 200)], [(300, 300)], [(9, 9000)]])
+def test_very_large_scores(kqctx, D, G, scale, terms, seqs):
+    """scores of up to 2^32 and more whose maxima stand far above the rest: the weights are 1 and 0, so the result is
+    the value of the key with the largest score.  (Equal products make a score: fp32's roundings are far below the
+    steps between scores.)  The weight of the maximum need not be a power of two (the reference m may be a little off it) and so has a rounding to fp16 that
+    the sum of the weights has not, and the result has one: half a step each, and a few of fp32's."""
+    rng = np.random.default_rng(D + G)
+    lens = [n for _, n in seqs]
+    p = R.Paged(rng, lens, 1, 16, D)
+    starts = np.cumsum([0] + [r for r, _ in seqs]).astype(np.int32)
+    q = np.zeros((starts[-1], G, D), np.float16)
+    q[:, :, :terms] = rng.choice([-60000, -3000, 3000, 60000], q.shape[:2])[..., None]
+    for s, n in enumerate(lens):
+        p.keys[s][:] = 0
+        p.keys[s][:, 0, :terms] = (rng.permutation(n) * (8 if n > 4000 else 32) - 32 * (n // 8))[:, None]
+        for j in range(n):
+            p.k[p.table[s, j // 16], :, j % 16] = p.keys[s][j]
+    assert len(np.unique(p.keys[0][:, 0, 0])) == lens[0] or lens[0] > 4000
+    kv_len = dev(np.array(lens, np.int32))
+    o1, o2 = dev(np.full_like(q, SENTINEL)), dev(np.full_like(q[:len(lens)], SENTINEL))
+    cache = cache_of(p)
+    prompt = kq.Attention(cache, dev(q), o1, kv_len, q_start=dev(starts), scale=scale)   # (lives until they ended)
+    token = kq.Attention(cache, dev(q[starts[1:] - 1]), o2, kv_len, scale=scale)
+    kqctx.attn_prefill_async(prompt)
+    kqctx.attn_decode_async(token)
+    kqctx.synchronize()
+    got, last = o1.cpu().numpy(), o2.cpu().numpy()
+    checked = 0
+
+    def close_to(x, v):
+        v = v.astype(np.float64)
+        return (np.abs(x.astype(np.float64) - v) <= np.abs(v) * (2 * R.HALF16 + 16 * R.U32) + R.TINY16).all()
+
+    for s, (r, n) in enumerate(seqs):
+        for i in range(r):
+            e = p.keys[s][:n - r + i + 1, 0, 0].astype(np.float64)
+            for g in range(G):
+                score = e * float(q[starts[s] + i, g, 0])
+                at = np.flatnonzero(score == score.max())
+                if len(at) > 1:                           # (fp16 holds no 9,000 such numbers: a tie tells nothing)
+                    continue
+                checked += 1
+                assert close_to(got[starts[s] + i, g], p.values[s][at[0], 0]), (s, i, g)
+                if i == r - 1:
+                    assert close_to(last[s, g], p.values[s][at[0], 0]), (s, g)
+    assert checked > 4
