@@ -149,7 +149,7 @@ struct Joint {
     __device__ __forceinline__ uint2 result() const {
         if (!seen && L == L) return make_uint2(0u, 0u);
         const float inv = 1.0f / L;
-        return make_uint2(f2_to_h2(v.x * inv, v.y * inv), f2_to_h2(v.z * inv, v.w * inv));
+        return make_uint2(mean_to_h2(v.x * inv, v.y * inv), mean_to_h2(v.z * inv, v.w * inv));
     }
 };
 
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
                     for (int c = 0; c < VC; ++c) {
                         uint32_t v[4];
 #pragma unroll
-                        for (int jj = 0; jj < 4; ++jj) v[jj] = f2_to_h2(o[b][4 * c + jj][e] * inv, o[b][4 * c + jj][e + 2] * inv);
+                        for (int jj = 0; jj < 4; ++jj) v[jj] = mean_to_h2(o[b][4 * c + jj][e] * inv, o[b][4 * c + jj][e + 2] * inv);
                         *reinterpret_cast<uint4 *>(a.out + it.seq * a.out_stride + (head0 + r) * D + 64 * c + 8 * g) =
                             make_uint4(v[0], v[1], v[2], v[3]);
                     }

@@ -12,6 +12,19 @@ __device__ __forceinline__ uint32_t f2_to_h2(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Two weighted means as fp16.  The weights of the sum of values were rounded to fp16 and those of the sum of weights
+// were not, so a mean of values near fp16's largest may lie up to 2^-11 beyond it: it stands for the largest, as no
+// mean is larger than its values.  (This form takes an infinity for the largest too; mean_to_h2 keeps it.)
+__device__ __forceinline__ uint32_t finite_mean_to_h2(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ uint32_t mean_to_h2(float a, float b) {
+    auto held = [](float x) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x; };
+    return f2_to_h2(held(a), held(b));
+}
+
 // One more arrival at a counter other CTAs count on too: releases this thread's (and, after a barrier,
 // its CTA's) writes, acquires those of the arrivals before it, whose number it returns.
 __device__ __forceinline__ unsigned count_arrival(unsigned *count) {
@@ -106,7 +119,7 @@ __device__ __noinline__ void attn_row(const KvView &c, int seq, int kv_head, KvS
     const float inv = seen ? 1.0f / sum : 0.0f;  // scores all -inf: 0 / 0, NaN as in the formula
 #pragma unroll
     for (int i = 0; i < W; ++i)
-        reinterpret_cast<uint32_t *>(out)[lane * W + i] = seen ? f2_to_h2(acc[i].x * inv, acc[i].y * inv) : 0u;
+        reinterpret_cast<uint32_t *>(out)[lane * W + i] = seen ? mean_to_h2(acc[i].x * inv, acc[i].y * inv) : 0u;
 }
 
 }  // namespace kq

@@ -736,7 +736,7 @@ __device__ __forceinline__ void mend_rows(const PrefillParams &p, Shared &sh, co
 }
 
 // 32 values of a row, times `by`, rounded, to out (where `write`).  `odd` turns NaN when one is not
-// finite (0 times it is NaN).  With rows that allow it 32 bytes a store: a warp's lanes write to 32
+// finite (0 times it is NaN); such a row is computed again, so its infinities need not be kept here.  With rows that allow it 32 bytes a store: a warp's lanes write to 32
 // rows, so a 16-byte store would fill half a sector at each.
 __device__ __forceinline__ void put32(const float *o, float by, uint16_t *out, bool write, bool wide, float2 &odd) {
     uint32_t h[16];
@@ -745,7 +745,7 @@ __device__ __forceinline__ void put32(const float *o, float by, uint16_t *out, b
     for (int e = 0; e < 16; ++e) {
         const float2 v = __fmul2_rn(make_float2(o[2 * e], o[2 * e + 1]), by2);
         odd = __ffma2_rn(v, zero, odd);
-        h[e] = f2_to_h2(v.x, v.y);
+        h[e] = finite_mean_to_h2(v.x, v.y);
     }
     if (!write) return;
     if (wide) {

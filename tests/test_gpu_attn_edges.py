@@ -93,3 +93,38 @@ def test_very_large_scores(kqctx, D, G, scale, terms, seqs):
                 if i == r - 1:
                     assert close_to(last[s, g], p.values[s][at[0], 0]), (s, g)
     assert checked > 4
+
+
+@pytest.mark.parametrize("D, G", [(64, 2), (128, 4), (256, 1), (128, 16)])
+@pytest.mark.parametrize("seqs", [[(90, 90), (2, 300)], [(300, 300)], [(9, 9000)]])
+def test_means_of_the_largest_values(kqctx, D, G, seqs):
+    """a weighted mean of 65504s is 65504: not an infinity, although every weight but one is rounded up by most of
+    half a step (they are 0.5 (1 + 1.2 2^-11) of the largest)"""
+    rng = np.random.default_rng(D + G)
+    lens = [n for _, n in seqs]
+    p = R.Paged(rng, lens, 1, 32, D)
+    starts = np.cumsum([0] + [r for r, _ in seqs]).astype(np.int32)
+    score = np.log(0.5 * (1 + 1.2 * 2.0 ** -11))
+    coarse = np.float16(score)
+    fine = np.float16((score - float(coarse)) * 1024)
+    q = np.zeros((starts[-1], G, D), np.float16)
+    q[:, :, 0], q[:, :, 1] = 1, 2.0 ** -10
+    for s, n in enumerate(lens):
+        p.keys[s][:] = 0
+        p.keys[s][1:, 0, 0], p.keys[s][1:, 0, 1] = coarse, fine
+        p.values[s][:, :, ::2], p.values[s][:, :, 1::2] = 65504, -65504
+        for j in range(n):
+            p.k[p.table[s, j // 32], :, j % 32] = p.keys[s][j]
+            p.v[p.table[s, j // 32], :, j % 32] = p.values[s][j]
+    cache, kv_len = cache_of(p), dev(np.array(lens, np.int32))
+    o1, o2 = dev(np.full_like(q, SENTINEL)), dev(np.full_like(q[:len(lens)], SENTINEL))
+    prompt = kq.Attention(cache, dev(q), o1, kv_len, q_start=dev(starts), scale=1.0)
+    token = kq.Attention(cache, dev(q[starts[1:] - 1]), o2, kv_len, scale=1.0)
+    kqctx.attn_prefill_async(prompt)
+    kqctx.attn_decode_async(token)
+    kqctx.synchronize()
+    rows = [(starts[s] + i, s, n - r + i, n) for s, (r, n) in enumerate(seqs) for i in {0, r // 2, r - 1}]
+    want, tol = R.expect(p, q, rows, 0, 0, scale=1.0)
+    close(o1.cpu().numpy()[[r[0] for r in rows]], want, tol)
+    want, tol = R.expect(p, q, [(starts[s + 1] - 1, s, n - 1, n) for s, n in enumerate(lens)], 0, 0, scale=1.0)
+    close(o2.cpu().numpy(), want, tol)
