@@ -37,6 +37,7 @@ namespace {
 // Weights reach 2^kBias: their fp16 rounding (11 bits, for the second product) then stays relative
 // down to 2^-22 of the largest instead of 2^-14; sums stay fp32.
 constexpr float kBias = 8.0f;
+constexpr float kLeastHalf = 5.9604645e-8f;  // fp16's smallest number: weights for the second product, as kLeast
 constexpr int kUnit = 16;  // keys of a unit; a page holds a multiple of it
 // Beginning an item (its queries, its first page) costs a warp about as much as this many units:
 // every item counts that many more when the work is cut, or the warps with the short sequences
@@ -132,8 +133,8 @@ struct Joint {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     __device__ __forceinline__ void add(float2 ml, float4 x) {
         const float top = fmaxf(M, ml.x);
-        const float old = M == -INFINITY ? 1.0f : exp2f(M - top);  // before the first score: L is 0 or NaN, v is 0
-        const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
+        const float old = M == -INFINITY ? 1.0f : at_least(exp2f(M - top), kLeast);  // before the first score: L is 0 or NaN, v is 0
+        const float w = ml.x == -INFINITY ? 0.0f : at_least(exp2f(ml.x - top), kLeast);
         L = L * old + (ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.0f) : w * ml.y);
         v.x = v.x * old + w * x.x;
         v.y = v.y * old + w * x.y;
@@ -313,11 +314,12 @@ __global__ __launch_bounds__(Cfg<D, NB>::THREADS, 1) void kq_attn_decode(const _
                 for (int e = 0; e < 2; ++e) {
                     const float mn = fmaxf(m[b][e], max_over_keys(fmaxf(s[e], s[e + 2])));
                     const float ref = (mn == -INFINITY) ? 0.0f : mn;
-                    al[e] = exp2f(m[b][e] - ref);
+                    al[e] = at_least(exp2f(m[b][e] - ref), kLeast);
                     m[b][e] = mn;
-                    s[e] = exp2f(s[e] - ref + kBias);
-                    s[e + 2] = exp2f(s[e + 2] - ref + kBias);
-                    l[b][e] = l[b][e] * al[e] + (s[e] + s[e + 2]);
+                    const float w0 = exp2f(s[e] - ref + kBias), w1 = exp2f(s[e + 2] - ref + kBias);
+                    l[b][e] = l[b][e] * al[e] + (w0 + w1);
+                    s[e] = s[e] == -INFINITY ? 0.0f : at_least(w0, kLeastHalf);
+                    s[e + 2] = s[e + 2] == -INFINITY ? 0.0f : at_least(w1, kLeastHalf);
                 }
                 if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
 #pragma unroll

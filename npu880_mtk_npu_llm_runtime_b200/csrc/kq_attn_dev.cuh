@@ -25,6 +25,12 @@ __device__ __forceinline__ uint32_t mean_to_h2(float a, float b) {
     return f2_to_h2(held(a), held(b));
 }
 
+// No weight, and no factor of what was summed before, is less than this: a value that is infinite stays so under
+// a weight that would vanish (0 times it is NaN), and to finite ones it adds nothing that fp32 holds.  (A score
+// of -inf has the weight 0; NaN stays.)
+constexpr float kLeast = 1.17549435e-38f;  // fp32's smallest normal number
+__device__ __forceinline__ float at_least(float w, float least) { return w < least ? least : w; }
+
 // One more arrival at a counter other CTAs count on too: releases this thread's (and, after a barrier,
 // its CTA's) writes, acquires those of the arrivals before it, whose number it returns.
 __device__ __forceinline__ unsigned count_arrival(unsigned *count) {
@@ -84,8 +90,8 @@ __device__ __noinline__ void attn_row(const KvView &c, int seq, int kv_head, KvS
         for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         top = fmaxf(m, top);
         // before the first score above -inf there is nothing to rescale; a NaN score stays NaN
-        const float old = (m == -INFINITY) ? 1.0f : __expf(m - top);
-        const float w = (at < 0 || s == -INFINITY) ? 0.0f : __expf(s - top);
+        const float old = (m == -INFINITY) ? 1.0f : at_least(__expf(m - top), kLeast);
+        const float w = (at < 0 || s == -INFINITY) ? 0.0f : at_least(__expf(s - top), kLeast);
         m = top;
         sum = sum * old + w;
 #pragma unroll

@@ -128,3 +128,49 @@ def test_means_of_the_largest_values(kqctx, D, G, seqs):
     close(o1.cpu().numpy()[[r[0] for r in rows]], want, tol)
     want, tol = R.expect(p, q, [(starts[s + 1] - 1, s, n - 1, n) for s, n in enumerate(lens)], 0, 0, scale=1.0)
     close(o2.cpu().numpy(), want, tol)
+
+
+@pytest.mark.parametrize("D, G", [(64, 2), (128, 4), (256, 1), (128, 16)])
+@pytest.mark.parametrize("n, new", [(40, 40), (300, 3), (9000, 9)])
+@pytest.mark.parametrize("gap", [30, 45, 140, 300, 900])
+def test_infinite_values_under_vanishing_weights(kqctx, D, G, n, new, gap):
+    """a weight of 2^-gap of the largest is no zero: an infinite value under it is infinite, before the largest
+    score and behind it, one of each sign is NaN; under a score of -inf it is NaN, as 0 times infinity"""
+    rng = np.random.default_rng(D + G + n)
+    p = R.Paged(rng, [n], 1, 16, D)
+    q = np.zeros((new, G, D), np.float16)
+    q[:, :, 0] = 1
+    top = min(n - new, n // 2)                             # every row sees the largest score (row 0 of a prompt: only that)
+    places = [(0, 1, np.inf), (min(top + 1, n - 1), 2, -np.inf), (n - 1, 3, np.inf), (0, 4, np.inf), (n - 1, 4, -np.inf)]
+    p.keys[0][:, 0] = 0
+    p.keys[0][:, 0, 0] = -gap * np.log(2)
+    p.keys[0][top, 0, 0] = 0
+    zero = n // 3 if n // 3 not in (0, top, top + 1, n - 1) else n // 3 + 2
+    p.keys[0][zero, 0, 0] = -np.inf
+    p.values[0][zero, 0, 5] = np.inf
+    for j, d, x in places:
+        p.values[0][j, 0, d] = x
+    for j in range(n):
+        p.k[p.table[0, j // 16], :, j % 16] = p.keys[0][j]
+        p.v[p.table[0, j // 16], :, j % 16] = p.values[0][j]
+    cache, kv_len = cache_of(p), i32(n)
+    o1, o2 = dev(np.full_like(q, SENTINEL)), dev(np.full_like(q[:1], SENTINEL))
+    prompt = kq.Attention(cache, dev(q), o1, kv_len, q_start=i32(0, new), scale=1.0)
+    token = kq.Attention(cache, dev(q[:1]), o2, kv_len, scale=1.0)
+    kqctx.attn_prefill_async(prompt)
+    kqctx.attn_decode_async(token)
+    kqctx.synchronize()
+    for got, i in [(o1.cpu().numpy()[i], i) for i in sorted({0, new // 2, new - 1})] + [(o2.cpu().numpy()[0], new - 1)]:
+        seen = n - new + i + 1
+        e = p.keys[0][:seen, 0, 0].astype(np.float64)
+        with np.errstate(invalid="ignore"):
+            w = np.exp(e - e.max())
+            want = (w[:, None] * p.values[0][:seen, 0].astype(np.float64)).sum(0) / w.sum()
+        odd = ~np.isfinite(want)
+        assert odd[1] and (i < new - 1 or odd[[1, 2, 3, 4, 5]].all())
+        for g in range(G):
+            assert np.array_equal(got[g][odd].astype(np.float64), want[odd], equal_nan=True), (i, got[g][:6], want[:6])
+            # the rest: bounded as any row's, the weights' 16 bits and the few below them (2^-29 of the largest)
+            W = (w[:, None] * np.abs(p.values[0][:seen, 0][:, ~odd].astype(np.float64))).sum(0) / w.sum()
+            off = np.abs(got[g][~odd].astype(np.float64) - want[~odd])
+            assert (off <= R.HALF16 * (np.abs(want[~odd]) + W) + 2 * R.U32 * (seen + 64) * W + seen * 2.0 ** -29 * 8 + R.TINY16).all()
