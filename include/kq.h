@@ -222,7 +222,10 @@ int kq_run_ffn_async(kq_ctx *ctx, const kq_weight *gate, const kq_weight *up, co
  * position rotation, the append to a paged key-value cache, and attention over that cache -- of one
  * new token per sequence (decode) or of ragged prompt rows (prefill).  fp16 in and out; sums,
  * softmax statistics and norms in fp32, rotation angles reduced in fp64, one rounding to fp16 of
- * each result.  DEVICE pointers, enqueued on the context's stream; all buffers belong to the caller
+ * each result.  The attention weights that multiply the values are rounded to fp16 as well: each by
+ * half a step (2^-11 of it) or by 2^-32 (prefill) or 2^-40 (decode) of the row's largest weight,
+ * whichever is more; their sum is taken before.  A value that is infinite reaches every row that sees
+ * it, however small its weight (0 under a score of -inf).  DEVICE pointers, enqueued on the context's stream; all buffers belong to the caller
  * and to the context's device.  No counterpart on the reference's matmul path: its attention is
  * ENG:7787-7915 (QK-norm, RoPE, active-window GQA).
  *

@@ -34,9 +34,10 @@ namespace kq {
 
 namespace {
 
-// Weights reach 2^kBias: their fp16 rounding (11 bits, for the second product) then stays relative
-// down to 2^-22 of the largest instead of 2^-14; sums stay fp32.
-constexpr float kBias = 8.0f;
+// The weights are rounded to fp16, the type of the values, for the second product; all sums, that of the weights
+// too, stay fp32 (32-bit weights would need a second product of their low parts).  They reach 2^kBias, as much as
+// fp16 holds: the rounding is half a step (2^-11) down to 2^-29 of the largest weight, and 2^-40 of it below.
+constexpr float kBias = 15.0f;
 constexpr float kLeastHalf = 5.9604645e-8f;  // fp16's smallest number: weights for the second product, as kLeast
 constexpr int kUnit = 16;  // keys of a unit; a page holds a multiple of it
 // Beginning an item (its queries, its first page) costs a warp about as much as this many units:

@@ -40,7 +40,10 @@ namespace kq {
 
 namespace {
 
-constexpr float kBias = 4.0f;  // weights reach 2^(kBias + kLag) < 65504: fp16's relative precision reaches further down
+// The weights are rounded to fp16, the type of the values, for the second product (fp32 sums).  They reach
+// 2^(kBias + kLag), as much as fp16 holds: the rounding is half a step (2^-11) down to 2^-21 of the row's largest
+// weight, and 2^-32 of it below.
+constexpr float kBias = 7.0f;
 constexpr float kLag = 8.0f;
 // The weights' exponents are one multiply-add from the scores, x scale - m in a single rounding, but m is a
 // rounded product itself: past 2^20 it is more than 1/16 off, from 2^28 on by more than fp16 holds.  Rows whose

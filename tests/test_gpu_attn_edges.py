@@ -174,3 +174,35 @@ def test_infinite_values_under_vanishing_weights(kqctx, D, G, n, new, gap):
             W = (w[:, None] * np.abs(p.values[0][:seen, 0][:, ~odd].astype(np.float64))).sum(0) / w.sum()
             off = np.abs(got[g][~odd].astype(np.float64) - want[~odd])
             assert (off <= R.HALF16 * (np.abs(want[~odd]) + W) + 2 * R.U32 * (seen + 64) * W + seen * 2.0 ** -29 * 8 + R.TINY16).all()
+
+
+@pytest.mark.parametrize("prefill", [True, False])
+def test_many_small_weights(kqctx, prefill):
+    """a million keys of weight 2^-30.3 behind the first: each weight is off by half a step of fp16 or 2^-32 of the
+    largest (decode: 2^-40), and so is the mean of values of one size, times their number.  As many sequences as
+    SMs, on the same two pages, so that no item is split and its largest weight is everywhere the same."""
+    import torch
+    D, n, S, page = 64, 1 << 20, torch.cuda.get_device_properties(0).multi_processor_count, 256
+    table = np.zeros((S, n // page), np.int32)
+    table[:, 0] = 1
+    k, v = np.zeros((2, 1, page, D), np.float16), np.ones((2, 1, page, D), np.float16)
+    k[:, :, :, 0] = -30.3 * np.log(2)
+    k[1, 0, 0] = 0
+    v[1, 0, 0] = 0
+    cache = kq.KvCache(dev(k), dev(v), dev(table))
+    q = np.zeros((S, 1, D), np.float16)
+    q[:, :, 0] = 1
+    out = dev(np.full_like(q, SENTINEL))
+    a = kq.Attention(cache, dev(q), out, dev(np.full(S, n, np.int32)), q_start=dev(np.arange(S + 1, dtype=np.int32)) if prefill else None,
+                     scale=1.0)
+    (kqctx.attn_prefill_async if prefill else kqctx.attn_decode_async)(a)
+    kqctx.synchronize()
+    w = np.exp(float(k[0, 0, 0, 0])) * (n - 1)
+    want = w / (1 + w)
+    # fp32: the score's product and the exponential (8 half steps), sums of n / 16 terms that grow evenly
+    tol = want * (2 * R.HALF16 + U32_SUM) + n * 2.0 ** (-32 if prefill else -40)
+    off = np.abs(out.cpu().numpy().astype(np.float64) - want)
+    assert off.max() <= tol, (off.max(), tol, want)
+
+
+U32_SUM = (8 + (1 << 16)) * 2 * R.U32                      # a rounding (a step) for every 16 of the million keys
