@@ -450,7 +450,10 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
     // Whole items in snake order, unless the fullest CTA would get more than an even share and a join.
     const int G = gridDim.x, items = tiles * heads;
     const Shares even(total > 0 ? total : 1, G);
-    bool whole = items >= 32 * G, ordered = false;  // (so many that the order evens out)
+    // Without a look at the order where there are many items, short enough that no CTA can get more than twice an even
+    // share (the look costs 3 us of 120 for 4,800 items of a block).  A long item among them: one sequence of 131,072
+    // keys and 600 of 100 take 330 us in equal shares, whole 1,650.
+    bool whole = items >= 32 * G && (long long)((items + G - 1) / G) * most <= 2 * even.q, ordered = false;
     if (!whole && most <= even.q + kJoinBlocks) {
         // longest first: from the last tile on where no tile is longer than the next (one prompt), else by rank
         bool rising = true;

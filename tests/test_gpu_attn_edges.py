@@ -206,3 +206,47 @@ def test_many_small_weights(kqctx, prefill):
 
 
 U32_SUM = (8 + (1 << 16)) * 2 * R.U32                      # a rounding (a step) for every 16 of the million keys
+
+
+def test_one_long_sequence_among_many_short_ones(kqctx):
+    """hundreds of one-token sequences and one of 131,072 keys: the long one's keys are spread over the GPU, so that
+    the batch takes no longer than its parts apart (a CTA that took a whole head of it took 11 times as long)"""
+    import torch
+    rng = np.random.default_rng(21)
+    D, H, K, page, long, short = 128, 32, 8, 64, 131072, 100
+    lens = [long] + [short] * 600
+    need = [-(-n // page) for n in lens]
+    table = np.zeros((len(lens), max(need)), np.int32)
+    at = np.cumsum([0] + need)
+    for s, n in enumerate(need):
+        table[s, :n] = np.arange(at[s], at[s] + n)
+    k, v = (torch.empty((at[-1], K, page, D), dtype=torch.float16, device="cuda").normal_() for _ in range(2))
+    q = dev(rng.standard_normal((len(lens), H, D)).astype(np.float16))
+    out = torch.full_like(q, SENTINEL)
+
+    def call(pick):
+        a = kq.Attention(kq.KvCache(k, v, dev(table[pick])), q[pick[0]:pick[-1] + 1], out[pick[0]:pick[-1] + 1],
+                         dev(np.array(lens, np.int32)[pick]), q_start=dev(np.arange(len(pick) + 1, dtype=np.int32)))
+        torch.cuda.synchronize()
+        best, stream = 1e9, torch.cuda.ExternalStream(kqctx.stream)
+        for _ in range(5):
+            e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            e[0].record(stream)
+            for _ in range(4):
+                kqctx.attn_prefill_async(a)
+            e[1].record(stream)
+            kqctx.synchronize()
+            best = min(best, e[0].elapsed_time(e[1]))
+        return best
+
+    alone = call(np.arange(1)) + call(np.arange(1, len(lens)))
+    together = call(np.arange(len(lens)))
+    assert together < 3 * alone, (together, alone)
+    got = out.cpu().numpy()
+    p = R.Paged(rng, [0] * len(lens), K, page, D)
+    rows = [0, 1, 77, 600]
+    for s in rows:
+        t = table[s, :need[s]]
+        p.keys[s], p.values[s] = (x[torch.from_numpy(t).long().cuda()].permute(0, 2, 1, 3).reshape(-1, K, D)[:lens[s]].cpu().numpy() for x in (k, v))
+    want, tol = R.expect(p, q.cpu().numpy(), [(s, s, lens[s] - 1, lens[s]) for s in rows], 0, 0)
+    close(got[rows], want, tol)
