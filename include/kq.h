@@ -81,7 +81,8 @@ const char *kq_last_error(const kq_ctx *ctx);
  * "timeout_ms" / "timeout_us" -- limit of every device-side wait (default 1000 ms);
  * "inject_timeout" -- failure-path test: matrix-product and prefill attention kernels first wait on a
  * barrier that nothing completes, so the wait runs out, the kernel returns early and the call reports
- * KQ_ERR_TIMEOUT (default 0);
+ * KQ_ERR_TIMEOUT (default 0; 2 lets prefill attention fail on every other CTA only, so that the others
+ * leave counts behind that the next call has to clear);
  * "gemm_path" -- products of more than 8 activation rows: 0 chooses by a cost model, 1 always
  * the weight-row-major tensor-core kernel (tcgen05; weight rows as the MMA's A operand), 2 always
  * the GEMV kernel in tiles of 8 rows, 3 always the token-major tensor-core kernel (activation

@@ -37,7 +37,7 @@ struct kq_ctx {
     bool pdl = true;
     float *exp_tab = nullptr;    // SwiGLU: expf(-g) for every fp16 g, from this host's C library
     bool swiglu_gpu_exp = false; // option "swiglu_exp" = 1: exp in fp64 on the GPU instead
-    bool inject_timeout = false;  // test hook: GEMV consumers wait on a barrier nothing completes
+    int inject_timeout = 0;  // test hook: consumers wait on a barrier nothing completes (2: of odd CTAs)
     unsigned long long timeout_ns = 1000000000ull;
     std::string err;
 
@@ -542,7 +542,8 @@ extern "C" int kq_set_option(kq_ctx *c, const char *name, long long value) {
         return KQ_OK;
     }
     if (!strcmp(name, "inject_timeout")) {
-        c->inject_timeout = value != 0;
+        if (value < 0 || value > 2) return fail(c, KQ_ERR_INVALID_ARGUMENT, "inject_timeout must be 0, 1 or 2");
+        c->inject_timeout = (int)value;
         return KQ_OK;
     }
     if (!strcmp(name, "timeout_ms")) {
@@ -1189,7 +1190,7 @@ int attn_launch(kq_ctx *c, const kq_kv_cache *cache, const kq_attn *a, bool pref
     L.num_sms = c->num_sms;
     L.pdl = c->pdl;
     L.timeout_ns = c->timeout_ns;
-    L.inject = c->inject_timeout ? 1 : 0;
+    L.inject = c->inject_timeout;
     return KQ_OK;
 }
 

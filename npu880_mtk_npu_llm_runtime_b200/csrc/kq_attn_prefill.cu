@@ -83,7 +83,7 @@ struct PrefillParams {
     int box_rows;     // keys of one K/V box: the smaller of a page and a block
     int k_stages, v_stages;
     unsigned long long timeout_ns;
-    int inject;
+    int inject;       // 1: every CTA stops early; 2: those of odd index, so that the others' arrivals stay behind
     int wide;         // rows of out start at multiples of 32 bytes
 };
 
@@ -647,7 +647,7 @@ __device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, con
     constexpr uint32_t kStep = C::STAGE >> 4;
     Cursor ka, va;            // the rings' next blocks to read
     uint32_t np[2] = {0, 0};  // P's begun of each slot
-    if (p.inject && !wait(sh.never, 0)) return;
+    if (p.inject && (p.inject == 1 || (blockIdx.x & 1)) && !wait(sh.never, 0)) return;
     const uint32_t q_lo = desc_lo(q0, 16), k_lo = desc_lo(k_ring, 16), v_lo = desc_lo(v_ring, BN * 128);
     // S slot = Q tile t times the K block in ring stage st
     auto mma_s = [&](int t, int slot, uint32_t st) {

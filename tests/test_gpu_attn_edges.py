@@ -250,3 +250,67 @@ def test_one_long_sequence_among_many_short_ones(kqctx):
         p.keys[s], p.values[s] = (x[torch.from_numpy(t).long().cuda()].permute(0, 2, 1, 3).reshape(-1, K, D)[:lens[s]].cpu().numpy() for x in (k, v))
     want, tol = R.expect(p, q.cpu().numpy(), [(s, s, lens[s] - 1, lens[s]) for s in rows], 0, 0)
     close(got[rows], want, tol)
+
+
+@pytest.mark.parametrize("D, H, K, n, new", [(128, 8, 2, 20000, 20), (64, 16, 1, 26000, 16), (256, 4, 1, 9000, 9)])
+def test_counts_left_behind_by_a_call_that_stopped_early(kqctx, D, H, K, n, new):
+    """every other CTA stops early, so the rest have counted arrivals at shared items that never get complete: the
+    next call clears them, of either kind, and so does one after a capture that only recorded the clearing"""
+    import torch
+    rng = np.random.default_rng(D)
+    ctx, stream = kq.Context(0), torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    p = R.Paged(rng, [n], K, 64, D)
+    q = rng.standard_normal((new, H, D)).astype(np.float16)
+    out, o1, cache, kv_len = dev(np.zeros_like(q)), dev(np.zeros_like(q[:1])), cache_of(p), i32(n)
+    prompt = kq.Attention(cache, dev(q), out, kv_len, q_start=i32(0, new))
+    token = kq.Attention(cache, dev(q[-1:]), o1, kv_len)
+    want, tol = R.expect(p, q, [(i, 0, n - new + i, n) for i in range(new)], 0, 0)
+    other = dev((2 * p.v.astype(np.float32)).astype(np.float16))      # parts of other values lie in the scratch
+    before = kq.Attention(kq.KvCache(cache.k, other, cache.page_table), prompt.keep[0], out, kv_len, q_start=prompt.keep[3])
+
+    def stop():
+        ctx.attn_prefill_async(before)
+        ctx.set_option("timeout_ms", 20)
+        ctx.set_option("inject_timeout", 2)
+        ctx.attn_prefill_async(prompt)
+        with pytest.raises(kq.KQError) as e:
+            ctx.synchronize()
+        assert e.value.status == -7
+        ctx.set_option("inject_timeout", 0)
+        ctx.set_option("timeout_ms", 1000)
+
+    def check(call, prefill=True):
+        for t in (out, o1):
+            t.fill_(SENTINEL)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            call()
+        ctx.synchronize()
+        if prefill:
+            close(out.cpu().numpy(), want, tol)
+        else:
+            close(o1.cpu().numpy(), want[-1:], tol[-1:])
+
+    torch.cuda.synchronize()
+    try:
+        ctx.attn_prefill_async(prompt)
+        stop()
+        for _ in range(2):
+            check(lambda: ctx.attn_prefill_async(prompt))
+        stop()
+        for _ in range(2):
+            check(lambda: ctx.attn_decode_async(token), prefill=False)
+        check(lambda: ctx.attn_prefill_async(prompt))
+        stop()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            ctx.attn_prefill_async(prompt)
+        for call in (lambda: ctx.attn_prefill_async(prompt), g.replay, g.replay):
+            check(call)
+        del g, call
+        with pytest.raises(kq.KQError):
+            ctx.set_option("inject_timeout", 3)
+    finally:
+        torch.cuda.synchronize()
+        ctx.close()
