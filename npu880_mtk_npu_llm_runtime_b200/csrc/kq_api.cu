@@ -10,6 +10,7 @@
 #include "../../include/kq.h"
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -51,6 +52,7 @@ struct kq_ctx {
     bool gemv_split = true;
     bool gemv_half = true;  // Q4_K / Q5_K GEMV launches of 1-2 rows: 8-row halves per CTA where better
     bool ffn_fused = true;  // FFN blocks of 1-2 tokens as one persistent kernel where a plan exists
+    std::array<int, 10> block_sized{};  // the attention block whose scratch was last made sure of
     bool split_dirty = false;
     bool attn_dirty = false;  // an attention kernel that stopped early may have left arrival counts
     bool graph_holds_scratch = false;  // a call of this context was captured into a CUDA graph
@@ -117,6 +119,7 @@ int ensure(kq_ctx *c, DevBuf &b, size_t bytes) {
         cudaFree(b.p);
         b.p = nullptr;
         b.cap = 0;
+        c->block_sized = {};  // (should the allocation fail)
     }
     size_t want = std::max<size_t>(bytes, 4096);
     want = (want + 255) & ~(size_t)255;
@@ -184,23 +187,25 @@ int validate_mk(kq_ctx *c, int M, int K) {
 // 64 MB (very long Q8_0 rows).
 // The arrival counts of balanced launches (gemv_split_slots ints), then the two words of the fused
 // FFN kernel's grid barrier and its `extra` pair counts, all zero; cleared again after a launch
-// that stopped early.
-int split_counts(kq_ctx *c, size_t extra = 0) {
+// that stopped early.  size_only: memory, but nothing enqueued.
+int split_counts(kq_ctx *c, size_t extra = 0, bool size_only = false) {
     const size_t cb = sizeof(int) * ((size_t)kq::gemv_split_slots(c->num_sms) + 2 + extra);
-    if (!c->gcount.p || c->split_dirty || c->gcount.cap < cb) {
+    if (!c->gcount.p || c->gcount.cap < cb) {
         if (int r = ensure(c, c->gcount, cb)) return r;
-        KQ_CUDA(c, cudaMemsetAsync(c->gcount.p, 0, cb, c->stream));
-        c->split_dirty = false;
+        c->split_dirty = true;
     }
+    if (!c->split_dirty || size_only) return KQ_OK;
+    KQ_CUDA(c, cudaMemsetAsync(c->gcount.p, 0, cb, c->stream));
+    c->split_dirty = false;
     return KQ_OK;
 }
 
-int gemv_split_scratch(kq_ctx *c, int type, int K, int mt, kq::GemvLaunch &L) {
+int gemv_split_scratch(kq_ctx *c, int type, int K, int mt, kq::GemvLaunch &L, bool size_only) {
     if (!c->gemv_split) return KQ_OK;
     const size_t bytes = kq::gemv_split_bytes(type, K, mt, c->num_sms);
     if (bytes > ((size_t)64 << 20)) return KQ_OK;
     if (int r = ensure(c, c->gsplit, bytes)) return r;
-    if (int r = split_counts(c)) return r;
+    if (int r = split_counts(c, 0, size_only)) return r;
     L.split_terms = static_cast<float *>(c->gsplit.p);
     L.split_terms_bytes = c->gsplit.cap;
     L.split_count = static_cast<int *>(c->gcount.p);
@@ -216,6 +221,7 @@ struct GemvExtra {
     const uint32_t *out_ids = nullptr;     // tasks[0]: output column of local row r (device)
     bool no_pdl = false;                   // the weights were written by the previous kernel
     const kq::PeerOut *peer = nullptr;     // task 0's fp32 outputs also into every rank's gather buffer
+    bool size_only = false;                // allocate what the launches need, and launch nothing
 };
 
 int run_gemv(kq_ctx *c, const kq_task *tasks, int n, int M, int K, const __half *x, long long x_stride,
@@ -301,6 +307,7 @@ int run_gemv(kq_ctx *c, const kq_task *tasks, int n, int M, int K, const __half 
                     T.terms = c->tcterms.p;
                 }
             }
+            if (ex.size_only) continue;
             if (cudaError_t e = tc2 ? kq::launch_gemm_tc2(T, c->stream) : kq::launch_gemm_tc(T, c->stream))
                 return cuda_fail(c, e, "tensor-core gemm launch");
             continue;
@@ -349,7 +356,12 @@ int run_gemv(kq_ctx *c, const kq_task *tasks, int n, int M, int K, const __half 
             L.argmax_f16 = ex.argmax_f16;
             L.inject_wait = c->inject_timeout ? 1 : 0;
             if (ex.peer) L.peer = *ex.peer;
-            if (int r = gemv_split_scratch(c, type, K, mt, L)) return r;
+            if (ex.size_only) {  // (the largest tile, and the smaller ones that may stand in for it)
+                for (; mt > 0; --mt)
+                    if (int r = gemv_split_scratch(c, type, K, mt, L, true)) return r;
+                break;
+            }
+            if (int r = gemv_split_scratch(c, type, K, mt, L, false)) return r;
             L.half_ok = c->gemv_half;
             cudaError_t e = kq::launch_gemv(L, c->stream);
             if (e == cudaErrorInvalidConfiguration && mt > 1) {
@@ -1152,12 +1164,16 @@ struct OnDevice {
 };
 
 // Scratch of the attention kernels: one size for all shapes, so that it never grows after the first call.
-int attn_scratch(kq_ctx *c, kq::AttnLaunch &L) {
+int attn_memory(kq_ctx *c) {
     if (int r = ensure(c, c->attn_parts, std::max(kq::attn_decode_part_bytes(c->num_sms),
                                                             kq::attn_prefill_part_bytes(c->num_sms)))) return r;
-    const bool clear = !c->attn_count.p || c->attn_dirty;
-    if (int r = ensure(c, c->attn_count, sizeof(unsigned) * kq::attn_counts(c->num_sms))) return r;
-    if (clear) {
+    if (!c->attn_count.p) c->attn_dirty = true;
+    return ensure(c, c->attn_count, sizeof(unsigned) * kq::attn_counts(c->num_sms));
+}
+
+int attn_scratch(kq_ctx *c, kq::AttnLaunch &L) {
+    if (int r = attn_memory(c)) return r;
+    if (c->attn_dirty) {
         KQ_CUDA(c, cudaMemsetAsync(c->attn_count.p, 0, c->attn_count.cap, c->stream));
         // a capture has only recorded it: the counts stay as they are until the graph runs
         cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -1304,7 +1320,6 @@ extern "C" int kq_run_attn_async(kq_ctx *c, const kq_attn_layer *l, int M, const
     uint16_t *xn = reinterpret_cast<uint16_t *>(base), *qkv = reinterpret_cast<uint16_t *>(base + xnb);
     uint16_t *att = reinterpret_cast<uint16_t *>(base + xnb + qkvb);
     void *q8 = base + xnb + qkvb + ab, *q80 = base + xnb + qkvb + ab + q8b;
-    // every refusal before the first launch
     kq_heads hq{qkv, (size_t)rows, qkv, (size_t)rows, l->heads, l->q_gamma};
     kq_heads hk{qkv + qd, (size_t)rows, nullptr, 0, l->cache->kv_heads, l->k_gamma};
     kq_heads hv{qkv + qd + kd, (size_t)rows, nullptr, 0, l->cache->kv_heads, nullptr};
@@ -1312,10 +1327,7 @@ extern "C" int kq_run_attn_async(kq_ctx *c, const kq_attn_layer *l, int M, const
     if (int r = kq::check_append(l->cache, l->rope, M, seq, pos, &hq, &hk, &hv, &why)) return fail(c, r, "%s", why);
     if (int r = kq::check_attn(l->cache, &at, q_start != nullptr, &why)) return fail(c, r, "%s", why);
     if (!(l->eps >= 0.0f)) return fail(c, KQ_ERR_INVALID_ARGUMENT, "eps must not be negative");
-
-    KQ_CUDA(c, kq::launch_rmsnorm_q8k(x_in, l->gamma, xn, q8, M, hidden, c->stream, c->pdl));
     const bool any_q80 = l->q->type == KQ_TYPE_Q8_0 || l->k->type == KQ_TYPE_Q8_0 || l->v->type == KQ_TYPE_Q8_0;
-    if (any_q80) KQ_CUDA(c, kq::launch_quantize(KQ_TYPE_Q8_0, xn, hidden, M, hidden, q80, c->stream));
     kq_task t[3] = {};
     const kq_weight *w[3] = {l->q, l->k, l->v};
     const int at_row[3] = {0, qd, qd + kd};
@@ -1325,6 +1337,30 @@ extern "C" int kq_run_attn_async(kq_ctx *c, const kq_attn_layer *l, int M, const
         t[i].dst = qkv + at_row[i];
         t[i].dst_stride = rows;
     }
+    kq_task o{};
+    o.w = l->o;
+    o.rows = hidden;
+    o.dst = x_out;
+    o.dst_stride = hidden;
+    o.residual = x_in;
+    o.res_stride = hidden;
+    // All scratch before the first launch, so that a call that is refused for want of it (in a capture, or out of
+    // memory) has written nothing: after that only a launch itself can fail.
+    // (Scratch never shrinks, so what was sized for a block of the same shape still is.)
+    const __half *ax = reinterpret_cast<const __half *>(att);
+    const std::array<int, 10> shape = {M, hidden, qd, kd, (int)l->q->type, (int)l->k->type, (int)l->v->type,
+                                       (int)l->o->type, c->gemm_path, c->gemv_split};
+    if (shape != c->block_sized) {
+        GemvExtra size;
+        size.size_only = true;
+        if (int r = run_gemv(c, t, 3, M, hidden, nullptr, 0, q8, any_q80 ? q80 : nullptr, size)) return r;
+        if (int r = run_gemv(c, &o, 1, M, qd, ax, qd, nullptr, nullptr, size)) return r;
+        if (int r = attn_memory(c)) return r;
+        c->block_sized = shape;
+    }
+
+    KQ_CUDA(c, kq::launch_rmsnorm_q8k(x_in, l->gamma, xn, q8, M, hidden, c->stream, c->pdl));
+    if (any_q80) KQ_CUDA(c, kq::launch_quantize(KQ_TYPE_Q8_0, xn, hidden, M, hidden, q80, c->stream));
     if (int r = run_gemv(c, t, 3, M, hidden, nullptr, 0, q8, any_q80 ? q80 : nullptr)) return r;
     if (int r = kq_kv_append_async(c, l->cache, l->rope, M, seq, pos, &hq, &hk, &hv, l->eps)) return r;
     if (q_start) {
@@ -1334,14 +1370,7 @@ extern "C" int kq_run_attn_async(kq_ctx *c, const kq_attn_layer *l, int M, const
     } else if (int r = kq_attn_decode_async(c, l->cache, &at)) {
         return r;
     }
-    kq_task o{};
-    o.w = l->o;
-    o.rows = hidden;
-    o.dst = x_out;
-    o.dst_stride = hidden;
-    o.residual = x_in;
-    o.res_stride = hidden;
-    return run_gemv(c, &o, 1, M, qd, reinterpret_cast<const __half *>(att), qd, nullptr, nullptr);
+    return run_gemv(c, &o, 1, M, qd, ax, qd, nullptr, nullptr);
 }
 
 // =================================================================== LM head

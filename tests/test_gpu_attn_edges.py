@@ -7,7 +7,9 @@ import pytest
 
 import attn_ref as R
 import npu880_mtk_npu_llm_runtime_b200 as kq
+from npu880_mtk_npu_llm_runtime_b200 import synth
 from test_gpu_attn import SENTINEL, SHAPE, cache_of, close, dev
+from test_gpu_attn_block import HIDDEN, Block
 
 pytestmark = pytest.mark.gpu
 
@@ -313,4 +315,55 @@ def test_counts_left_behind_by_a_call_that_stopped_early(kqctx, D, H, K, n, new)
             ctx.set_option("inject_timeout", 3)
     finally:
         torch.cuda.synchronize()
+        ctx.close()
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+def test_block_refused_for_want_of_scratch_has_done_nothing(kqctx, prefill):
+    """the block's first call of a context in a capture, where an FFN block has left all scratch but attention's: it is
+    refused, and what the graph holds writes neither the cache nor the output"""
+    import torch
+    ctx, stream = kq.Context(0), torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    ctx.set_option("gemv_split", 0)
+    b, ffn = Block(ctx, (12, 14, 12, 12)), 2048
+    x = torch.randn((3, HIDDEN), device="cuda").half()
+    out = torch.full_like(x, SENTINEL)
+    w = [ctx.upload(synth.gen_weights(12, r, c, 50 + i), 12, r, c) for i, (r, c) in enumerate([(ffn, HIDDEN)] * 2 + [(HIDDEN, ffn)])]
+    seq, pos, lens, start = i32(0, 1, 2), i32(4, 5, 6), i32(5, 6, 7), i32(0, 1, 2, 3)
+    ctx.run_ffn_async(*w, 3, x, b.dg[0], torch.empty_like(x))
+    ctx.synchronize()
+    b.ck.fill_(SENTINEL)
+    b.cv.fill_(SENTINEL)
+    torch.cuda.synchronize()
+    try:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            with pytest.raises(kq.KQError):
+                ctx.run_attn_async(b.layer, seq, pos, lens, x, out, q_start=start if prefill else None)
+        with torch.cuda.stream(stream):
+            g.replay()
+        ctx.synchronize()
+        assert (b.ck == SENTINEL).all() and (b.cv == SENTINEL).all() and (out == SENTINEL).all()
+        del g
+        ctx.run_attn_async(b.layer, seq, pos, lens, x, out, q_start=start if prefill else None)   # eagerly it runs
+        ctx.synchronize()
+        want, _ = b.steps(ctx, seq, pos, lens, x, start if prefill else None)
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+        g = torch.cuda.CUDAGraph()                          # and then in a graph
+        with torch.cuda.graph(g, stream=stream):
+            ctx.run_attn_async(b.layer, seq, pos, lens, x, out, q_start=start if prefill else None)
+        out.fill_(SENTINEL)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            g.replay()
+        ctx.synchronize()
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+        del g
+    finally:
+        torch.cuda.synchronize()
+        b.free()
+        for t in w:
+            t.free()
         ctx.close()
