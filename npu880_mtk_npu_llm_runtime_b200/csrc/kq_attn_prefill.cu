@@ -728,6 +728,7 @@ __device__ __forceinline__ void mend_rows(const PrefillParams &p, Shared &sh, co
                                           int lane) {
     uint32_t todo = __ballot_sync(0xffffffffu, odd);
     if (!todo) return;
+    __syncwarp();  // the rows' plain results, stored by a lane each, before other lanes store over them (votes order no memory)
     if (lane == 0) atomicAdd(&sh.mending, 1);
     while (todo) {
         const int src = __ffs(todo) - 1;

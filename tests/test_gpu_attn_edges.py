@@ -367,3 +367,35 @@ def test_block_refused_for_want_of_scratch_has_done_nothing(kqctx, prefill):
         for t in w:
             t.free()
         ctx.close()
+
+
+@pytest.mark.parametrize("D, pad", [(64, 0), (128, 8), (256, 16)])
+def test_rows_stored_twice(kqctx, D, pad):
+    """rows that are computed again (an infinity in one of every row's values, and rows that see nothing) are stored
+    over their plain results by other threads: the second result is the one that stays, every time"""
+    import torch
+    rng = np.random.default_rng(D + pad)
+    n, H = 200, 4
+    p = R.Paged(rng, [n, 5], 2, 16, D)
+    p.values[0][0, :, 7] = np.inf
+    p.v[p.table[0, 0], :, 0, 7] = np.inf
+    rows = n + 40                                          # sequence 1: 35 rows in front of its first key
+    q = rng.standard_normal((rows, H, D)).astype(np.float16)
+    buf = torch.full((rows, H * D + pad), SENTINEL, dtype=torch.float16, device="cuda")
+    out = buf[:, :H * D]
+    a = kq.Attention(cache_of(p), dev(q.reshape(rows, -1)), out, i32(n, 5), q_start=i32(0, n, rows), heads=H)
+    torch.cuda.synchronize()
+    kqctx.attn_prefill_async(a)
+    kqctx.synchronize()
+    first = out.cpu().numpy()
+    got, keep = first.reshape(rows, H, D), np.delete(np.arange(D), 7)
+    p.values[0][0, :, 7] = 0
+    want, tol = R.expect(p, q, [(i, 0, i, n) for i in range(n)] + [(n + i, 1, i - 35, 5) for i in range(40)], 0, 0)
+    close(got[..., keep], want[..., keep], tol[..., keep])
+    assert np.isposinf(got[:n, :, 7]).all() and (got[n:n + 35] == 0).all()
+    for _ in range(30):
+        buf.fill_(SENTINEL)
+        torch.cuda.synchronize()
+        kqctx.attn_prefill_async(a)
+        kqctx.synchronize()
+        assert np.array_equal(out.cpu().numpy().view(np.uint16), first.view(np.uint16))
