@@ -268,8 +268,8 @@ typedef struct kq_kv_cache {
     int table_stride;           /* table entries per sequence; table_stride * page_size <= 2^30, times n_seqs <= 2^34 */
 } kq_kv_cache;
 
-/* One set of heads of M rows: in -> out (the same buffer and stride, or one that does not
- * overlap).  gamma (fp16 [head_dim], or NULL for no norm) scales the RMS-normed head:
+/* One set of heads of M rows: in -> out (the same address and stride, or rows that share no byte with any rows
+ * that the call reads or with the cache; rows between the rows of another set are fine).  gamma (fp16 [head_dim], or NULL for no norm) scales the RMS-normed head:
  * x * gamma / sqrt(mean(x^2) + eps). */
 typedef struct kq_heads {
     const uint16_t *in;
@@ -347,7 +347,7 @@ typedef struct kq_attn_layer {
 } kq_attn_layer;
 /* M rows of x_in / x_out (fp16 [M][hidden]); seq_dev and pos_dev as in kq_kv_append_async, kv_len_dev
  * and q_start_dev as in kq_attn (kv_len counts the appended rows; without q_start row i is sequence i,
- * so seq_dev[i] is i, or -1 with kv_len_dev[i] = 0 for padding).  x_out may not overlap x_in.  A row of no
+ * so seq_dev[i] is i, or -1 with kv_len_dev[i] = 0 for padding).  x_out may not overlap x_in or the cache.  A row of no
  * sequence (such padding, or a row outside the q_start ranges) comes out as it went in.  One eager call
  * at the largest M sizes the scratch; then a call allocates nothing and can be captured into a CUDA
  * graph, which keeps reading x_in, the tables and the lengths where they were.  As for every call of

@@ -1190,6 +1190,7 @@ int attn_launch(kq_ctx *c, const kq_kv_cache *cache, const kq_attn *a, bool pref
     if (!c) return KQ_ERR_INVALID_ARGUMENT;
     const char *why = "";
     if (int r = kq::check_attn(cache, a, prefill, &why)) return fail(c, r, "%s", why);
+    if (int r = kq::check_attn_apart(cache, a, &why)) return fail(c, r, "%s", why);
     L.cache = kv_view(cache);
     L.q = a->q;
     L.q_stride = (long long)a->q_stride;
@@ -1226,6 +1227,7 @@ extern "C" int kq_qk_norm_rope_async(kq_ctx *c, const kq_rope *rope, int head_di
         return fail(c, KQ_ERR_INVALID_ARGUMENT, "positions are NULL or not 4-byte aligned");
     if (!(eps >= 0.0f)) return fail(c, KQ_ERR_INVALID_ARGUMENT, "eps must not be negative");
     if (M == 0 || (!q && !k)) return KQ_OK;
+    if (int e = kq::check_heads_apart(nullptr, head_dim, M, q, k, nullptr, &why)) return fail(c, e, "%s", why);
     const OnDevice on(c->device);
     kq::RopeLaunch L{};
     L.q = q;
@@ -1250,6 +1252,7 @@ extern "C" int kq_kv_append_async(kq_ctx *c, const kq_kv_cache *cache, const kq_
     if (int r = kq::check_append(cache, rope, M, seq, pos, q, k, v, &why)) return fail(c, r, "%s", why);
     if (!(eps >= 0.0f)) return fail(c, KQ_ERR_INVALID_ARGUMENT, "eps must not be negative");
     if (M == 0) return KQ_OK;
+    if (int r = kq::check_heads_apart(cache, cache->head_dim, M, q, k, v, &why)) return fail(c, r, "%s", why);
     const OnDevice on(c->device);
     const kq::KvView view = kv_view(cache);
     kq::RopeLaunch L{};
@@ -1309,6 +1312,9 @@ extern "C" int kq_run_attn_async(kq_ctx *c, const kq_attn_layer *l, int M, const
     if (int r = validate_mk(c, M, qd)) return r;
     const uintptr_t xi = (uintptr_t)x_in, xo = (uintptr_t)x_out, xb = (uintptr_t)M * hidden * 2;
     if (xi < xo + xb && xo < xi + xb) return fail(c, KQ_ERR_INVALID_ARGUMENT, "x_out may not overlap x_in");
+    const kq::Rows xr{x_out, 0, (size_t)xb, 1};
+    if (kq::rows_overlap(xr, kq::pages_of(l->cache, l->cache->k)) || kq::rows_overlap(xr, kq::pages_of(l->cache, l->cache->v)))
+        return fail(c, KQ_ERR_INVALID_ARGUMENT, "x_out may not overlap the cache");
     const OnDevice on(c->device);
     // scratch: xn [M][hidden] | q, k, v rows side by side | attention's output | q8k(xn) | q8_0(xn)
     auto al = [](size_t v) { return (v + 255) & ~(size_t)255; };

@@ -6,6 +6,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 
 #include "../../include/kq.h"
 
@@ -296,6 +297,93 @@ inline int check_attn(const kq_kv_cache *c, const kq_attn *a, bool prefill, cons
     // (256 products of fp16's largest values stay below fp32's with it, so no finite score is lost)
     if (!(a->scale >= 0.0f) || a->scale > 1e24f) {
         *why = "scale must be 0 or a positive number up to 1e24";
+        return KQ_ERR_INVALID_ARGUMENT;
+    }
+    return KQ_OK;
+}
+
+// ---- what a call writes may not lie over what it reads
+
+// n rows of `width` bytes, `stride` bytes apart (stride >= width, or n = 1).
+struct Rows {
+    const void *at;
+    size_t stride, width;
+    int n;
+};
+
+// Do two sets of rows share a byte?  (Rows of one set between rows of the other do not.)
+inline bool rows_overlap(const Rows &a, const Rows &b) {
+    if (!a.n || !b.n || !a.at || !b.at) return false;
+    const long long at = (long long)(uintptr_t)a.at, bt = (long long)(uintptr_t)b.at;
+    const long long as = (long long)a.stride, bs = (long long)b.stride, aw = (long long)a.width, bw = (long long)b.width;
+    if (at + (a.n - 1) * as + aw <= bt || bt + (b.n - 1) * bs + bw <= at) return false;
+    if (a.n == 1 || b.n == 1 || as != bs) {
+        // both in the order of their addresses
+        for (int i = 0, j = 0; i < a.n && j < b.n;) {
+            const long long x = at + i * as, y = bt + j * bs;
+            if (x + aw <= y) ++i;
+            else if (y + bw <= x) ++j;
+            else return true;
+        }
+        return false;
+    }
+    // one stride: row i of a and row i + t of b overlap, for every i, when -bw < d + t s < aw
+    const long long s = as, d = bt - at, least = 1 - bw - d;
+    long long t = least / s + (least % s > 0);  // the smallest t of the first
+    if (t < 1 - a.n) t = 1 - a.n;
+    return t < b.n && d + t * s < aw;
+}
+
+inline Rows rows_of(const uint16_t *p, size_t stride, int heads, int head_dim, int M) {
+    return Rows{p, stride * 2, (size_t)heads * head_dim * 2, M};
+}
+inline Rows pages_of(const kq_kv_cache *c, const uint16_t *p) {
+    return Rows{p, 0, (size_t)c->n_pages * c->kv_heads * c->page_size * c->head_dim * 2, 1};
+}
+
+// The rows of a norm, rotation or append call, checked one by one before.
+inline int check_heads_apart(const kq_kv_cache *c, int head_dim, int M, const kq_heads *q, const kq_heads *k,
+                             const kq_heads *v, const char **why) {
+    *why = "";
+    const kq_heads *h[3] = {q, k, v};
+    for (int i = 0; i < 3; ++i) {
+        if (!h[i] || !h[i]->out) continue;
+        const Rows out = rows_of(h[i]->out, h[i]->out_stride, h[i]->heads, head_dim, M);
+        for (int j = 0; j < 3; ++j) {
+            if (!h[j]) continue;
+            const bool in_place = i == j && h[i]->in == h[i]->out && (M == 1 || h[i]->in_stride == h[i]->out_stride);
+            if (!in_place && rows_overlap(out, rows_of(h[j]->in, h[j]->in_stride, h[j]->heads, head_dim, M))) {
+                *why = "out must be the rows themselves or lie apart from all rows that the call reads";
+                return KQ_ERR_INVALID_ARGUMENT;
+            }
+            if (j < i && h[j]->out && rows_overlap(out, rows_of(h[j]->out, h[j]->out_stride, h[j]->heads, head_dim, M))) {
+                *why = "two sets of heads go to the same place";
+                return KQ_ERR_INVALID_ARGUMENT;
+            }
+        }
+    }
+    if (!c) return KQ_OK;
+    if (rows_overlap(pages_of(c, c->k), pages_of(c, c->v))) {
+        *why = "the cache's keys and values lie over each other";
+        return KQ_ERR_INVALID_ARGUMENT;
+    }
+    for (const uint16_t *pages : {c->k, c->v})
+        for (int i = 0; i < 3; ++i)
+            if (h[i] && (rows_overlap(pages_of(c, pages), rows_of(h[i]->in, h[i]->in_stride, h[i]->heads, head_dim, M)) ||
+                         rows_overlap(pages_of(c, pages), rows_of(h[i]->out, h[i]->out_stride, h[i]->heads, head_dim, M)))) {
+                *why = "rows lie in the cache's pages";
+                return KQ_ERR_INVALID_ARGUMENT;
+            }
+    return KQ_OK;
+}
+
+// The output of an attention call, checked before.
+inline int check_attn_apart(const kq_kv_cache *c, const kq_attn *a, const char **why) {
+    *why = "";
+    const Rows out = rows_of(a->out, a->out_stride, a->heads, c->head_dim, a->M);
+    if (rows_overlap(out, rows_of(a->q, a->q_stride, a->heads, c->head_dim, a->M)) || rows_overlap(out, pages_of(c, c->k)) ||
+        rows_overlap(out, pages_of(c, c->v))) {
+        *why = "out may not overlap q or the cache";
         return KQ_ERR_INVALID_ARGUMENT;
     }
     return KQ_OK;

@@ -399,3 +399,40 @@ def test_rows_stored_twice(kqctx, D, pad):
         kqctx.attn_prefill_async(a)
         kqctx.synchronize()
         assert np.array_equal(out.cpu().numpy().view(np.uint16), first.view(np.uint16))
+
+
+def test_outputs_that_lie_over_inputs_are_refused(kqctx):
+    import torch
+    D, H, K, M = 64, 4, 2, 6
+    rng = np.random.default_rng(3)
+    p = R.Paged(rng, [5] * M, K, 16, D)
+    cache = cache_of(p)
+    rows = torch.randn((M + 1, (H + 2 * K) * D), device="cuda").half()
+    q, k, v = rows[:M, :H * D], rows[:M, H * D:(H + K) * D], rows[:M, (H + K) * D:]
+    free = torch.empty((M, H * D), dtype=torch.float16, device="cuda")
+    lens, seq, pos, rope = i32(*[5] * M), i32(*range(M)), i32(*[4] * M), kq.Rope(D)
+    pages = cache.k.view(-1)
+    over_cache = pages[:M * H * D].view(M, H * D)
+    for out in (rows[1:, :H * D], rows[:M, 8:H * D + 8], over_cache):
+        with pytest.raises(kq.KQError):
+            kqctx.attn_decode_async(kq.Attention(cache, q, out, lens))
+        with pytest.raises(kq.KQError):
+            kqctx.kv_append_async(cache, rope, seq, pos, kq.Heads(k, K), kq.Heads(v, K), q=kq.Heads(q, H, out=out))
+    for bad_q in (kq.Heads(q, H, out=rows[:M, K * D:(H + K) * D]), kq.Heads(q, H, out=free)):
+        with pytest.raises(kq.KQError):
+            kqctx.qk_norm_rope_async(rope, pos, bad_q, kq.Heads(k, K, out=free[:, :K * D]))
+    with pytest.raises(kq.KQError):
+        kqctx.kv_append_async(kq.KvCache(cache.k, cache.k, cache.page_table), rope, seq, pos, kq.Heads(k, K), kq.Heads(v, K))
+    kqctx.synchronize()
+    # in place and between the other rows of the buffer it runs: out over k and v once they are in the cache
+    kqctx.kv_append_async(cache, rope, seq, pos, kq.Heads(k, K), kq.Heads(v, K), q=kq.Heads(q, H, out=q))
+    kqctx.synchronize()
+    hq = q.cpu().numpy().reshape(M, H, D)
+    a = kq.Attention(cache, q, rows[:M, H * D:], lens)
+    kqctx.attn_decode_async(a)
+    kqctx.synchronize()
+    at = p.table[np.arange(M), 0]
+    for s in range(M):
+        p.keys[s], p.values[s] = (t.cpu().numpy()[at[s], :, :5].transpose(1, 0, 2) for t in (cache.k, cache.v))
+    want, tol = R.expect(p, hq, [(s, s, 4, 5) for s in range(M)], 0, 0)
+    close(rows[:M, H * D:].cpu().numpy().reshape(M, H, D), want, tol)
