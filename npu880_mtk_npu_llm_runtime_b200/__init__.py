@@ -224,6 +224,20 @@ def _dp(t):
     return t.data_ptr()
 
 
+def _int32(v, what: str) -> int:
+    """v, where a C int holds it (ctypes would keep its low 32 bits)"""
+    if not -2 ** 31 <= v < 2 ** 31:
+        raise ValueError(f"{what}: {v} is no 32-bit number")
+    return v
+
+
+def _scale(v: float) -> float:
+    """v, unless fp32 makes 0 of it, which stands for 1 / sqrt(head_dim)"""
+    if v != 0 and C.c_float(v).value == 0:
+        raise ValueError(f"scale: {v} is 0 in fp32")
+    return v
+
+
 def _rows(t, what: str, heads: int):
     """(pointer, row stride, head size, rows) of an fp16 tensor [rows, heads * head_dim] (or [rows,
     heads, head_dim]) whose rows may lie apart"""
@@ -235,7 +249,7 @@ def _rows(t, what: str, heads: int):
     width = t.shape[1] if t.dim() == 2 else t.shape[1] * t.shape[2]
     if t.stride(-1) != 1 or heads < 1 or width % heads:
         raise ValueError(f"{what}: rows of {heads} heads with values side by side are needed")
-    stride = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    stride = t.stride(0) if _int32(t.shape[0], what) > 1 else max(t.stride(0), width)
     return t.data_ptr(), stride, width // heads, t.shape[0]
 
 
@@ -254,7 +268,7 @@ class Rope:
 
     def __init__(self, rot_dim: int, base: float = 1e4, style: str = "half", inv_freq=None):
         self.struct = RopeStruct()
-        st = load_library().kq_rope_init(C.addressof(self.struct), rot_dim, self.STYLES[style], base)
+        st = load_library().kq_rope_init(C.addressof(self.struct), _int32(rot_dim, "rot_dim"), self.STYLES[style], base)
         if st != 0:
             raise KQError(st, f"rope of {rot_dim} values, base {base}")
         if inv_freq is not None:
@@ -320,7 +334,7 @@ class Attention:
         s.out, s.out_stride, od, om = _rows(out, "out", heads)
         if (qd, od, om) != (dim, dim, s.M):
             raise ValueError(f"q and out must have the same rows of {heads} heads of {dim}")
-        s.heads, s.window, s.sinks, s.scale = heads, window, sinks, scale
+        s.heads, s.window, s.sinks, s.scale = heads, _int32(window, "window"), _int32(sinks, "sinks"), _scale(scale)
         s.kv_len = _ints(kv_len, "kv_len", cache.index, cache.struct.n_seqs)
         if q_start is not None:
             s.q_start = _ints(q_start, "q_start", cache.index, cache.struct.n_seqs + 1)
@@ -361,8 +375,8 @@ class AttnLayer:
                 raise ValueError(f"{what}: {n} fp16 values side by side on the cache's device are needed")
         s = self.struct = AttnLayerStruct(q=q.handle, k=k.handle, v=v.handle, o=o.handle, gamma=_dp(gamma),
                                           q_gamma=_dp(q_gamma), k_gamma=_dp(k_gamma), rope=rope and rope.ref,
-                                          cache=cache.ref, heads=q.rows // dim, window=window, sinks=sinks, scale=scale,
-                                          eps=eps)
+                                          cache=cache.ref, heads=q.rows // dim, window=_int32(window, "window"),
+                                          sinks=_int32(sinks, "sinks"), scale=_scale(scale), eps=eps)
         self.cache, self.hidden, self.ref, self.weights = cache, q.cols, C.addressof(s), (q, k, v, o)
         self.keep = (gamma, q_gamma, k_gamma, rope)
 

@@ -9,6 +9,9 @@ import subprocess
 import pytest
 
 from conftest import ROOT
+
+import npu880_mtk_npu_llm_runtime_b200 as kq
+from npu880_mtk_npu_llm_runtime_b200 import build as kqbuild
 from test_attn_host import INVALID, attn_struct, cache_struct, heads_struct
 
 SOURCE = r'''
@@ -154,3 +157,18 @@ def test_outputs_over_inputs(host):
     assert attend(q_at, row) == INVALID and attend(q_at + 16, 8 * D) == INVALID
     assert attend((1 << 30) - 2 * 8 * D * M, 8 * D) == 0 and attend((1 << 30) - 2 * 8 * D * M + 16, 8 * D) == INVALID
     assert attend((1 << 31) + size, 8 * D) == 0 and attend((1 << 31) + size - 16, 8 * D) == INVALID
+
+
+def test_numbers_of_32_bits():
+    kqbuild.build()
+    for rot in (2 ** 32 + 64, 2 ** 32, -2 ** 32 + 16):
+        with pytest.raises(ValueError):
+            kq.Rope(rot)
+    assert kq._int32(2 ** 31 - 1, "x") == 2 ** 31 - 1 and kq._int32(-2 ** 31, "x") == -2 ** 31
+    for v in (2 ** 31, -2 ** 31 - 1, 2 ** 64):
+        with pytest.raises(ValueError):
+            kq._int32(v, "x")
+    assert kq._scale(0) == 0 and kq._scale(1e-40) == 1e-40
+    for v in (1e-50, -1e-60):
+        with pytest.raises(ValueError):
+            kq._scale(v)

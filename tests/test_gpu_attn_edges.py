@@ -436,3 +436,24 @@ def test_outputs_that_lie_over_inputs_are_refused(kqctx):
         p.keys[s], p.values[s] = (t.cpu().numpy()[at[s], :, :5].transpose(1, 0, 2) for t in (cache.k, cache.v))
     want, tol = R.expect(p, hq, [(s, s, 4, 5) for s in range(M)], 0, 0)
     close(rows[:M, H * D:].cpu().numpy().reshape(M, H, D), want, tol)
+
+
+def test_numbers_that_do_not_fit_are_refused(kqctx):
+    """2^32 as a window is not 0, nor 1e-50 as a scale the default"""
+    import torch
+    cache = cache_of(R.Paged(np.random.default_rng(0), [5, 5], 2, 16, 64))
+    q = torch.zeros((2, 256), dtype=torch.float16, device="cuda")
+    lens = i32(5, 5)
+    for bad in (dict(window=2 ** 32), dict(window=2 ** 31), dict(window=4, sinks=2 ** 32), dict(scale=1e-50)):
+        with pytest.raises(ValueError):
+            kq.Attention(cache, q, torch.empty_like(q), lens, **bad)
+    b = Block(kqctx)
+    for bad in (dict(window=2 ** 32), dict(window=4, sinks=-2 ** 32 - 1), dict(scale=-1e-50)):
+        with pytest.raises(ValueError):
+            kq.AttnLayer(*b.w, b.dg[0], b.cache, **bad)
+    with pytest.raises(ValueError):                          # (rows that a stride of 0 makes)
+        kq.Heads(q[:1].expand(2 ** 32, 256), 2)
+    a = kq.Attention(cache, q, torch.empty_like(q), lens, window=2 ** 31 - 1, sinks=2 ** 31 - 1, scale=1e-40)
+    kqctx.attn_decode_async(a)
+    kqctx.synchronize()
+    b.free()
