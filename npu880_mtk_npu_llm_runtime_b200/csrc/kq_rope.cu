@@ -125,8 +125,8 @@ __global__ __launch_bounds__(kThreads, kCtasPerSm) void kq_norm_rope(const __gri
         {
             uint4 ga = make_uint4(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u), gb = ga;  // ones
             if (s.gamma) {
-                ga = __ldg(reinterpret_cast<const uint4 *>(s.gamma + 8 * l));
-                gb = __ldg(reinterpret_cast<const uint4 *>(s.gamma + 8 * (src % LPH)));
+                ga = *reinterpret_cast<const uint4 *>(s.gamma + 8 * l);
+                gb = *reinterpret_cast<const uint4 *>(s.gamma + 8 * (src % LPH));
             }
             const uint32_t aw[4] = {ga.x, ga.y, ga.z, ga.w}, bw[4] = {gb.x, gb.y, gb.z, gb.w};
 #pragma unroll
