@@ -182,6 +182,15 @@ int validate_mk(kq_ctx *c, int M, int K) {
     return KQ_OK;
 }
 
+// Whether the stream is being captured.  A clearing enqueued into a capture has only been recorded: counts stay as
+// they are, and their buffer dirty, until an eager call clears them.
+int capturing(kq_ctx *c, bool &yes) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    KQ_CUDA(c, cudaStreamIsCapturing(c->stream, &cap));
+    yes = cap != cudaStreamCaptureStatusNone;
+    return KQ_OK;
+}
+
 // Scratch of a balanced GEMV launch (CTAs own equal tile ranges; see GemvParams::split).  The
 // launch keeps whole row groups per CTA when the option is off or the term slots would exceed
 // 64 MB (very long Q8_0 rows).
@@ -195,9 +204,9 @@ int split_counts(kq_ctx *c, size_t extra = 0, bool size_only = false) {
         c->split_dirty = true;
     }
     if (!c->split_dirty || size_only) return KQ_OK;
-    KQ_CUDA(c, cudaMemsetAsync(c->gcount.p, 0, cb, c->stream));
-    c->split_dirty = false;
-    return KQ_OK;
+    // all of it (a launch before may have used more than this one), and done only once it has run: see capturing
+    KQ_CUDA(c, cudaMemsetAsync(c->gcount.p, 0, c->gcount.cap, c->stream));
+    return capturing(c, c->split_dirty);
 }
 
 int gemv_split_scratch(kq_ctx *c, int type, int K, int mt, kq::GemvLaunch &L, bool size_only) {
@@ -1175,10 +1184,7 @@ int attn_scratch(kq_ctx *c, kq::AttnLaunch &L) {
     if (int r = attn_memory(c)) return r;
     if (c->attn_dirty) {
         KQ_CUDA(c, cudaMemsetAsync(c->attn_count.p, 0, c->attn_count.cap, c->stream));
-        // a capture has only recorded it: the counts stay as they are until the graph runs
-        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-        KQ_CUDA(c, cudaStreamIsCapturing(c->stream, &cap));
-        c->attn_dirty = cap != cudaStreamCaptureStatusNone;
+        if (int r = capturing(c, c->attn_dirty)) return r;
     }
     L.parts = static_cast<float *>(c->attn_parts.p);
     L.count = static_cast<unsigned *>(c->attn_count.p);

@@ -2,6 +2,8 @@
 against the plain 64-bit forms (attn_ref)."""
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -457,3 +459,61 @@ def test_numbers_that_do_not_fit_are_refused(kqctx):
     kqctx.attn_decode_async(a)
     kqctx.synchronize()
     b.free()
+
+
+@pytest.mark.parametrize("what", ["products", "attention"])
+def test_clearing_that_a_capture_only_records(kqctx, what):
+    """after a call that stopped early every capture clears the arrival counts, until an eager call has done so"""
+    import torch
+    ctx, stream = kq.Context(0), torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    rows, K, n = 300, 4096, 300
+    w = ctx.upload(synth.gen_weights(12, rows, K, seed=5), 12, rows, K)
+    x, y = torch.randn((2, K), device="cuda").half(), torch.zeros((2, rows), dtype=torch.float16, device="cuda")
+    p = R.Paged(np.random.default_rng(1), [n], 2, 16, 128)
+    q = torch.randn((n, 4 * 128), device="cuda").half()
+    a = kq.Attention(cache_of(p), q, torch.empty_like(q), i32(n), q_start=i32(0, n))
+
+    def call():
+        if what == "products":
+            ctx.gemm_multi_async(x, 2, K, [dict(w=w, dst=y)])
+        else:
+            ctx.attn_prefill_async(a)
+
+    def clears():
+        """whether a capture of the call holds a memset"""
+        g = torch.cuda.CUDAGraph(keep_graph=True)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=stream):
+            call()
+        graph, n, cu = C.c_void_p(g.raw_cuda_graph()), C.c_size_t(), C.CDLL("libcuda.so.1")
+        assert cu.cuGraphGetNodes(graph, None, C.byref(n)) == 0 and n.value > 0
+        nodes, kind = (C.c_void_p * n.value)(), C.c_int()
+        assert cu.cuGraphGetNodes(graph, nodes, C.byref(n)) == 0
+        kinds = []
+        for node in nodes:
+            assert cu.cuGraphNodeGetType(C.c_void_p(node), C.byref(kind)) == 0
+            kinds.append(kind.value)
+        return 2 in kinds                                  # CU_GRAPH_NODE_TYPE_MEMSET
+
+    try:
+        torch.cuda.synchronize()
+        call()
+        ctx.synchronize()
+        assert not clears()
+        ctx.set_option("timeout_ms", 20)
+        ctx.set_option("inject_timeout", 1)
+        call()
+        with pytest.raises(kq.KQError) as e:
+            ctx.synchronize()
+        assert e.value.status == -7
+        ctx.set_option("inject_timeout", 0)
+        ctx.set_option("timeout_ms", 1000)
+        assert clears() and clears()
+        call()
+        ctx.synchronize()
+        assert not clears()
+    finally:
+        torch.cuda.synchronize()
+        w.free()
+        ctx.close()
