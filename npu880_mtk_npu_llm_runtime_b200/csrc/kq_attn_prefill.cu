@@ -31,6 +31,7 @@
 // block and 2.5 in each item's epilogue; a block takes 1.75 us at 1.9 GHz, 0.6 of it MMAs that the
 // tile's own softmax waits for.
 #include "kq_attn_dev.cuh"
+#include "kq_tcgen05.cuh"
 
 #include <cuda.h>
 #include <mutex>
@@ -106,9 +107,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
         "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(0), "r"(kDescHi));
 }
-__device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap *m, int x, int y, int z, int w, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
@@ -121,40 +119,12 @@ __device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *m, int x, 
         "l"(m), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *r) {
-    uint32_t *u = reinterpret_cast<uint32_t *>(r);
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
-          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
-          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
-          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-        : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
-}
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ bool elect_one() {
-    uint32_t pred;
-    asm volatile("{ .reg .pred P; elect.sync _|P, 0xffffffff; selp.u32 %0, 1, 0, P; }" : "=r"(pred));
-    return pred != 0;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -617,7 +587,7 @@ __device__ __forceinline__ void load_role(const PrefillParams &p, Shared &sh, co
 #pragma unroll
                     for (int c = 0; c < CH; ++c)
                         *reinterpret_cast<uint4 *>(to + c * (BN * 128) + e * 16) = make_uint4(0, 0, 0, 0);
-                fence_async();
+                fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&full));
             }
@@ -656,7 +626,7 @@ __device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, con
         for (int e = 0; e < D / 16; ++e)
             mma_ss(tmem + slot * C::S_COL, qb + (e / 4) * (128 * 128 / 16) + (e % 4) * 2, kb + (e / 4) * (BN * 128 / 16) + (e % 4) * 2,
                    C::IDESC_S, e > 0);
-        commit(smem_u32(&sh.s_full[slot]));
+        tc_commit(smem_u32(&sh.s_full[slot]));
     };
     // O tile t (+)= half h of the slot's P times its keys' rows of the V block in ring stage st
     auto mma_o = [&](int t, int slot, uint32_t st, bool first, int h) {
@@ -692,24 +662,24 @@ __device__ __forceinline__ void mma_role(const PrefillParams &p, Shared &sh, con
                 const int slot = NT == 2 ? t : j & 1;
                 if (j >= 0) {
                     if (!wait_p(slot, 0)) return;
-                    fence_after();
+                    tc_fence_after();
                     if (elect_one()) mma_o(t, slot, v, j == 0, 0);
                     __syncwarp();
                     if (!wait_p(slot, 1)) return;
                 }
-                fence_after();
+                tc_fence_after();
                 if (elect_one()) {
                     if (j >= 0) {
                         mma_o(t, slot, v, false, 1);
-                        if (j == nb - 1) commit(smem_u32(&sh.o_full[t]));
-                        else if (NT == 1) commit(smem_u32(&sh.pv_done));
-                        if (t == subs - 1) commit(smem_u32(&sh.v_empty[v]));
+                        if (j == nb - 1) tc_commit(smem_u32(&sh.o_full[t]));
+                        else if (NT == 1) tc_commit(smem_u32(&sh.pv_done));
+                        if (t == subs - 1) tc_commit(smem_u32(&sh.v_empty[v]));
                     }
                     if (js < nb) {
                         mma_s(t, slot, kk);
                         if (t == subs - 1) {
-                            commit(smem_u32(&sh.k_empty[kk]));
-                            if (js == nb - 1) commit(smem_u32(&sh.q_empty));
+                            tc_commit(smem_u32(&sh.k_empty[kk]));
+                            if (js == nb - 1) tc_commit(smem_u32(&sh.q_empty));
                         }
                     }
                 }
@@ -811,11 +781,11 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                 const bool full = j0 + BN <= all_hi && (j0 >= all_lo || j0 + BN <= all_kept);
                 if (!wait(sh.s_full[slot], ns[slot] & 1)) return;
                 ++ns[slot];
-                fence_after();
+                tc_fence_after();
                 float x[BN];
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_base + 32 * c, x + 32 * c);
-                wait_ld();
+                for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_base + 32 * c, reinterpret_cast<uint32_t *>(x + 32 * c));
+                tmem_wait_ld();
                 if (!full) {
 #pragma unroll
                     for (int c = 0; c < BN / 32; ++c) {
@@ -846,13 +816,13 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                         if (NT == 1) {
                             // S of this block only tells that P V of the block before the last is done
                             if (!wait(sh.pv_done, (npv + (i - b0) - 1) & 1)) return;
-                            fence_after();
+                            tc_fence_after();
                         }
 #pragma unroll 1
                         for (int c = 0; c < D / 16; ++c) {
                             uint32_t o[16];
                             tmem_ld16(o_base + 16 * c, o);
-                            wait_ld();
+                            tmem_wait_ld();
 #pragma unroll
                             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
                             tmem_st16(o_base + 16 * c, o);
@@ -877,8 +847,8 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
                         }
                         tmem_st16(s_base + 16 * c, h);
                     }
-                    wait_st();
-                    fence_before();
+                    tmem_wait_st();
+                    tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&sh.p_ready[slot][half]));
                 }
@@ -887,15 +857,15 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
             if (!wait(sh.o_full[t], no & 1)) return;
             ++no;
             npv += b1 - b0 - 1;
-            fence_after();
+            tc_fence_after();
             const bool bad = *reinterpret_cast<const volatile int *>(&s.bad) != 0;
             if (whole) {
                 float2 odd = make_float2(0.0f, 0.0f);
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     float o[32];
-                    tmem_ld32(o_base + 32 * c, o);
-                    wait_ld();
+                    tmem_ld32(o_base + 32 * c, reinterpret_cast<uint32_t *>(o));
+                    tmem_wait_ld();
                     put32(o, 1.0f / l, out + 32 * c, mine, p.wide, odd);
                 }
                 mend_rows<D>(p, sh, s, mine && (bad || coarse || m == -INFINITY || (l == l && !(odd.x + odd.y == 0.0f))), tok, head, lane);
@@ -905,8 +875,8 @@ __device__ __forceinline__ void softmax_role(const PrefillParams &p, Shared &sh,
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     float o[32];
-                    tmem_ld32(o_base + 32 * c, o);
-                    wait_ld();
+                    tmem_ld32(o_base + 32 * c, reinterpret_cast<uint32_t *>(o));
+                    tmem_wait_ld();
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         if (mine) part[(8 * c + e) * part_rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
@@ -1082,10 +1052,10 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
     }
     pdl_wait();
     make_plan<D>(p, sh, seq_tiles, order, *reinterpret_cast<PlanScratch *>(s_k));
-    fence_async();  // the ring's memory goes from the plan to the TMA
-    fence_before();
+    fence_async_smem();  // the ring's memory goes from the plan to the TMA
+    tc_fence_before();
     __syncthreads();
-    fence_after();
+    tc_fence_after();
     const uint32_t tmem = sh.tmem;
     const Waiter wait{sh, p.timeout_ns, a.status};
 
@@ -1106,7 +1076,7 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
             __syncwarp();
             if (*reinterpret_cast<volatile int *>(&sh.abort)) {
                 // let the MMAs in flight end before the accumulators go (bounded)
-                if (elect_one()) commit(smem_u32(&sh.never));
+                if (elect_one()) tc_commit(smem_u32(&sh.never));
                 __syncwarp();
                 const uint64_t t0 = global_timer_ns();
                 while (!mbar_test_wait(smem_u32(&sh.never), 0) && global_timer_ns() - t0 < 2000000ull) {
@@ -1118,7 +1088,7 @@ __global__ __launch_bounds__(kThreads, 1) void kq_attn_prefill(const __grid_cons
         if (warp < C::SOFTMAX_WARPS) softmax_role<D>(p, sh, wait, tmem);
     }
     __syncwarp();
-    fence_before();
+    tc_fence_before();
     __syncthreads();
     if (warp == kWarpMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
