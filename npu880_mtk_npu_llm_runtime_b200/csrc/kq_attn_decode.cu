@@ -5,7 +5,8 @@
 // M = max(m, m'), l 2^(m - M) + l' 2^(m' - M), and o likewise.
 //
 // Bound by the cache's bytes: every visible key and value once, 4 D bytes for 4 D G operations
-// (G query heads share a key head).  So the work is cut by bytes: a unit is 16 keys of one
+// (G query heads share a key head; of heads of 256 the registers hold 8 at a time, so with more of them a key head is
+// two items, and its bytes come twice: see below).  So the work is cut by bytes: a unit is 16 keys of one
 // (sequence, key head) item, the units of all items stand in one row, and every CTA (one per SM)
 // and in it every warp takes an equal, contiguous range of them -- few or many sequences, equal
 // or ragged, load the SMs alike.  A warp works alone, without shared memory or barriers, and keeps
@@ -22,9 +23,12 @@
 //   keys of a dimension with byte permutes; P^T's fragment is S^T's transposed by movmatrix.
 // tcgen05 has nothing to add here: the tensor pipe (8.7% busy) idles either way while the bytes come in.
 //
-// 4 sequences x 131,072 keys, 8 key heads of 128 (2.15 GB): 331 us, 6.5 TB/s, 0.99 of a measured copy;
-// 64 sequences of 1..8,192 keys (239 MB): 49 us, of which 38 stream; 1 x 1,000 keys: 10 us, six dependent
+// 4 sequences x 131,072 keys, 8 key heads of 128 (2.15 GB): 327-346 us from box to box, 6.2-6.5 TB/s, 0.95-0.99 of a
+// measured copy; 64 sequences of 1..8,192 keys (239 MB): 49 us, of which 38 stream; 1 x 1,000 keys: 10 us, six dependent
 // memory latencies and the launch.  16 x 8,192 keys read 1.0004 x their bytes from DRAM.
+// Heads of 256, 4 key heads, 65,536 keys (268 MB): 57 us with 4 query heads a key head, 62 with 8 (4.4 TB/s; 8 warps an SM,
+// 255 registers and 68 bytes of spills), 83 with 16: the two items of a key head are read at the same time, so DRAM gives 1.01 x the
+// bytes and L2 the second copy.
 #include "kq_attn_dev.cuh"
 
 #include <mutex>

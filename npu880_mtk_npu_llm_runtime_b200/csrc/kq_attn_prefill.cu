@@ -26,9 +26,9 @@
 // in order by the last of them (in two steps where they are many), no finer than the joins pay for
 // (make_plan).
 //
-// 512 rows behind 32,256 keys, 32 / 8 heads of 128: 283 us, 970 TFLOP/s, at the power cap (1.47 GHz); tensor
-// pipe and exponential unit 60% busy.  A 2,048-token prompt: 43 us, of which 3.3 pass before the first
-// block and 2.5 in each item's epilogue; a block takes 1.75 us at 1.9 GHz, 0.6 of it MMAs that the
+// 512 rows behind 32,256 keys, 32 / 8 heads of 128: 279-295 us from box to box, 920-980 TFLOP/s, at the power cap
+// (1.47 GHz); tensor pipe and exponential unit 60% busy.  A 2,048-token prompt: 42-45 us, of which 3.3 pass before
+// the first block and 2.5 in each item's epilogue; a block takes 1.75 us at 1.9 GHz, 0.6 of it MMAs that the
 // tile's own softmax waits for.
 #include "kq_attn_dev.cuh"
 #include "kq_tcgen05.cuh"
@@ -53,9 +53,15 @@ constexpr float kCoarse = 1048576.0f;
 constexpr int kThreads = 384;  // 8 softmax warps, MMA, K and Q loads, V loads, one idle
 constexpr int kWarpMma = 8, kWarpK = 9, kWarpV = 10;
 constexpr int kSortTiles = 512;
-// A join costs about as much as this many blocks: whole items unless the longest is that much
-// longer than an even share.
+// Both sides of the plan's choices are counted in blocks.  A block takes about as long for every head size: 512
+// rows behind 32,256 keys give 1.8, 2.7 (at the power cap; 1.75 else) and 1.7 us a block of a CTA for heads of 64, 128
+// and 256 (whose blocks are half as many keys).
+// What splitting an item costs beside the blocks, its last part's wait for the others and the join, is about this
+// many of them: whole items unless the fullest CTA gets that much more than an even share.
 constexpr int kJoinBlocks = 8;
+// What one part more costs, when the number of parts is chosen: R D / 54,000 + 0.17 blocks for R rows (256 rows of
+// 128: 0.78, or 1.4 us, where the join reads such a part in 1.5 to 2).
+constexpr float kPartValues = 54000.0f, kPartLatency = 0.17f;
 constexpr int kJoinAhead = 3;  // parts whose values a join has on their way at once
 // Parts are joined in two steps where there are more than kOneStep and together more than kOneStepRows rows (18
 // parts of 128 rows 68 us against 59, of 256 rows 74 against 63; but 18 of 32 rows 45.4 against 46.9, 12 of
@@ -398,7 +404,7 @@ __device__ __forceinline__ void make_plan(const PrefillParams &p, Shared &sh, in
         sum += s.nb;
         most = max(most, s.nb);
         // an item's blocks times what joining a part of it costs, in blocks: its rows' bytes and a latency
-        split = fmaxf(split, s.nb * (s.n_tok * p.group * (D / 54000.0f) + 0.17f));
+        split = fmaxf(split, s.nb * (s.n_tok * p.group * (D / kPartValues) + kPartLatency));
     }
     {
         const long long warp_sum = sum_of_warp(sum);

@@ -51,9 +51,10 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __
 // value z of its pair: y = (x A + z B) / sqrt(mean(x^2) + eps), so a head costs little more than
 // its loads, conversions and the sum of squares.
 //
-// Bound by the bytes, 2 in and 2 out per value, and close behind by the instructions.  4,096 rows of
-// 40 heads of 128 (84 MB): 19 us, 4.4 TB/s; a CTA per row that applied gamma, cos and sin to every
-// head took 29; 6 CTAs an SM (more registers, but a second wave of 0.15) 24; batches of 2 passes 20.
+// Bound by the bytes, 2 in and 2 out per value.  4,096 rows of 40 heads of 128 (84 MB): 19 us, 4.4 TB/s; a CTA per row that
+// applied gamma, cos and sin to every head took 29; 6 CTAs an SM (more registers, but a second wave of 0.15) 24; batches
+// of 2 passes 20.  7 CTAs an SM leave 72 registers a thread, 5 or 6 fewer than the batch ahead wants (20-24 bytes spilled,
+// 68-72 loaded again a thread): less than the second wave costs.
 template <int D>
 __global__ __launch_bounds__(kThreads, kCtasPerSm) void kq_norm_rope(const __grid_constant__ RopeParams p) {
     constexpr int LPH = D / 8, HPP = 32 / LPH;
