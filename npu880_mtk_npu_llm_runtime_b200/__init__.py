@@ -585,7 +585,9 @@ class Context:
         self.check(self.L.kq_run_ffn_async(self.handle, gate.handle, up.handle, down.handle, M, _dp(x_dev),
                                            _dp(gamma_dev), _dp(out_dev)))
 
-    # ---- attention over a paged cache (kq_rope, kq_kv_cache, kq_heads, kq_attn)
+    # ---- attention over a paged cache (kq_rope, kq_kv_cache, kq_heads, kq_attn).  The calls are enqueued: their
+    # objects, which keep the tensors, have to live until the context's stream has passed them (a tensor freed
+    # before goes to the next allocation on its own stream)
     def _here(self, *objects):
         for o in objects:
             if o is not None and o.index != self.device:

@@ -23,7 +23,7 @@
 //   keys of a dimension with byte permutes; P^T's fragment is S^T's transposed by movmatrix.
 // tcgen05 has nothing to add here: the tensor pipe (8.7% busy) idles either way while the bytes come in.
 //
-// 4 sequences x 131,072 keys, 8 key heads of 128 (2.15 GB): 327-346 us from box to box, 6.2-6.5 TB/s, 0.95-0.99 of a
+// 4 sequences x 131,072 keys, 8 key heads of 128 (2.15 GB): 327-346 us from run to run, 6.2-6.5 TB/s, 0.95-0.99 of a
 // measured copy; 64 sequences of 1..8,192 keys (239 MB): 49 us, of which 38 stream; 1 x 1,000 keys: 10 us, six dependent
 // memory latencies and the launch.  16 x 8,192 keys read 1.0004 x their bytes from DRAM.
 // Heads of 256, 4 key heads, 65,536 keys (268 MB): 57 us with 4 query heads a key head, 62 with 8 (4.4 TB/s; 8 warps an SM,

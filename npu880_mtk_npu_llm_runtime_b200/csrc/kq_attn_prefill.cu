@@ -26,7 +26,7 @@
 // in order by the last of them (in two steps where they are many), no finer than the joins pay for
 // (make_plan).
 //
-// 512 rows behind 32,256 keys, 32 / 8 heads of 128: 279-295 us from box to box, 920-980 TFLOP/s, at the power cap
+// 512 rows behind 32,256 keys, 32 / 8 heads of 128: 279-295 us from run to run, 920-980 TFLOP/s, at the power cap
 // (1.47 GHz); tensor pipe and exponential unit 60% busy.  A 2,048-token prompt: 42-45 us, of which 3.3 pass before
 // the first block and 2.5 in each item's epilogue; a block takes 1.75 us at 1.9 GHz, 0.6 of it MMAs that the
 // tile's own softmax waits for.
@@ -719,8 +719,9 @@ __device__ __forceinline__ void mend_rows(const PrefillParams &p, Shared &sh, co
 }
 
 // 32 values of a row, times `by`, rounded, to out (where `write`).  `odd` turns NaN when one is not
-// finite (0 times it is NaN); such a row is computed again, so its infinities need not be kept here.  With rows that allow it 32 bytes a store: a warp's lanes write to 32
-// rows, so a 16-byte store would fill half a sector at each.
+// finite (0 times it is NaN); such a row is computed again, so its infinities need not be kept here.
+// With rows that allow it 32 bytes a store: a warp's lanes write to 32 rows, so a 16-byte store would
+// fill half a sector at each.
 __device__ __forceinline__ void put32(const float *o, float by, uint16_t *out, bool write, bool wide, float2 &odd) {
     uint32_t h[16];
     const float2 by2 = make_float2(by, by), zero = make_float2(0.0f, 0.0f);
